@@ -307,6 +307,117 @@ int iq4xs_mul_mat_noalloc(const void* W, const float* X, float* Y, int64_t K, in
 int iq4xs_mul_mat_fused(const void* W, const float* X, float* Y, int64_t K, int64_t N, int64_t M, int layout,
                         int32_t* S, void* stream);
 
+/* ===================== the attention half of a layer =====================
+ * What runs between the q/k/v projections and o: norm and position rotation of
+ * queries and keys, a paged key/value cache, and attention over it.  No
+ * counterpart in the reference, which leaves these ops to stock ggml.  The
+ * calls allocate nothing, never synchronise and may be captured.
+ * head_dim is 64, 128 or 256 (IQ4XS_ERROR_NOT_SUPPORTED otherwise); every
+ * pointer is 16-byte aligned; token strides are in elements and multiples of 8,
+ * a token's heads lie one after another. */
+
+/* Element types */
+#define IQ4XS_TYPE_F32 0
+#define IQ4XS_TYPE_F16 1
+#define IQ4XS_TYPE_BF16 2
+#define IQ4XS_TYPE_Q8 3 /* int8 codes, one fp16 scale for each 32 channels; caches only */
+
+/* Which channels turn together: i and i + rot/2, or 2i and 2i + 1 */
+#define IQ4XS_ROPE_HALF 0
+#define IQ4XS_ROPE_INTERLEAVED 1
+
+/* Key and value pages [pages][heads][page][head_dim] and, for IQ4XS_TYPE_Q8,
+ * their scales [pages][heads][page][head_dim/32] (NULL otherwise).  page, the
+ * tokens of a page, is a power of two of at least 16; pages * page < 2^31.  The
+ * token at slot s lies in page s / page at s % page. */
+struct iq4xs_kv_cache {
+    void* k;
+    void* v;
+    void* k_scales;
+    void* v_scales;
+    int64_t pages;
+    int32_t heads;
+    int32_t page;
+    int32_t head_dim;
+    int32_t type; /* IQ4XS_TYPE_F16, _BF16 or _Q8 */
+};
+
+struct iq4xs_qk_norm_rope_args {
+    const void* q; /* [tokens][q_heads][head_dim], in_type */
+    const void* k; /* [tokens][k_heads][head_dim], in_type */
+    const void* v; /* as k; iq4xs_qk_norm_rope_append only */
+    int64_t q_stride, k_stride, v_stride;
+    const int32_t* pos;   /* [tokens] */
+    const double* freqs;  /* [rot/2] radians for each position (scaling for long contexts included) */
+    const float* q_gamma; /* [head_dim], or NULL */
+    const float* k_gamma;
+    const int64_t* slots; /* [tokens]; iq4xs_qk_norm_rope_append only */
+    void* q_out;          /* [tokens][q_heads][head_dim], out_type */
+    void* k_out;          /* as k; iq4xs_qk_norm_rope only */
+    int64_t tokens;
+    int32_t q_heads, k_heads, head_dim;
+    int32_t rot;  /* channels that turn: a multiple of 16, 0 to head_dim */
+    int32_t rope; /* IQ4XS_ROPE_* */
+    int32_t in_type, out_type;
+    float eps;
+};
+
+/* For each head of q and k: y = x * rsqrt(mean(x^2) + eps) * gamma, then the
+ * first rot channels turned: (a, b) -> (a cos t - b sin t, b cos t + a sin t)
+ * with t = pos * freqs[i] for pair i.  fp32 throughout (t in 64 bits), rounded
+ * once.  tokens == 0 launches nothing. */
+int iq4xs_qk_norm_rope(const struct iq4xs_qk_norm_rope_args* args, void* stream);
+
+/* The same, with k and v (v as it is) written to the cache at slots; a token
+ * whose slot is negative or past the cache is not stored.  Two tokens of a call
+ * must not share a slot.  IQ4XS_TYPE_Q8: for each 32 channels
+ * d = fp16(min(amax / 127, 65504 / 127)), codes = rint(x / d) within +-127;
+ * a NaN makes its group's scale NaN. */
+int iq4xs_qk_norm_rope_append(const struct iq4xs_qk_norm_rope_args* args, const struct iq4xs_kv_cache* cache,
+                              void* stream);
+
+/* Cached tokens as dense rows: row starts[s] + j of k_out and v_out
+ * [total][heads][head_dim] (out_type) is token j of sequence s, at page
+ * table[s * table_width + j / page].  starts has seqs + 1 entries that never
+ * fall.  Rows outside every sequence, and those whose page is past the table or
+ * not in the cache, are zero.  Every element of the cache is read as stored,
+ * rounded once where out_type is narrower. */
+int iq4xs_kv_gather(const struct iq4xs_kv_cache* cache, const int32_t* table, int64_t table_width,
+                    const int32_t* starts, int64_t seqs, void* k_out, void* v_out, int64_t total, int out_type,
+                    void* stream);
+
+struct iq4xs_paged_attention_args {
+    const void* q; /* [total][q_heads][head_dim]; the cache's type, or F16/BF16 for a Q8 cache */
+    void* out;     /* [total][q_heads][head_dim], out_type */
+    float* lse;    /* [total][q_heads], or NULL */
+    const struct iq4xs_kv_cache* cache;
+    const int32_t* table;  /* [seqs][table_width] pages of each sequence; entries past its tokens are not read */
+    const int32_t* starts; /* [seqs + 1] first row of each sequence in q, never falling, the last at most total */
+    const int32_t* kv_len; /* [seqs] cached tokens, the new ones among them */
+    int64_t q_stride, table_width, seqs, total;
+    int64_t most_q, most_kv; /* at least the new and the cached tokens of any sequence */
+    int64_t window;          /* 0: none */
+    int32_t q_heads;         /* a multiple of the cache's heads: head h reads cache head h / (q_heads / heads) */
+    int32_t type;            /* of q */
+    int32_t out_type;        /* F32, F16 or BF16 */
+    int32_t causal;
+    float scale;
+};
+
+/* Bytes of workspace iq4xs_paged_attention needs; 0 also for arguments it refuses. */
+size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args);
+
+/* out = softmax(scale * q k^T over the visible keys) v, lse = log(sum(exp(scale
+ * * q k^T))) (natural).  New token i of a sequence stands at p = kv_len - new + i
+ * and sees key j < kv_len if j <= p (causal) and j > p - window (window > 0).  A
+ * row that sees nothing gives zeros and -Inf.  Keys and values that a row does
+ * not see (and all that lies past kv_len) do not reach it, whatever they hold.
+ * Scores, statistics and sums are fp32; weights are rounded to the type of q, or
+ * fp16 for a Q8 cache, for their product with the values.  Tokens on a page that is
+ * not in the cache are as masked ones.  Where kv_len is above most_kv or the
+ * table, the first keys count; rows past most_q are not written.  The same call gives the same bits. */
+int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
+
 /* ================================ debug exports ================================
  * No counterpart in the reference; they exist so the Q8_1 blocks and the
  * per-32-element int32 sums can be checked bit for bit. */

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libiq4xs_mi355x.so"
@@ -37,6 +38,12 @@ PATH_AUTO = -1
 PATH_GEMV = 0
 PATH_GEMM = 1
 GEMV_MAX_COLS = 8
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+TYPE_Q8 = 3
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
 
 # (restype, argtypes) of every exported symbol, in header order
 _P = ctypes.c_void_p
@@ -76,6 +83,11 @@ SIGNATURES = {
     "iq4xs_swiglu_q8_1": (_INT, [_P, _P, _I64, _I64, _P, ctypes.c_size_t, _P]),
     "iq4xs_rms_norm_mul_mat_group": (_INT, [_INT, _P, _P, _P, _P, _P, _P, _P, ctypes.c_float, _I64, _P]),
     "iq4xs_rms_norm_mul_mat_swiglu": (_INT, [_P, _P, _I64, _P, _P, _P, _P, ctypes.c_float, _I64, _P, _P, _P, _P]),
+    "iq4xs_qk_norm_rope": (_INT, [_P, _P]),
+    "iq4xs_qk_norm_rope_append": (_INT, [_P, _P, _P]),
+    "iq4xs_kv_gather": (_INT, [_P, _P, _I64, _P, _I64, _P, _P, _I64, _INT, _P]),
+    "iq4xs_paged_attention_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "iq4xs_paged_attention": (_INT, [_P, _P, ctypes.c_size_t, _P]),
     "iq4xs_q8_1_to_blocks": (_INT, [_P, _P, _I64, _I64, _P]),
     "iq4xs_subblock_sums": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _INT, _P]),
     "iq4xs_probe_mfma_i8": (_INT, [_P, _P, _P, _P]),
@@ -311,6 +323,192 @@ def dequant(W, n_blocks: int, out=None):
     out = torch.empty(n_blocks * QK_K, dtype=torch.float32, device=W.device) if out is None else out
     lib().check("dequant_iq4xs_gpu", W.data_ptr(), out.data_ptr(), n_blocks, 64, _stream(torch))
     return out
+
+
+# ---------------------------------------------------------------------------
+# the attention half of a layer: argument structs are packed in the header's order
+
+_CACHE = struct.Struct("@PPPPqiiii")
+_QK = struct.Struct("@PPPqqqPPPPPPPqiiiiiiif")
+_ATTENTION = struct.Struct("@PPPPPPPqqqqqqqiiiif")
+
+
+def _types(torch):
+    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def _rows(t, name: str, heads: int | None = None, d: int | None = None):
+    """Shape and token stride of [tokens][heads][head] whose heads lie one after another."""
+    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
+        raise ValueError(f"{name} must be [tokens, heads, head] with a token's heads one after another")
+    if (heads is not None and t.size(1) != heads) or (d is not None and t.size(2) != d):
+        raise ValueError(f"{name} must be [tokens, {heads}, {d}]")
+    # the stride of a single token says nothing
+    return t.size(0), t.size(1), t.size(2), t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+
+
+def _whole(t, name: str, dtype, *shape) -> int:
+    """Address of a contiguous tensor of that type and shape."""
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
+    return t.data_ptr()
+
+
+def _one_device(torch, *tensors) -> None:
+    """The calls launch on the current device."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError("every tensor must be on the current GPU")
+
+
+class KVCache:
+    """Key and value pages [pages, heads, page, head] in fp16, bf16 or as int8 codes, these with fp16 scales
+    [pages, heads, page, head / 32].  Holds the tensors; the calls below read and write them in place.
+
+    page is a power of two of at least 16; head is 64, 128 or 256.  The token at slot s lies in page s // page."""
+
+    def __init__(self, k_pages, v_pages, k_scales=None, v_scales=None):
+        torch = _torch()
+        if k_pages.dim() != 4:
+            raise ValueError("pages must be [pages, heads, page, head]")
+        self.pages, self.heads, self.page, self.head_dim = k_pages.shape
+        self.type = {torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16, torch.int8: TYPE_Q8}.get(k_pages.dtype)
+        if self.type is None:
+            raise ValueError("pages must be float16, bfloat16 or int8")
+        if self.head_dim not in (64, 128, 256):
+            raise ValueError("head must be 64, 128 or 256")
+        if self.page < 16 or self.page & (self.page - 1) or not 0 < self.pages * self.page < 1 << 31:
+            raise ValueError("page must be a power of two of at least 16, and the cache hold 1 to 2^31 - 1 tokens")
+        ptrs = [_whole(t, name, k_pages.dtype, *k_pages.shape) for t, name in ((k_pages, "k_pages"),
+                                                                              (v_pages, "v_pages"))]
+        if (self.type == TYPE_Q8) != (k_scales is not None) or (k_scales is None) != (v_scales is None):
+            raise ValueError("int8 pages need k_scales and v_scales, other pages take none")
+        if self.type == TYPE_Q8:
+            shape = (self.pages, self.heads, self.page, self.head_dim // 32)
+            ptrs += [_whole(k_scales, "k_scales", torch.float16, *shape),
+                     _whole(v_scales, "v_scales", torch.float16, *shape)]
+        else:
+            ptrs += [0, 0]
+        _one_device(torch, k_pages, v_pages, k_scales, v_scales)
+        self.device = k_pages.get_device()
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self._struct = ctypes.create_string_buffer(
+            _CACHE.pack(*ptrs, self.pages, self.heads, self.page, self.head_dim, self.type), _CACHE.size)
+        self._address = ctypes.addressof(self._struct)
+
+
+def _qk(torch, q, k, v, pos, slots, cache, freqs, q_gamma, k_gamma, eps, rope, out_type):
+    """Packed arguments and outputs of the two calls below."""
+    types = _types(torch)
+    tokens, hq, d, q_stride = _rows(q, "q")
+    kt, hk, _, k_stride = _rows(k, "k", None, d)
+    if kt != tokens or k.dtype != q.dtype or q.dtype not in types:
+        raise ValueError("q and k must hold the same tokens in one type (float32, float16 or bfloat16)")
+    out_type = q.dtype if out_type is None else out_type
+    if out_type not in types:
+        raise ValueError("out_type must be float32, float16 or bfloat16")
+    if rope not in (ROPE_HALF, ROPE_INTERLEAVED):
+        raise ValueError("rope must be ROPE_HALF or ROPE_INTERLEAVED")
+    rot = 0 if freqs is None else 2 * freqs.numel()
+    if rot > d or rot % 16:
+        raise ValueError("freqs must hold a multiple of 8 frequencies, at most one for each two channels")
+    fp = _whole(freqs, "freqs", torch.float64, rot // 2) if rot else 0
+    gq = 0 if q_gamma is None else _whole(q_gamma, "q_gamma", torch.float32, d)
+    gk = 0 if k_gamma is None else _whole(k_gamma, "k_gamma", torch.float32, d)
+    _one_device(torch, q, k, v, pos, slots, freqs, q_gamma, k_gamma)
+    q_out = torch.empty((tokens, hq, d), dtype=out_type, device=q.device)
+    k_out, vp, v_stride, sp = None, 0, 0, 0
+    if cache is None:
+        k_out = torch.empty((tokens, hk, d), dtype=out_type, device=q.device)
+    else:
+        if cache.device != q.get_device() or cache.heads != hk or cache.head_dim != d:
+            raise ValueError("the cache must hold k's heads, on the same GPU")
+        vt, _, _, v_stride = _rows(v, "v", hk, d)
+        if vt != tokens or v.dtype != q.dtype:
+            raise ValueError("v must hold the same tokens as k in the same type")
+        vp, sp = v.data_ptr(), _whole(slots, "slots", torch.int64, tokens)
+    args = _QK.pack(q.data_ptr(), k.data_ptr(), vp, q_stride, k_stride, v_stride,
+                    _whole(pos, "pos", torch.int32, tokens), fp, gq, gk, sp, q_out.data_ptr(),
+                    0 if k_out is None else k_out.data_ptr(), tokens, hq, hk, d, rot, rope, types[q.dtype],
+                    types[out_type], eps)
+    return args, q_out, k_out
+
+
+def qk_norm_rope(q, k, pos, freqs=None, q_gamma=None, k_gamma=None, eps: float = 1e-6, rope: int = ROPE_HALF,
+                 out_type=None):
+    """RMS norm of each head of q [tokens, q_heads, head] and k [tokens, k_heads, head], then the first
+    2 * len(freqs) channels turned by pos * freqs (float64 radians for each position): new q and k in out_type.
+
+    A token's heads lie one after another; tokens may be strided (views of a fused projection)."""
+    torch = _torch()
+    args, q_out, k_out = _qk(torch, q, k, None, pos, None, None, freqs, q_gamma, k_gamma, eps, rope, out_type)
+    lib().check("iq4xs_qk_norm_rope", args, _stream(torch))
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q, k, v, pos, slots, cache, freqs=None, q_gamma=None, k_gamma=None, eps: float = 1e-6,
+                        rope: int = ROPE_HALF, out_type=None):
+    """qk_norm_rope with k and v written to the cache at slots [tokens] (int64; negative or past the cache: the token is
+    not stored).  Returns the new q."""
+    torch = _torch()
+    args, q_out, _ = _qk(torch, q, k, v, pos, slots, cache, freqs, q_gamma, k_gamma, eps, rope, out_type)
+    lib().check("iq4xs_qk_norm_rope_append", args, cache._address, _stream(torch))
+    return q_out
+
+
+def kv_gather(cache, table, starts, total: int, out_type=None):
+    """The cached tokens of sequences as dense rows (k, v), each [total, heads, head]: token j of sequence s, at page
+    table[s, j // page], is row starts[s] + j.  Rows outside every sequence, and tokens on no page of the cache, are
+    zero.  out_type defaults to the cache's, float16 for codes."""
+    torch = _torch()
+    types = _types(torch)
+    if out_type is None:
+        out_type = torch.float16 if cache.type == TYPE_Q8 else cache.k_pages.dtype
+    if out_type not in types or total < 0:
+        raise ValueError("out_type must be float32, float16 or bfloat16, and total not negative")
+    seqs = starts.numel() - 1
+    width = table.size(1) if table.dim() == 2 else 0
+    tp, sp = _whole(table, "table", torch.int32, seqs, width), _whole(starts, "starts", torch.int32, seqs + 1)
+    _one_device(torch, cache.k_pages, table, starts)
+    k, v = (torch.empty((total, cache.heads, cache.head_dim), dtype=out_type, device=table.device) for _ in "kv")
+    lib().check("iq4xs_kv_gather", cache._address, tp, width, sp, seqs, k.data_ptr(), v.data_ptr(), total,
+                types[out_type], _stream(torch))
+    return k, v
+
+
+def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, causal: bool = True, window: int = 0,
+                    lse: bool = False, scale: float | None = None, out_type=None):
+    """Attention of new tokens q [total, q_heads, head] over the paged cache, which holds their own keys and values too.
+
+    starts [seqs + 1] (int32): first row of each sequence; kv_len [seqs] (int32): its cached tokens, new ones included;
+    table [seqs, pages of the longest] (int32).  most_q and most_kv: at least the new and the cached tokens of any
+    sequence.  New token i stands at p = kv_len - new + i and sees keys up to p (causal) and after p - window (window >
+    0).  scale defaults to head ** -0.5, out_type to q's.  Returns out, or (out, log-sum-exp of the scores [total,
+    q_heads] in fp32) with lse; a row that sees nothing gives zeros and -inf."""
+    torch = _torch()
+    types = _types(torch)
+    total, hq, d, q_stride = _rows(q, "q", None, cache.head_dim)
+    out_type = q.dtype if out_type is None else out_type
+    kind = types.get(q.dtype, TYPE_F32)
+    if kind == TYPE_F32 or (cache.type != TYPE_Q8 and cache.type != kind) or out_type not in types:
+        raise ValueError("q must have the cache's type (float16 or bfloat16 for codes), out_type be a float type")
+    if hq % cache.heads:
+        raise ValueError("q's heads must be a multiple of the cache's")
+    seqs = starts.numel() - 1
+    width = table.size(1) if table.dim() == 2 else 0
+    tp, sp = _whole(table, "table", torch.int32, seqs, width), _whole(starts, "starts", torch.int32, seqs + 1)
+    lp = _whole(kv_len, "kv_len", torch.int32, seqs)
+    _one_device(torch, cache.k_pages, q, table, starts, kv_len)
+    out = torch.empty((total, hq, d), dtype=out_type, device=q.device)
+    sums = torch.empty((total, hq), dtype=torch.float32, device=q.device) if lse else None
+    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), sums.data_ptr() if lse else 0, cache._address, tp, sp, lp,
+                           q_stride, width, seqs, total, most_q, most_kv, window, hq, kind, types[out_type],
+                           bool(causal), d ** -0.5 if scale is None else scale)
+    nbytes = lib().iq4xs_paged_attention_workspace_bytes(args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    lib().check("iq4xs_paged_attention", args, ws.data_ptr() if nbytes else 0, nbytes, _stream(torch))
+    return (out, sums) if lse else out
 
 
 def synthetic_weights(K: int, N: int, seed: int, first_block: int = 0, device=None):
