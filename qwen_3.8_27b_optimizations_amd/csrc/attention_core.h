@@ -1,0 +1,139 @@
+// attention_core.h -- what the two attention kernels share: which keys a row sees, how the keys are split over
+// workgroups, matrix products, and the outputs.
+#pragma once
+
+#include <float.h>
+#include <math.h>
+
+#include "attention_device.h"
+
+namespace iq4xs {
+
+struct AttentionArgs {
+    CachePages c;
+    const void* q;
+    void* out;
+    float* lse;
+    const int32_t *table, *starts, *kv_len;
+    float* part;      // [splits][total][q_heads][D] unnormalised sums, with splits > 1
+    float* part_ml;   // [splits][total][q_heads][2] their maxima (in powers of two) and sums of weights
+    int64_t q_stride, width;
+    int total, most_q, most_kv, window;  // window 0: none
+    int seqs, q_heads, group, out_type, causal;
+    int splits, chunk;  // keys of a split, a multiple of 128
+    int row_tiles;
+    float scale;  // times log2(e)
+};
+
+// One sequence of the call, cut to what the arguments allow.
+struct Sequence {
+    int first, fresh;  // its rows in q: first row, count
+    int keys;          // cached tokens
+    int seen_from;     // first key that the first row sees, a multiple of 32: where split 0 begins
+    const int32_t* pages;
+};
+
+__device__ inline int least_key(const AttentionArgs& a, const Sequence& s, int total_fresh, int token) {
+    const int64_t lo = (int64_t)s.keys - total_fresh + token + 1 - a.window;
+    return a.window > 0 && lo > 0 ? (lo < s.keys ? (int)lo : s.keys) : 0;
+}
+__device__ inline int end_key(const AttentionArgs& a, const Sequence& s, int total_fresh, int token) {
+    const int64_t hi = (int64_t)s.keys - total_fresh + token + 1;
+    return !a.causal || hi > s.keys ? s.keys : hi > 0 ? (int)hi : 0;
+}
+
+// total_fresh: the new tokens as the positions count them; s.fresh of them are rows to compute.
+__device__ inline Sequence sequence(const AttentionArgs& a, int seq, int& total_fresh) {
+    Sequence s;
+    s.first = a.starts[seq];
+    total_fresh = a.starts[seq + 1] - s.first;
+    s.fresh = total_fresh < a.most_q ? total_fresh : a.most_q;
+    if (s.first < 0) s.fresh = 0;
+    if (s.fresh > a.total - s.first) s.fresh = a.total - s.first;
+    int64_t keys = a.kv_len[seq];
+    keys = keys < a.most_kv ? keys : a.most_kv;
+    keys = keys < (a.width << a.c.shift) ? keys : a.width << a.c.shift;
+    s.keys = keys > 0 ? (int)keys : 0;
+    s.seen_from = least_key(a, s, total_fresh, 0) & ~31;
+    s.pages = a.table + (int64_t)seq * a.width;
+    return s;
+}
+
+// Where the sums of a row that sees the keys [lo, hi) go: with one split, to the outputs, from the workgroup of that
+// split; with several, to its place in the workspace, from every workgroup that has them, and the joining kernel writes
+// the outputs, as it does for a row that sees nothing.
+enum RowEnd { ROW_OUT, ROW_PART, ROW_NONE };
+
+__device__ inline bool one_split(const AttentionArgs& a, const Sequence& s, int lo, int hi) {
+    return a.splits == 1 || (hi > lo && (lo - s.seen_from) / a.chunk == (hi - 1 - s.seen_from) / a.chunk);
+}
+__device__ inline RowEnd row_end(const AttentionArgs& a, const Sequence& s, int lo, int hi, int split) {
+    if (!one_split(a, s, lo, hi)) return ROW_PART;
+    return a.splits == 1 || (lo - s.seen_from) / a.chunk == split ? ROW_OUT : ROW_NONE;
+}
+
+// Pairs of 16-bit numbers: those that are finite (0 for the others), and ones where there is +Inf or NaN, -Inf or NaN.
+template <uint32_t EXPONENT, uint32_t ONES>
+__device__ inline void part_pairs(u4 x, u4& finite, u4& up, u4& down) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        uint32_t keep = ~0u, u = 0, d = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t y = x[p] >> (16 * h) & 0xFFFFu, half = 0xFFFFu << (16 * h);
+            const bool odd = (y & EXPONENT) == EXPONENT, nan = (y & ~EXPONENT & 0x7FFFu) != 0, minus = y >> 15;
+            if (odd) keep &= ~half;
+            if (odd && (nan || !minus)) u |= ONES & half;
+            if (odd && (nan || minus)) d |= ONES & half;
+        }
+        finite[p] = x[p] & keep;
+        up[p] = u;
+        down[p] = d;
+    }
+}
+
+template <typename T>
+struct Matrix;
+template <>
+struct Matrix<_Float16> {
+    static __device__ f4 mma16(u4 a, u4 b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
+    }
+    static constexpr uint32_t EXPONENT = 0x7C00u, ONES = 0x3C003C00u;
+    static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
+        part_pairs<EXPONENT, ONES>(x, finite, up, down);
+    }
+};
+template <>
+struct Matrix<__bf16> {
+    static __device__ f4 mma16(u4 a, u4 b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t pack(float x, float y) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    }
+    static constexpr uint32_t EXPONENT = 0x7F80u, ONES = 0x3F803F80u;
+    static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
+        part_pairs<EXPONENT, ONES>(x, finite, up, down);
+    }
+};
+
+// x of this lane and of the lanes 16, 32 and 48 away, which hold other keys of the same row.
+__device__ inline float max_of_quarters(float x) {
+    u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ inline float sum_of_quarters(float x) {
+    u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r.x) + __uint_as_float(r.y);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+}  // namespace iq4xs

@@ -14,6 +14,11 @@ hipError_t launch_qk_norm_rope(const iq4xs_qk_norm_rope_args& args, const iq4xs_
 hipError_t launch_kv_gather(const iq4xs_kv_cache& cache, const int32_t* table, int64_t width, const int32_t* starts,
                             int64_t seqs, void* k_out, void* v_out, int64_t total, int out_type, hipStream_t stream);
 
+struct AttentionArgs;
+// Rows of few new tokens; `tiles` 16-row tiles for each workgroup (1 or 2).
+void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
+                             hipStream_t stream);
+
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& args);
 hipError_t launch_paged_attention(const iq4xs_paged_attention_args& args, void* ws, hipStream_t stream);
 

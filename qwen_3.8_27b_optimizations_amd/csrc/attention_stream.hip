@@ -1,0 +1,552 @@
+// attention_stream.hip -- attention of few rows over the paged cache: single tokens and short drafts.
+//
+//   o = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q k_j - m),  lse = m + log(sum_j w_j)
+//
+// The rows of a cache head (its new tokens times the query heads that read it, token by token) are the columns of
+// 16 x 16 matrix products: S^T = K Q^T and O^T = V^T W^T.  Bound by reading the cache, so everything is arranged around
+// that read:
+// - a wave goes through its keys alone, 32 at a time, straight from memory into registers: no LDS and no barrier in the
+//   loop.  Keys arrive as the product's left operand; of the values a lane takes 8 keys by head_dim / 16 channels and
+//   turns them there with byte permutations, 1 for every 2 elements;
+// - the result of S^T holds, in each lane, weights of exactly the 8 keys whose values the lane took, for one row: they
+//   are the right operand of O^T as they stand;
+// - the four waves of a workgroup and the splits of a long cache go through different keys; the waves join in LDS, the
+//   splits in a second launch.
+// The running maximum of a row moves only when a key passes it by 2^8 (in powers of two): weights up to 2^8 are as exact
+// in 16 bits as weights up to 1, and the sums need no rescaling in most steps.
+// An 8-bit cache's codes become fp16 (exact); a key's four or so scales multiply the parts of its score in fp32, the
+// values' scales multiply their codes in fp16 (half a step of 2^-11).  bf16 queries for it become fp16 with a power of
+// two taken out of each row, exact down to 2^-14 of the row's largest element.
+#include "attention_core.h"
+#include "attention_internal.h"
+#include "iq4xs_internal.h"
+
+namespace iq4xs {
+
+constexpr int STREAM_WAVES = 4;
+constexpr int STEP_KEYS = 32;  // of a wave at a time
+
+// The rows' queries, right operand of S^T: in registers, of 256 channels in LDS (every wave has the same), where the
+// registers do not hold them beside a step and the sums.
+template <int D, int NT>
+struct Queries {
+    u4 own[NT][D / 32];
+    __device__ u4 at(int i, int c) const { return own[i][c]; }
+};
+template <int NT>
+struct Queries<256, NT> {
+    const u4* own;  // of this lane; [tile][8][64 lanes]
+    __device__ u4 at(int i, int c) const { return own[(8 * i + c) * 64]; }
+};
+
+// Two tiles of 16 keys as they lie in the cache, in the lanes that use them.
+template <int D, typename KV>
+struct Step {
+    static constexpr int OWN = D / 16;  // channels of a value in a lane
+    u4 k[2][D / 32];
+    u4 v[8][OWN / 8 ? OWN / 8 : 1];
+
+    __device__ void load_keys(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
+        const uint16_t* p = static_cast<const uint16_t*>(a.c.k);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+                k[t][c] = *reinterpret_cast<const u4*>(p + row[t] * D + n * D + 32 * c + 8 * j);
+    }
+    __device__ void load_values(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
+        const uint16_t* p = static_cast<const uint16_t*>(a.c.v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint16_t* r = p + row[e / 4] * D + (4 * j + e % 4) * D;
+            if constexpr (OWN == 4) {
+                const u2 w = *reinterpret_cast<const u2*>(r + 4 * n);
+                v[e][0] = u4{w.x, w.y, 0, 0};
+            } else {
+#pragma unroll
+                for (int h = 0; h < OWN / 8; ++h) v[e][h] = *reinterpret_cast<const u4*>(r + 128 * h + 8 * n);
+            }
+        }
+    }
+    template <int NT>
+    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                s[i][t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) s[i][t] = Matrix<KV>::mma16(k[t][c], q.at(i, c), s[i][t]);
+            }
+    }
+    // Left operand of O^T for the lane's channel t: its 8 keys, two for each word.
+    __device__ u4 values(int t) const {
+        u4 x;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int h = t / 8, w = (t % 8) / 2;
+            x[p] = __builtin_amdgcn_perm(v[2 * p + 1][h][w], v[2 * p][h][w], t % 2 ? 0x07060302u : 0x05040100u);
+        }
+        return x;
+    }
+    __device__ void prepare_values() {}
+    // Whether a value in the slots of the mask is an infinity or NaN.
+    __device__ bool not_finite(u4 slots) const {
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!(slots[e / 2] >> (16 * (e % 2)) & 1)) continue;
+#pragma unroll
+            for (int w = 0; w < OWN / 2; ++w) {
+                const uint32_t x = v[e][w / 4][w % 4];
+                odd = odd || (x & Matrix<KV>::EXPONENT) == Matrix<KV>::EXPONENT ||
+                      (x & (Matrix<KV>::EXPONENT << 16)) == Matrix<KV>::EXPONENT << 16;
+            }
+        }
+        return odd;
+    }
+    // Clears the values in the slots outside the mask.
+    __device__ void keep_values(u4 slots) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < OWN / 2; ++w)
+                if (!(slots[e / 2] >> (16 * (e % 2)) & 1)) v[e][w / 4][w % 4] = 0;
+    }
+    // Copies for the compiler: work on them is not moved ahead of the branch they are in.
+    __device__ void opaque() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int h = 0; h < (OWN / 8 ? OWN / 8 : 1); ++h) asm volatile("" : "+v"(v[e][h]));
+    }
+    using Weight = KV;
+};
+
+// codes: bytes of `hi` and `lo` at place b as a pair of fp16 numbers (1024 + code + 128, then less 1152: both exact)
+__device__ inline h2 code_pair(uint32_t hi, uint32_t lo, int b) {
+    const uint32_t sel = 0x0C040C00u + 0x00010001u * b;
+    const uint32_t w = __builtin_amdgcn_perm(hi, lo, sel) | 0x64006400u;
+    return __builtin_bit_cast(h2, w) - h2{(_Float16)1152, (_Float16)1152};
+}
+
+template <int D>
+struct Step<D, int8_t> {
+    static constexpr int OWN = D / 16, WORDS = D / 64, HALVES = D == 256 ? 2 : 1, GROUPS = D / 32;
+    u2 k[2][D / 32];
+    uint32_t ks[2][4 * GROUPS / 2];  // fp16 scales of this lane's four keys of a tile, all groups
+    uint32_t v[8][WORDS];
+    uint16_t vs[8][HALVES];
+    h2 pair[HALVES][4];
+
+    __device__ void load_keys(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
+        const int8_t* p = static_cast<const int8_t*>(a.c.k);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+                k[t][c] = *reinterpret_cast<const u2*>(p + row[t] * D + n * D + 32 * c + 8 * j);
+            const u4* s = reinterpret_cast<const u4*>(a.c.ks + (row[t] + 4 * j) * GROUPS);
+#pragma unroll
+            for (int i = 0; i < GROUPS / 2; ++i) {
+                const u4 w = s[i];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) ks[t][4 * i + x] = w[x];
+            }
+        }
+    }
+    __device__ void load_values(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
+        const int8_t* p = static_cast<const int8_t*>(a.c.v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t r = row[e / 4] + 4 * j + e % 4;
+            if constexpr (OWN == 4) {
+                v[e][0] = *reinterpret_cast<const uint32_t*>(p + r * D + 4 * n);
+            } else {
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) {
+                    const u2 w = *reinterpret_cast<const u2*>(p + r * D + 128 * h + 8 * n);
+                    v[e][2 * h] = w.x;
+                    v[e][2 * h + 1] = w.y;
+                }
+            }
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(a.c.vs) + r * GROUPS;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) vs[e][h] = s[OWN == 4 ? n / 8 : 4 * h + n / 4];
+        }
+    }
+    template <int NT>
+    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) s[i][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                u4 x;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t b = (w < 2 ? k[t][c].x : k[t][c].y) ^ 0x80808080u;
+                    const uint32_t z = __builtin_amdgcn_perm(b, b, w % 2 ? 0x0C030C02u : 0x0C010C00u) | 0x64006400u;
+                    x[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, z) - h2{(_Float16)1152, (_Float16)1152});
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const f4 part = Matrix<_Float16>::mma16(x, q.at(i, c), f4{0, 0, 0, 0});
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = r * GROUPS + c;
+                        const _Float16 scale = __builtin_bit_cast(h2, ks[t][at / 2])[at % 2];
+                        s[i][t][r] = __builtin_fmaf((float)scale, part[r], s[i][t][r]);
+                    }
+                }
+            }
+        }
+    }
+    __device__ void prepare_values() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) v[e][w] ^= 0x80808080u;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                pair[h][p] = __builtin_bit_cast(h2, (uint32_t)vs[2 * p][h] | ((uint32_t)vs[2 * p + 1][h] << 16));
+    }
+    __device__ u4 values(int t) const {
+        u4 x;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            x[p] = __builtin_bit_cast(uint32_t, code_pair(v[2 * p + 1][t / 4], v[2 * p][t / 4], t % 4) * pair[t / 8][p]);
+        return x;
+    }
+    __device__ bool not_finite(u4 slots) const {
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+                odd = odd || ((slots[e / 2] >> (16 * (e % 2)) & 1) && (vs[e][h] & 0x7C00u) == 0x7C00u);
+        return odd;
+    }
+    __device__ void keep_values(u4 slots) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                pair[h][p] = __builtin_bit_cast(h2, __builtin_bit_cast(uint32_t, pair[h][p]) & slots[p]);
+    }
+    __device__ void opaque() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) asm volatile("" : "+v"(v[e][w]));
+    }
+    using Weight = _Float16;
+};
+
+// The lane's 8 keys of a step as word masks: pairs of 16-bit slots whose key lies in [lo, hi).
+__device__ inline u4 slots_in(int base, int j, int lo, int hi) {
+    u4 m;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int key = base + (p < 2 ? 0 : 16) + 4 * j + 2 * (p % 2);
+        m[p] = (key >= lo && key < hi ? 0xFFFFu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+    }
+    return m;
+}
+
+template <int D, typename Q, typename KV, int NT>
+__global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void stream_attention_kernel(AttentionArgs a) {
+    constexpr int OWN = D / 16, PART = D == 64 ? 64 : 128;
+    using W = typename Step<D, KV>::Weight;
+    constexpr uint32_t ONES = Matrix<W>::ONES;
+    __shared__ float so[STREAM_WAVES][16][PART + 4];
+    __shared__ float sm[STREAM_WAVES][16], sl[STREAM_WAVES][16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int n = lane % 16, j = lane / 16;
+    unsigned x = blockIdx.x;
+    const int head = x % a.c.heads;
+    x /= a.c.heads;
+    const int seq = x % a.seqs;
+    x /= a.seqs;
+    const int tile = x % a.row_tiles, split = x / a.row_tiles;
+    int total_fresh;
+    const Sequence s = sequence(a, seq, total_fresh);
+    const int rows = s.fresh * a.group, row0 = tile * 16 * NT;
+    if (row0 >= rows) return;
+    const int last = (rows < row0 + 16 * NT ? rows : row0 + 16 * NT) - 1;
+    const int token0 = row0 / a.group, token1 = last / a.group;
+    // keys that some row of the tile sees, and those that all see
+    const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
+    const int all_lo = least_key(a, s, total_fresh, token1), all_hi = end_key(a, s, total_fresh, token0);
+    int k0 = s.seen_from + split * a.chunk, k1 = any_hi;
+    if (a.splits > 1) {
+        k1 = any_hi < k0 + a.chunk ? any_hi : k0 + a.chunk;
+        if (k1 <= k0 || k0 + a.chunk <= any_lo) return;
+    }
+    if (k0 < (any_lo & ~31)) k0 = any_lo & ~31;
+
+    // this lane's rows and their keys (lanes without a row repeat the last)
+    int token[NT], lo[NT], hi[NT];
+    float factor[NT];
+    u4 q[NT][D / 32];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int r = row0 + 16 * i + n <= last ? row0 + 16 * i + n : last;
+        token[i] = r / a.group;
+        lo[i] = least_key(a, s, total_fresh, token[i]);
+        hi[i] = end_key(a, s, total_fresh, token[i]);
+        const int64_t at = (int64_t)(s.first + token[i]) * a.q_stride + (head * a.group + r % a.group) * D + 8 * j;
+        const u4* p = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) q[i][c] = p[4 * c];
+        factor[i] = a.scale;
+        if constexpr (sizeof(KV) == 1 && sizeof(Q) == 2 && __is_same(Q, __bf16)) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t u = q[i][c][w] & 0x7FFF7FFFu;
+                    top = top > (u & 0xFFFFu) ? top : u & 0xFFFFu;
+                    top = top > u >> 16 ? top : u >> 16;
+                }
+            // the largest finite exponent of the row: its element becomes 1 to 2
+            const float size = max_of_quarters(__uint_as_float(top << 16));
+            const int e = size > 0.0f && size <= FLT_MAX ? ilogbf(size) : 0;
+            factor[i] = ldexpf(a.scale, e);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    q[i][c][w] = Matrix<_Float16>::pack(ldexpf(__uint_as_float(q[i][c][w] << 16), -e),
+                                                        ldexpf(__uint_as_float(q[i][c][w] & 0xFFFF0000u), -e));
+        }
+    }
+
+    Queries<D, NT> queries;
+    if constexpr (D == 256) {
+        __shared__ u4 sq[NT][D / 32][64];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+                if (wave == 0) sq[i][c][lane] = q[i][c];
+        __syncthreads();
+        queries.own = &sq[0][0][lane];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) queries.own[i][c] = q[i][c];
+    }
+
+    f4 o[NT][OWN];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        m[i] = -FLT_MAX;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < OWN; ++t) o[i][t] = f4{0, 0, 0, 0};
+    }
+
+    // where tile t of the step at `base` lies; a tile past the end or on no page of the cache reads page 0 and is masked
+    auto find = [&](int base, int64_t(&row)[2], bool(&there)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = base + 16 * t;
+            int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
+            there[t] = page >= 0 && page < a.c.pages;
+            row[t] = page_row(a.c, there[t] ? page : 0, head, there[t] ? key & ((1 << a.c.shift) - 1) : 0);
+        }
+    };
+
+    Step<D, KV> step;
+    int64_t row[2];
+    bool there[2];
+    int base = k0 + STEP_KEYS * wave;
+    if (base < k1) {
+        find(base, row, there);
+        step.load_keys(a, row, n, j);
+        step.load_values(a, row, n, j);
+    }
+    while (base < k1) {
+        const int next = base + STEP_KEYS * STREAM_WAVES;
+        int64_t next_row[2];
+        bool next_there[2];
+        find(next, next_row, next_there);
+        f4 z[NT][2];
+        step.scores(queries, z);
+        if (next < k1) step.load_keys(a, next_row, n, j);
+        const bool full = there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
+        u4 w[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    z[i][t][r] *= factor[i];
+                    if (!full) {
+                        const int key = base + 16 * t + 4 * j + r;
+                        if (!there[t] || key < lo[i] || key >= hi[i]) z[i][t][r] = -INFINITY;
+                    }
+                    top = fmaxf(top, z[i][t][r]);
+                }
+            if (__any(top > m[i] + 8.0f)) {
+                const float up = fmaxf(max_of_quarters(top), m[i]), keep = __builtin_amdgcn_exp2f(m[i] - up);
+                m[i] = up;
+                l[i] *= keep;
+#pragma unroll
+                for (int t = 0; t < OWN; ++t) o[i][t] *= keep;
+            }
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(z[i][e / 4][e % 4] - m[i]);
+                l[i] += p[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[i][e] = Matrix<W>::pack(p[2 * e], p[2 * e + 1]);
+        }
+        step.prepare_values();
+        // a weight of zero times an infinity is NaN: what no row sees is cleared, and where rows differ in what they see
+        // and a value is not finite, such values are left out of the product and reach the rows that see them as
+        // infinities (a NaN as both)
+        bool odd = false;
+        if (!full) {
+            u4 some = slots_in(base, j, any_lo, any_hi);
+            if (!there[0]) some.x = some.y = 0;
+            if (!there[1]) some.z = some.w = 0;
+            step.keep_values(some);
+            odd = token0 != token1 && __any(step.not_finite(some));
+        }
+        if (!odd) {
+#pragma unroll
+            for (int t = 0; t < OWN; ++t) {
+                const u4 x = step.values(t);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) o[i][t] = Matrix<W>::mma16(x, w[i], o[i][t]);
+                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            step.opaque();
+#pragma unroll
+            for (int t = 0; t < OWN; ++t) {
+                const u4 x = step.values(t);
+                u4 finite, up, down;
+                Matrix<W>::part(x, finite, up, down);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const u4 sees = slots_in(base, j, lo[i], hi[i]) & u4{ONES, ONES, ONES, ONES};
+                    const f4 y = Matrix<W>::mma16(up, sees, f4{0, 0, 0, 0}), z = Matrix<W>::mma16(down, sees, f4{0, 0, 0, 0});
+                    o[i][t] = Matrix<W>::mma16(finite, w[i], o[i][t]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (y[r] > 0.0f) o[i][t][r] += INFINITY;
+                        if (z[r] > 0.0f) o[i][t][r] -= INFINITY;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (next < k1) step.load_values(a, next_row, n, j);
+        base = next;
+        there[0] = next_there[0];
+        there[1] = next_there[1];
+    }
+
+    // the waves' sums join in LDS, 16 rows and up to 128 channels at a time, in the waves' order
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const float lw = sum_of_quarters(l[i]);
+        __syncthreads();
+        if (j == 0) {
+            sm[wave][n] = m[i];
+            sl[wave][n] = lw;
+        }
+        __syncthreads();
+        float top = sm[0][n];
+#pragma unroll
+        for (int w = 1; w < STREAM_WAVES; ++w) top = fmaxf(top, sm[w][n]);
+        const float f = __builtin_amdgcn_exp2f(m[i] - top);
+#pragma unroll
+        for (int part = 0; part < D / PART; ++part) {
+            if (part) __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < PART / 16; t += 4) {
+                    const int u = 8 * part + t;
+                    *reinterpret_cast<f4*>(&so[wave][n][(4 * j + r) * (PART / 16) + t]) =
+                        f4{o[i][u][r] * f, o[i][u + 1][r] * f, o[i][u + 2][r] * f, o[i][u + 3][r] * f};
+                }
+            __syncthreads();
+            constexpr int LANES = PART / 4, AT_ONCE = 64 * STREAM_WAVES / LANES;
+            for (int y = threadIdx.x / LANES; y < 16; y += AT_ONCE) {
+                const int r = row0 + 16 * i + y, c = threadIdx.x % LANES * 4;
+                if (r > last) continue;
+                float best = sm[0][y];
+#pragma unroll
+                for (int w = 1; w < STREAM_WAVES; ++w) best = fmaxf(best, sm[w][y]);
+                float sum = 0.0f;
+                f4 v{0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < STREAM_WAVES; ++w) {
+                    sum += sl[w][y] * __builtin_amdgcn_exp2f(sm[w][y] - best);
+                    v += *reinterpret_cast<const f4*>(&so[w][y][c]);
+                }
+                const int tok = r / a.group, h = head * a.group + r % a.group;
+                const int64_t out = (int64_t)(s.first + tok) * a.q_heads + h;
+                const RowEnd end = row_end(a, s, least_key(a, s, total_fresh, tok), end_key(a, s, total_fresh, tok), split);
+                if (end == ROW_OUT) {
+                    store4(a.out, out * D + PART * part + c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / sum);
+                    if (a.lse && part == 0 && c == 0)
+                        a.lse[out] = sum == 0.0f ? -INFINITY : (best + __log2f(sum)) * 0.69314718056f;
+                } else if (end == ROW_PART) {
+                    const int64_t at = (int64_t)split * a.total * a.q_heads + out;
+                    *reinterpret_cast<f4*>(a.part + at * D + PART * part + c) = v;
+                    if (part == 0 && c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(best, sum);
+                }
+            }
+        }
+    }
+}
+
+template <int D, int NT>
+void launch_types(const AttentionArgs& a, int type, int cache_type, dim3 grid, hipStream_t stream) {
+    const dim3 block(64 * STREAM_WAVES);
+    if (cache_type == IQ4XS_TYPE_F16)
+        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, _Float16, NT>), grid, block, 0, stream, a);
+    else if (cache_type == IQ4XS_TYPE_BF16)
+        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, __bf16, NT>), grid, block, 0, stream, a);
+    else if (type == IQ4XS_TYPE_F16)
+        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, int8_t, NT>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, int8_t, NT>), grid, block, 0, stream, a);
+}
+
+template <int D>
+void launch_tiles(const AttentionArgs& a, int tiles, int type, int cache_type, dim3 grid, hipStream_t stream) {
+    if (tiles == 1)
+        launch_types<D, 1>(a, type, cache_type, grid, stream);
+    else
+        launch_types<D, 2>(a, type, cache_type, grid, stream);
+}
+
+void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
+                             hipStream_t stream) {
+    const dim3 blocks((unsigned)grid);
+    if (head_dim == 64)
+        launch_tiles<64>(a, tiles, type, cache_type, blocks, stream);
+    else if (head_dim == 128)
+        launch_tiles<128>(a, tiles, type, cache_type, blocks, stream);
+    else
+        launch_tiles<256>(a, tiles, type, cache_type, blocks, stream);
+}
+
+}  // namespace iq4xs
