@@ -63,7 +63,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(AttentionArgs
 
 // What a call launches.
 struct AttentionPlan {
-    int tiles;      // 16-row tiles of a workgroup
+    int tiles;      // 16-row tiles of a workgroup that streams the cache, or 0: the kernel of many rows
     int row_tiles;  // workgroups for the rows of a sequence and cache head
     int splits, chunk;
     int64_t grid;
@@ -72,14 +72,16 @@ struct AttentionPlan {
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
-    p.tiles = most_q * group <= 16 ? 1 : 2;
-    const int64_t row_tiles = (most_q * group + 16 * p.tiles - 1) / (16 * p.tiles);
+    p.tiles = most_q * group <= 16 ? 1 : most_q * group <= 32 ? 2 : 0;
+    const int64_t tile = p.tiles ? 16 * p.tiles : 128, row_tiles = (most_q * group + tile - 1) / tile;
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;
     if (g.window > 0 && g.window + most_q + 32 < span) span = g.window + most_q + 32;
-    // enough workgroups for three on every CU twice over, none with less than 128 keys (32 for a wave)
-    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, want = 6 * (int64_t)device_cu_count();
-    int64_t splits = (want + pairs - 1) / pairs, most = (span + 127) / 128;
+    // few rows: enough workgroups for three on every CU twice over, none with less than 128 keys (32 for a wave); many:
+    // for two on every CU, none with less than 512 keys
+    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, want = (p.tiles ? 6 : 2) * (int64_t)device_cu_count();
+    const int64_t least = p.tiles ? 128 : 512, most = (span + least - 1) / least;
+    int64_t splits = (want + pairs - 1) / pairs;
     splits = splits < most ? splits : most;
     const int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
     p.splits = (int)((span + chunk - 1) / chunk);
@@ -111,7 +113,10 @@ hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws,
                           g.scale * 1.44269504089f};
     const int64_t join = g.total * g.q_heads;
     if (p.grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
-    launch_stream_attention(a, D, p.tiles, g.type, g.cache->type, p.grid, stream);
+    if (p.tiles)
+        launch_stream_attention(a, D, p.tiles, g.type, g.cache->type, p.grid, stream);
+    else
+        launch_tile_attention(a, D, g.type, g.cache->type, p.grid, stream);
     if (p.splits > 1) {
         const dim3 blocks((unsigned)join), threads(JOIN_THREADS);
         if (D == 64)

@@ -9,6 +9,8 @@
 
 namespace iq4xs {
 
+typedef float fx16 __attribute__((ext_vector_type(16)));
+
 struct AttentionArgs {
     CachePages c;
     const void* q;
@@ -92,6 +94,15 @@ __device__ inline void part_pairs(u4 x, u4& finite, u4& up, u4& down) {
     }
 }
 
+template <uint32_t EXPONENT>
+__device__ inline bool odd_pairs(u4 x) {
+    bool odd = false;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+        odd = odd || (x[p] & EXPONENT) == EXPONENT || (x[p] & (EXPONENT << 16)) == EXPONENT << 16;
+    return odd;
+}
+
 template <typename T>
 struct Matrix;
 template <>
@@ -99,10 +110,14 @@ struct Matrix<_Float16> {
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
+    static __device__ fx16 mma32(u4 a, u4 b, fx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
     static __device__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
     }
     static constexpr uint32_t EXPONENT = 0x7C00u, ONES = 0x3C003C00u;
+    static __device__ bool not_finite(u4 x) { return odd_pairs<EXPONENT>(x); }
     static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
         part_pairs<EXPONENT, ONES>(x, finite, up, down);
     }
@@ -112,11 +127,15 @@ struct Matrix<__bf16> {
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }
+    static __device__ fx16 mma32(u4 a, u4 b, fx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
     static __device__ uint32_t pack(float x, float y) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
     }
     static constexpr uint32_t EXPONENT = 0x7F80u, ONES = 0x3F803F80u;
+    static __device__ bool not_finite(u4 x) { return odd_pairs<EXPONENT>(x); }
     static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
         part_pairs<EXPONENT, ONES>(x, finite, up, down);
     }
@@ -134,6 +153,45 @@ __device__ inline float sum_of_quarters(float x) {
     x = __uint_as_float(r.x) + __uint_as_float(r.y);
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// The same for the lane 32 away.
+__device__ inline float max_of_halves(float x) {
+    const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ inline float sum_of_halves(float x) {
+    const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// bf16 queries of a row for an 8-bit cache, as fp16 with a power of two taken out: 2^-e q, exact down to 2^-14 of the
+// row's largest element.  `top` is the largest magnitude of the row as bf16 bits, in every lane that holds a part of it.
+__device__ inline int query_exponent(uint32_t top) {
+    const float size = __uint_as_float(top << 16);
+    return size > 0.0f && size <= FLT_MAX ? ilogbf(size) : 0;
+}
+template <int N>
+__device__ inline uint32_t query_top(const u4 (&q)[N]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t u = q[c][w] & 0x7FFF7FFFu;
+            top = top > (u & 0xFFFFu) ? top : u & 0xFFFFu;
+            top = top > u >> 16 ? top : u >> 16;
+        }
+    return top;
+}
+template <int N>
+__device__ inline void queries_to_f16(u4 (&q)[N], int e) {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            q[c][w] = Matrix<_Float16>::pack(ldexpf(__uint_as_float(q[c][w] << 16), -e),
+                                             ldexpf(__uint_as_float(q[c][w] & 0xFFFF0000u), -e));
 }
 
 }  // namespace iq4xs

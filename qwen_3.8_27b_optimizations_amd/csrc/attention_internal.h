@@ -18,6 +18,9 @@ struct AttentionArgs;
 // Rows of few new tokens; `tiles` 16-row tiles for each workgroup (1 or 2).
 void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
                              hipStream_t stream);
+// Rows of many, 128 for each workgroup.
+void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, int64_t grid,
+                           hipStream_t stream);
 
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& args);
 hipError_t launch_paged_attention(const iq4xs_paged_attention_args& args, void* ws, hipStream_t stream);

@@ -304,25 +304,10 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void strea
         for (int c = 0; c < D / 32; ++c) q[i][c] = p[4 * c];
         factor[i] = a.scale;
         if constexpr (sizeof(KV) == 1 && sizeof(Q) == 2 && __is_same(Q, __bf16)) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t u = q[i][c][w] & 0x7FFF7FFFu;
-                    top = top > (u & 0xFFFFu) ? top : u & 0xFFFFu;
-                    top = top > u >> 16 ? top : u >> 16;
-                }
-            // the largest finite exponent of the row: its element becomes 1 to 2
-            const float size = max_of_quarters(__uint_as_float(top << 16));
-            const int e = size > 0.0f && size <= FLT_MAX ? ilogbf(size) : 0;
+            // the largest magnitudes of a row's four lanes, as numbers (a NaN lets the others through)
+            const int e = query_exponent(__float_as_uint(max_of_quarters(__uint_as_float(query_top(q[i]) << 16))) >> 16);
             factor[i] = ldexpf(a.scale, e);
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    q[i][c][w] = Matrix<_Float16>::pack(ldexpf(__uint_as_float(q[i][c][w] << 16), -e),
-                                                        ldexpf(__uint_as_float(q[i][c][w] & 0xFFFF0000u), -e));
+            queries_to_f16(q[i], e);
         }
     }
 

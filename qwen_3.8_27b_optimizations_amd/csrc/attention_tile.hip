@@ -1,0 +1,371 @@
+// attention_tile.hip -- attention of many rows over the paged cache: prompts, chunks of prompts and longer drafts.
+//
+//   o = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q k_j - m),  lse = m + log(sum_j w_j)
+//
+// A workgroup takes 128 rows of a cache head (new tokens times the query heads that read it, token by token, so that
+// rows of one token share every key) and goes through the keys in tiles; each of its four waves has 32 rows as the
+// columns of 32 x 32 matrix products, S^T = K Q^T and O^T = V^T W^T.  Bound by the matrix products, and next to them by
+// the exponentials (a quarter of the rate of other vector operations: 16 for every 16 x 32 x 32 products), so:
+// - tiles of keys and values reach LDS by asynchronous copies, the next tile's in flight during this tile's products;
+//   pieces of 16 bytes are exchanged within a row so that reads of rows (keys) and of columns (values, turned by the
+//   LDS on their way) touch every bank once;
+// - S^T leaves in each lane the weights of one row, for exactly the keys whose values the second product wants from
+//   that lane: weights stay in registers;
+// - two workgroups share a CU, so that one's products run beside the other's exponentials;
+// - the running maximum of a row moves only when a key passes it by 2^8 (in powers of two).
+// An 8-bit cache becomes fp16 on its way into LDS (half a step of 2^-11 for each key and value); bf16 queries for it
+// become fp16 with a power of two taken out of each row.
+#include <type_traits>
+
+#include "attention_core.h"
+#include "attention_internal.h"
+#include "iq4xs_internal.h"
+
+namespace iq4xs {
+
+constexpr int TILE_WAVES = 4, TILE_ROWS = 32 * TILE_WAVES;
+
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(const_cast<void*>(p));
+}
+
+// 16 bytes for each lane, from global base + offset to LDS at lds + 16 * lane, asynchronously (lds the same in all
+// lanes).  As asm: the compiler would let every later LDS read wait for it.  The kernel waits before the barrier that
+// ends a tile.
+__device__ inline void copy_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ inline u4 read_row(uint32_t lds) {
+    return *reinterpret_cast<__attribute__((address_space(3))) const u4*>((uintptr_t)lds);
+}
+// Four keys of the lane's channel: 16 lanes read 4 rows of 16 channels and each gets a column.
+__device__ inline u2 read_column(uint32_t lds) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4*>((uintptr_t)lds)));
+}
+
+// Geometry of a tile in LDS: KEYS rows of 2 * D bytes, 16-byte pieces exchanged within a row.
+template <int D>
+struct Tile {
+    static constexpr int KEYS = D == 256 ? 32 : 64;
+    static constexpr int ROW = 2 * D, BYTES = KEYS * ROW;
+    static constexpr int PIECES = D / 8;               // of a row
+    static constexpr int ROWS = 64 / PIECES;           // of 64 pieces
+    static constexpr int LOADS = KEYS * PIECES / 256;  // for each lane
+    // keys are read by rows: 16 rows' pieces of one place lie in 16 places
+    static __device__ int key_place(int row, int piece) {
+        return piece ^ (D == 64 ? (row >> 1) & 7 : row & 15);
+    }
+    // values by columns: 4 rows' groups of 4 pieces lie apart
+    static __device__ int value_place(int row, int piece) {
+        return piece ^ (D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2);
+    }
+};
+
+// 16-byte piece of 8 codes as fp16, times the scale of their group.
+__device__ inline u4 codes_to_f16(u2 w, _Float16 scale) {
+    u4 x;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const uint32_t b = (p < 2 ? w.x : w.y) ^ 0x80808080u;
+        const uint32_t z = __builtin_amdgcn_perm(b, b, p % 2 ? 0x0C030C02u : 0x0C010C00u) | 0x64006400u;
+        x[p] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(h2, z) - h2{(_Float16)1152, (_Float16)1152}) *
+                                                h2{scale, scale});
+    }
+    return x;
+}
+
+template <int D, typename Q, typename KV>
+__global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attention_kernel(AttentionArgs a) {
+    using T = Tile<D>;
+    constexpr bool CODES = sizeof(KV) == 1;
+    using W = typename std::conditional<CODES, _Float16, KV>::type;
+    using M = Matrix<W>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][T::BYTES];  // [buffer][keys, values]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int n = lane % 32, half = lane / 32;
+
+    unsigned x = blockIdx.x;
+    const int head = x % a.c.heads;
+    x /= a.c.heads;
+    const int seq = x % a.seqs;
+    x /= a.seqs;
+    // the last rows see the most keys: first
+    const int tile = a.row_tiles - 1 - x % a.row_tiles, split = x / a.row_tiles;
+    int total_fresh;
+    const Sequence s = sequence(a, seq, total_fresh);
+    const int rows = s.fresh * a.group, row0 = tile * TILE_ROWS;
+    if (row0 >= rows) return;
+    const int last = (rows < row0 + TILE_ROWS ? rows : row0 + TILE_ROWS) - 1;
+    const int token0 = row0 / a.group, token1 = last / a.group;
+    const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
+    int k0 = s.seen_from + split * a.chunk, k1 = any_hi;
+    if (a.splits > 1) {
+        k1 = any_hi < k0 + a.chunk ? any_hi : k0 + a.chunk;
+        if (k1 <= k0 || k0 + a.chunk <= any_lo) return;
+    }
+    if (k0 < (any_lo & ~31)) k0 = any_lo & ~31;
+
+    // this lane's row (lanes without one repeat the last) and this wave's keys
+    const int wave0 = row0 + 32 * wave;
+    const int r = wave0 + n <= last ? wave0 + n : last, token = r / a.group;
+    const int lo = least_key(a, s, total_fresh, token), hi = end_key(a, s, total_fresh, token);
+    const int wave_first = (wave0 <= last ? wave0 : last) / a.group;
+    const int wave_last = (wave0 + 31 <= last ? wave0 + 31 : last) / a.group;
+    const int some_lo = least_key(a, s, total_fresh, wave_first), some_hi = end_key(a, s, total_fresh, wave_last);
+    const int all_lo = least_key(a, s, total_fresh, wave_last), all_hi = end_key(a, s, total_fresh, wave_first);
+    const int query_head = head * a.group + r % a.group;
+
+    u4 q[D / 16];
+    float factor = fabsf(a.scale);
+    {
+        const u4* p = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q) +
+                                                  (int64_t)(s.first + token) * a.q_stride + query_head * D + 8 * half);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) q[c] = p[2 * c];
+        if constexpr (CODES && __is_same(Q, __bf16)) {
+            const int e =
+                query_exponent(__float_as_uint(max_of_halves(__uint_as_float(query_top(q) << 16))) >> 16);
+            factor = ldexpf(factor, e);
+            queries_to_f16(q, e);
+        }
+        // a negative scale goes with the queries; one of zero must not meet the -Inf of hidden keys
+        if (a.scale < 0.0f) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) q[c] ^= 0x80008000u;
+        }
+        factor = fmaxf(factor, FLT_MIN);
+    }
+
+    fx16 o[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = -FLT_MAX, l = 0.0f;
+
+    const uint32_t at = lds_address(lds);
+    // a tile's rows on their way: wave w brings rows [w KEYS / 4, (w + 1) KEYS / 4), which lie in one page; a page that
+    // is not in the cache, or past the keys, is read as page 0 and masked
+    const int bring = wave * (T::KEYS / 4), piece = lane % T::PIECES, in_load = lane / T::PIECES;
+    u2 code[2][CODES ? T::LOADS : 1];
+    _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    auto fetch = [&](int base, int buffer) {
+        const int key = base + bring;
+        const int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
+        const bool there = page >= 0 && page < a.c.pages;
+        const int64_t row = page_row(a.c, there ? page : 0, head, there ? key & ((1 << a.c.shift) - 1) : 0);
+        if constexpr (CODES) {
+            const int8_t* kp = static_cast<const int8_t*>(a.c.k) + row * D;
+            const int8_t* vp = static_cast<const int8_t*>(a.c.v) + row * D;
+            const _Float16 *ks = a.c.ks + row * (D / 32), *vs = a.c.vs + row * (D / 32);
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) {
+                const int rr = i * T::ROWS + in_load;
+                code[0][i] = *reinterpret_cast<const u2*>(kp + rr * D + 8 * piece);
+                code[1][i] = *reinterpret_cast<const u2*>(vp + rr * D + 8 * piece);
+                code_scale[0][i] = ks[rr * (D / 32) + piece / 4];
+                code_scale[1][i] = vs[rr * (D / 32) + piece / 4];
+            }
+        } else {
+            const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + row * T::ROW;
+            const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + row * T::ROW;
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) {
+                const int rr = i * T::ROWS + in_load;
+                const uint32_t to = at + buffer * 2 * T::BYTES + (bring + i * T::ROWS) * T::ROW;
+                copy_to_lds(kp, rr * T::ROW + 16 * T::key_place(bring + rr, piece), to);
+                copy_to_lds(vp, rr * T::ROW + 16 * T::value_place(bring + rr, piece), to + T::BYTES);
+            }
+        }
+    };
+    // an 8-bit tile goes through registers: fetched before a tile's products, put down after them
+    auto put = [&](int buffer) {
+        if constexpr (CODES) {
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) {
+                const int rr = bring + i * T::ROWS + in_load;
+                uint8_t* to = &lds[buffer][0][rr * T::ROW];
+                *reinterpret_cast<u4*>(to + 16 * T::key_place(rr, piece)) = codes_to_f16(code[0][i], code_scale[0][i]);
+                *reinterpret_cast<u4*>(to + T::BYTES + 16 * T::value_place(rr, piece)) =
+                    codes_to_f16(code[1][i], code_scale[1][i]);
+            }
+        }
+    };
+
+    // where this lane reads: keys by rows n, values by columns
+    const uint32_t key_at = at + n * T::ROW;
+    const int column = lane % 16;
+    const int value_row = 4 * half + column / 4;
+    const uint32_t value_at = at + T::BYTES + value_row * T::ROW + 8 * (column % 2);
+    const int value_piece = 2 * ((lane / 16) % 2) + (column % 4) / 2;
+
+    fetch(k0, 0);
+    put(0);
+    int buffer = 0;
+    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+        wait_for_copies();
+        __syncthreads();
+        if (base + T::KEYS < k1) fetch(base + T::KEYS, buffer ^ 1);
+        const uint32_t here = buffer * 2 * T::BYTES;
+        // pages of this tile that are not in the cache
+        uint32_t missing = 0;
+        for (int i = 0; i < T::KEYS / 16; ++i) {
+            const int key = base + 16 * i;
+            const int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
+            if (page < 0 || page >= a.c.pages) missing |= 1u << i;
+        }
+        const bool full = missing == 0 && base >= all_lo && base + T::KEYS <= all_hi;
+        if (base + T::KEYS > some_lo && base < some_hi) {
+            fx16 z[T::KEYS / 32];
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < T::KEYS / 32; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[t][i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c)
+                    z[t] = M::mma32(read_row(here + key_at + 32 * t * T::ROW + 16 * T::key_place(n, 2 * c + half)),
+                                    q[c], z[t]);
+            }
+            if (!full) {
+#pragma unroll
+                for (int t = 0; t < T::KEYS / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int in = 32 * t + 8 * (i / 4) + 4 * half + i % 4, key = base + in;
+                        if (key < lo || key >= hi || (missing >> (in / 16) & 1)) z[t][i] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < T::KEYS / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, z[t][i]);
+            top *= factor;
+            if (__any(top > m + 8.0f)) {
+                const float up = fmaxf(max_of_halves(top), m), keep = __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t) o[t] *= keep;
+            }
+            u4 w[T::KEYS / 16];
+#pragma unroll
+            for (int t = 0; t < T::KEYS / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i], factor, -m));
+                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i + 1], factor, -m));
+                    l += x0 + x1;
+                    w[2 * t + i / 8][i % 8 / 2] = M::pack(x0, x1);
+                }
+#pragma unroll
+            for (int k = 0; k < T::KEYS / 16; ++k) {
+                // the lane's 8 keys of 16: 4 half + 0..3 and 8 more
+                u4 some{~0u, ~0u, ~0u, ~0u}, sees = some;
+                if (!full) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const int key = base + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
+                        some[p] = (key >= some_lo && key < some_hi ? 0xFFFFu : 0u) |
+                                  (key + 1 >= some_lo && key + 1 < some_hi ? 0xFFFF0000u : 0u);
+                        sees[p] = (key >= lo && key < hi ? 0xFFFFu : 0u) |
+                                  (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+                        if (missing >> k & 1) some[p] = 0;
+                        sees[p] &= M::ONES;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t) {
+                    const uint32_t from = here + value_at + 16 * k * T::ROW +
+                                          16 * T::value_place(value_row, 4 * t + value_piece);
+                    const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
+                    u4 v{x0.x, x0.y, x1.x, x1.y};
+                    if (full) {
+                        o[t] = M::mma32(v, w[k], o[t]);
+                        continue;
+                    }
+                    // a weight of zero times an infinity is NaN: what no row of the wave sees is cleared; other values
+                    // that are not finite reach the rows that see them as infinities (a NaN as both)
+                    v &= some;
+                    if (!__any(M::not_finite(v))) {
+                        o[t] = M::mma32(v, w[k], o[t]);
+                    } else {
+                        u4 finite, up, down;
+                        M::part(v, finite, up, down);
+                        o[t] = M::mma32(finite, w[k], o[t]);
+                        fx16 zero;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
+                        const fx16 y = M::mma32(up, sees, zero);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (y[i] > 0.0f) o[t][i] += INFINITY;
+                        const fx16 y2 = M::mma32(down, sees, zero);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (y2[i] > 0.0f) o[t][i] -= INFINITY;
+                    }
+                }
+            }
+        }
+        if constexpr (CODES) {
+            if (base + T::KEYS < k1) put(buffer ^ 1);
+        }
+    }
+
+    if (wave0 + n > last) return;
+    l = sum_of_halves(l);
+    const int64_t out = (int64_t)(s.first + token) * a.q_heads + query_head;
+    const RowEnd end = row_end(a, s, lo, hi, split);
+    if (end == ROW_OUT) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f4 y = f4{o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]} * inv;
+                store4(a.out, out * D + 32 * t + 2 * i + 4 * half, a.out_type, l == 0.0f ? f4{0, 0, 0, 0} : y);
+            }
+        if (a.lse && half == 0) a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718056f;
+    } else if (end == ROW_PART) {
+        const int64_t part = (int64_t)split * a.total * a.q_heads + out;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f4*>(a.part + part * D + 32 * t + 2 * i + 4 * half) =
+                    f4{o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
+        if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
+    }
+}
+
+template <int D>
+void launch_types(const AttentionArgs& a, int type, int cache_type, dim3 grid, hipStream_t stream) {
+    const dim3 block(64 * TILE_WAVES);
+    if (cache_type == IQ4XS_TYPE_F16)
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, _Float16>), grid, block, 0, stream, a);
+    else if (cache_type == IQ4XS_TYPE_BF16)
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, __bf16>), grid, block, 0, stream, a);
+    else if (type == IQ4XS_TYPE_F16)
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t>), grid, block, 0, stream, a);
+}
+
+void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, int64_t grid,
+                           hipStream_t stream) {
+    const dim3 blocks((unsigned)grid);
+    if (head_dim == 64)
+        launch_types<64>(a, type, cache_type, blocks, stream);
+    else if (head_dim == 128)
+        launch_types<128>(a, type, cache_type, blocks, stream);
+    else
+        launch_types<256>(a, type, cache_type, blocks, stream);
+}
+
+}  // namespace iq4xs
