@@ -74,39 +74,44 @@ __device__ inline RowEnd row_end(const AttentionArgs& a, const Sequence& s, int 
     return a.splits == 1 || (lo - s.seen_from) / a.chunk == split ? ROW_OUT : ROW_NONE;
 }
 
-// Pairs of 16-bit numbers: those that are finite (0 for the others), and ones where there is +Inf or NaN, -Inf or NaN.
-template <uint32_t EXPONENT, uint32_t ONES>
-__device__ inline void part_pairs(u4 x, u4& finite, u4& up, u4& down) {
+// Pairs of 16-bit numbers as masks: 0xFFFF where a number is an infinity or NaN and `which` says so of its sign (0 or 1)
+// and of being NaN.
+template <uint32_t EXPONENT, typename Which>
+__device__ inline u4 odd_pairs(u4 x, Which which) {
+    u4 out;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        uint32_t keep = ~0u, u = 0, d = 0;
+        out[p] = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t y = x[p] >> (16 * h) & 0xFFFFu, half = 0xFFFFu << (16 * h);
-            const bool odd = (y & EXPONENT) == EXPONENT, nan = (y & ~EXPONENT & 0x7FFFu) != 0, minus = y >> 15;
-            if (odd) keep &= ~half;
-            if (odd && (nan || !minus)) u |= ONES & half;
-            if (odd && (nan || minus)) d |= ONES & half;
+            const uint32_t y = x[p] >> (16 * h) & 0xFFFFu;
+            if ((y & EXPONENT) == EXPONENT && which(y >> 15 != 0, (y & ~EXPONENT & 0x7FFFu) != 0))
+                out[p] |= 0xFFFFu << (16 * h);
         }
-        finite[p] = x[p] & keep;
-        up[p] = u;
-        down[p] = d;
     }
+    return out;
 }
 
-template <uint32_t EXPONENT>
-__device__ inline bool odd_pairs(u4 x) {
-    bool odd = false;
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-        odd = odd || (x[p] & EXPONENT) == EXPONENT || (x[p] & (EXPONENT << 16)) == EXPONENT << 16;
-    return odd;
-}
+// What the kernels do with pairs of 16-bit numbers: `finite` keeps those (0 for the others), `above` has ones where
+// there is +Inf or NaN, `below` where there is -Inf or NaN.
+template <uint32_t E, uint32_t ONE>
+struct Pairs {
+    static constexpr uint32_t EXPONENT = E, ONES = ONE;
+    static __device__ u4 finite(u4 x) {
+        return x & ~odd_pairs<E>(x, [](bool, bool) { return true; });
+    }
+    static __device__ u4 above(u4 x) {
+        return odd_pairs<E>(x, [](bool minus, bool nan) { return nan || !minus; }) & ONE;
+    }
+    static __device__ u4 below(u4 x) {
+        return odd_pairs<E>(x, [](bool minus, bool nan) { return nan || minus; }) & ONE;
+    }
+};
 
 template <typename T>
 struct Matrix;
 template <>
-struct Matrix<_Float16> {
+struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
@@ -116,14 +121,9 @@ struct Matrix<_Float16> {
     static __device__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
     }
-    static constexpr uint32_t EXPONENT = 0x7C00u, ONES = 0x3C003C00u;
-    static __device__ bool not_finite(u4 x) { return odd_pairs<EXPONENT>(x); }
-    static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
-        part_pairs<EXPONENT, ONES>(x, finite, up, down);
-    }
 };
 template <>
-struct Matrix<__bf16> {
+struct Matrix<__bf16> : Pairs<0x7F80u, 0x3F803F80u> {
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }
@@ -133,11 +133,6 @@ struct Matrix<__bf16> {
     static __device__ uint32_t pack(float x, float y) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
-    }
-    static constexpr uint32_t EXPONENT = 0x7F80u, ONES = 0x3F803F80u;
-    static __device__ bool not_finite(u4 x) { return odd_pairs<EXPONENT>(x); }
-    static __device__ void part(u4 x, u4& finite, u4& up, u4& down) {
-        part_pairs<EXPONENT, ONES>(x, finite, up, down);
     }
 };
 

@@ -423,17 +423,17 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void strea
 #pragma unroll
             for (int t = 0; t < OWN; ++t) {
                 const u4 x = step.values(t);
-                u4 finite, up, down;
-                Matrix<W>::part(x, finite, up, down);
+                const u4 above = Matrix<W>::above(x), below = Matrix<W>::below(x), finite = Matrix<W>::finite(x);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const u4 sees = slots_in(base, j, lo[i], hi[i]) & u4{ONES, ONES, ONES, ONES};
-                    const f4 y = Matrix<W>::mma16(up, sees, f4{0, 0, 0, 0}), z = Matrix<W>::mma16(down, sees, f4{0, 0, 0, 0});
+                    const u4 sees = slots_in(base, j, lo[i], hi[i]) & ONES;
+                    const f4 plus = Matrix<W>::mma16(above, sees, f4{0, 0, 0, 0});
+                    const f4 minus = Matrix<W>::mma16(below, sees, f4{0, 0, 0, 0});
                     o[i][t] = Matrix<W>::mma16(finite, w[i], o[i][t]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        if (y[r] > 0.0f) o[i][t][r] += INFINITY;
-                        if (z[r] > 0.0f) o[i][t][r] -= INFINITY;
+                        if (plus[r] > 0.0f) o[i][t][r] += INFINITY;
+                        if (minus[r] > 0.0f) o[i][t][r] -= INFINITY;
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);

@@ -154,9 +154,30 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     const int bring = wave * (T::KEYS / 4), piece = lane % T::PIECES, in_load = lane / T::PIECES;
     u2 code[2][CODES ? T::LOADS : 1];
     _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    constexpr int PARTS = T::KEYS / 16;
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    i4 pages{-1, -1, -1, -1};  // of the tile to fetch next, looked up a tile before; -1: none, or not in the cache
+    auto look_up = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int key = base + 16 * i;
+            pages[i] = key < k1 ? s.pages[key >> a.c.shift] : -1;
+        }
+    };
+    // which 16 keys of the tile that was looked up are not there
+    auto lacking = [&]() {
+        uint32_t out = 0;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+            if (pages[i] < 0 || pages[i] >= a.c.pages) out |= 1u << i;
+        return out;
+    };
     auto fetch = [&](int base, int buffer) {
         const int key = base + bring;
-        const int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
+        int page = pages[0];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i)
+            if (bring / 16 == i) page = pages[i];
         const bool there = page >= 0 && page < a.c.pages;
         const int64_t row = page_row(a.c, there ? page : 0, head, there ? key & ((1 << a.c.shift) - 1) : 0);
         if constexpr (CODES) {
@@ -204,21 +225,21 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     const uint32_t value_at = at + T::BYTES + value_row * T::ROW + 8 * (column % 2);
     const int value_piece = 2 * ((lane / 16) % 2) + (column % 4) / 2;
 
+    look_up(k0);
     fetch(k0, 0);
+    uint32_t missing = lacking(), next_missing = 0;
+    look_up(k0 + T::KEYS);
     put(0);
     int buffer = 0;
-    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1, missing = next_missing) {
         wait_for_copies();
         __syncthreads();
-        if (base + T::KEYS < k1) fetch(base + T::KEYS, buffer ^ 1);
-        const uint32_t here = buffer * 2 * T::BYTES;
-        // pages of this tile that are not in the cache
-        uint32_t missing = 0;
-        for (int i = 0; i < T::KEYS / 16; ++i) {
-            const int key = base + 16 * i;
-            const int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
-            if (page < 0 || page >= a.c.pages) missing |= 1u << i;
+        if (base + T::KEYS < k1) {
+            fetch(base + T::KEYS, buffer ^ 1);
+            next_missing = lacking();
+            look_up(base + 2 * T::KEYS);
         }
+        const uint32_t here = buffer * 2 * T::BYTES;
         const bool full = missing == 0 && base >= all_lo && base + T::KEYS <= all_hi;
         if (base + T::KEYS > some_lo && base < some_hi) {
             fx16 z[T::KEYS / 32];
@@ -263,52 +284,64 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
                     l += x0 + x1;
                     w[2 * t + i / 8][i % 8 / 2] = M::pack(x0, x1);
                 }
+            auto value = [&](int k, int t) {
+                const uint32_t from = here + value_at + 16 * k * T::ROW +
+                                      16 * T::value_place(value_row, 4 * t + value_piece);
+                const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
+                return u4{x0.x, x0.y, x1.x, x1.y};
+            };
+            if (full) {
 #pragma unroll
-            for (int k = 0; k < T::KEYS / 16; ++k) {
-                // the lane's 8 keys of 16: 4 half + 0..3 and 8 more
-                u4 some{~0u, ~0u, ~0u, ~0u}, sees = some;
-                if (!full) {
+                for (int k = 0; k < T::KEYS / 16; ++k)
+#pragma unroll
+                    for (int t = 0; t < D / 32; ++t) o[t] = M::mma32(value(k, t), w[k], o[t]);
+            } else {
+                // a weight of zero times an infinity is NaN: what no row of the wave sees is cleared, and values that are
+                // not finite are left out of the product and reach the rows that see them as infinities (a NaN as both)
+                int from_key = base;
+                auto slots = [&](int k, int from, int to) {  // the lane's 8 keys of 16: 4 half + 0..3 and 8 more
+                    u4 x;
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int key = base + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
-                        some[p] = (key >= some_lo && key < some_hi ? 0xFFFFu : 0u) |
-                                  (key + 1 >= some_lo && key + 1 < some_hi ? 0xFFFF0000u : 0u);
-                        sees[p] = (key >= lo && key < hi ? 0xFFFFu : 0u) |
-                                  (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
-                        if (missing >> k & 1) some[p] = 0;
-                        sees[p] &= M::ONES;
+                        const int key = from_key + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
+                        x[p] = missing >> k & 1 ? 0u
+                                                : (key >= from && key < to ? 0xFFFFu : 0u) |
+                                                      (key + 1 >= from && key + 1 < to ? 0xFFFF0000u : 0u);
+                    }
+                    return x;
+                };
+                uint32_t odd = 0;
+#pragma unroll
+                for (int k = 0; k < T::KEYS / 16; ++k) {
+                    const u4 some = slots(k, some_lo, some_hi);
+#pragma unroll
+                    for (int t = 0; t < D / 32; ++t) {
+                        const u4 v = value(k, t) & some, f = M::finite(v), x = v ^ f;
+                        odd |= x.x | x.y | x.z | x.w;
+                        o[t] = M::mma32(f, w[k], o[t]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
+                if (__any(odd != 0)) {
+                    // anew, so that the compiler does not keep the pass above's for it
+                    asm volatile("" : "+s"(from_key)::"memory");
 #pragma unroll
-                for (int t = 0; t < D / 32; ++t) {
-                    const uint32_t from = here + value_at + 16 * k * T::ROW +
-                                          16 * T::value_place(value_row, 4 * t + value_piece);
-                    const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
-                    u4 v{x0.x, x0.y, x1.x, x1.y};
-                    if (full) {
-                        o[t] = M::mma32(v, w[k], o[t]);
-                        continue;
-                    }
-                    // a weight of zero times an infinity is NaN: what no row of the wave sees is cleared; other values
-                    // that are not finite reach the rows that see them as infinities (a NaN as both)
-                    v &= some;
-                    if (!__any(M::not_finite(v))) {
-                        o[t] = M::mma32(v, w[k], o[t]);
-                    } else {
-                        u4 finite, up, down;
-                        M::part(v, finite, up, down);
-                        o[t] = M::mma32(finite, w[k], o[t]);
-                        fx16 zero;
+                    for (int t = 0; t < D / 32; ++t) {
+                        fx16 plus, minus;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
-                        const fx16 y = M::mma32(up, sees, zero);
+                        for (int i = 0; i < 16; ++i) plus[i] = minus[i] = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (y[i] > 0.0f) o[t][i] += INFINITY;
-                        const fx16 y2 = M::mma32(down, sees, zero);
+                        for (int k = 0; k < T::KEYS / 16; ++k) {
+                            const u4 v = value(k, t) & slots(k, some_lo, some_hi), sees = slots(k, lo, hi) & M::ONES;
+                            plus = M::mma32(M::above(v), sees, plus);
+                            minus = M::mma32(M::below(v), sees, minus);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (y2[i] > 0.0f) o[t][i] -= INFINITY;
+                        for (int i = 0; i < 16; ++i) {
+                            if (plus[i] > 0.0f) o[t][i] += INFINITY;
+                            if (minus[i] > 0.0f) o[t][i] -= INFINITY;
+                        }
                     }
                 }
             }
