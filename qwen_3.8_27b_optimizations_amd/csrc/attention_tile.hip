@@ -102,7 +102,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     if (row0 >= rows) return;
     const int last = (rows < row0 + TILE_ROWS ? rows : row0 + TILE_ROWS) - 1;
     const int token0 = row0 / a.group, token1 = last / a.group;
+    // keys that some row sees, and those that all see
     const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
+    const int all_lo = least_key(a, s, total_fresh, token1), all_hi = end_key(a, s, total_fresh, token0);
     int k0 = s.seen_from + split * a.chunk, k1 = any_hi;
     if (a.splits > 1) {
         k1 = any_hi < k0 + a.chunk ? any_hi : k0 + a.chunk;
@@ -110,14 +112,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     }
     if (k0 < (any_lo & ~31)) k0 = any_lo & ~31;
 
-    // this lane's row (lanes without one repeat the last) and this wave's keys
+    // this lane's row (lanes without one repeat the last)
     const int wave0 = row0 + 32 * wave;
     const int r = wave0 + n <= last ? wave0 + n : last, token = r / a.group;
     const int lo = least_key(a, s, total_fresh, token), hi = end_key(a, s, total_fresh, token);
-    const int wave_first = (wave0 <= last ? wave0 : last) / a.group;
-    const int wave_last = (wave0 + 31 <= last ? wave0 + 31 : last) / a.group;
-    const int some_lo = least_key(a, s, total_fresh, wave_first), some_hi = end_key(a, s, total_fresh, wave_last);
-    const int all_lo = least_key(a, s, total_fresh, wave_last), all_hi = end_key(a, s, total_fresh, wave_first);
     const int query_head = head * a.group + r % a.group;
 
     u4 q[D / 16];
@@ -218,6 +216,23 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         }
     };
 
+    // the values of a tile once more, what no row sees cleared
+    auto again = [&](int base, int buffer, uint32_t missing) {
+        for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
+            const int rr = i / T::PIECES, p = i % T::PIECES, key = base + rr;
+            u4 v{0, 0, 0, 0};
+            if (key >= any_lo && key < any_hi && !(missing >> (rr / 16) & 1)) {
+                const int64_t row = page_row(a.c, s.pages[key >> a.c.shift], head, key & ((1 << a.c.shift) - 1));
+                if constexpr (CODES)
+                    v = codes_to_f16(*reinterpret_cast<const u2*>(static_cast<const int8_t*>(a.c.v) + row * D + 8 * p),
+                                     a.c.vs[row * (D / 32) + p / 4]);
+                else
+                    v = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.c.v) + row * D + 8 * p);
+            }
+            *reinterpret_cast<u4*>(&lds[buffer][1][rr * T::ROW + 16 * T::value_place(rr, p)]) = v;
+        }
+    };
+
     // where this lane reads: keys by rows n, values by columns
     const uint32_t key_at = at + n * T::ROW;
     const int column = lane % 16;
@@ -234,116 +249,112 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1, missing = next_missing) {
         wait_for_copies();
         __syncthreads();
+        const uint32_t here = buffer * 2 * T::BYTES;
+        const bool edge = missing != 0 || base < all_lo || base + T::KEYS > all_hi;
+        // A weight of zero times an infinity is NaN.  Where rows differ in what they see, values that no row sees and
+        // values that are not finite are cleared in LDS; the latter come again after the tile's products.
+        bool odd = false;
+        if (edge) {
+            for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
+                const int key = base + i / T::PIECES;
+                u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
+                const bool seen = key >= any_lo && key < any_hi && !(missing >> (i / T::PIECES / 16) & 1);
+                const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
+                odd = odd || (seen && (x.x | x.y | x.z | x.w) != 0);
+                *p = f;
+            }
+            odd = __syncthreads_or(odd);
+        }
+        const uint32_t now_missing = missing;
         if (base + T::KEYS < k1) {
             fetch(base + T::KEYS, buffer ^ 1);
             next_missing = lacking();
             look_up(base + 2 * T::KEYS);
         }
-        const uint32_t here = buffer * 2 * T::BYTES;
-        const bool full = missing == 0 && base >= all_lo && base + T::KEYS <= all_hi;
-        if (base + T::KEYS > some_lo && base < some_hi) {
-            fx16 z[T::KEYS / 32];
-            float top = -INFINITY;
+
+        fx16 z[T::KEYS / 32];
 #pragma unroll
-            for (int t = 0; t < T::KEYS / 32; ++t) {
+        for (int t = 0; t < T::KEYS / 32; ++t) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) z[t][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) z[t][i] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c)
-                    z[t] = M::mma32(read_row(here + key_at + 32 * t * T::ROW + 16 * T::key_place(n, 2 * c + half)),
-                                    q[c], z[t]);
-            }
-            if (!full) {
-#pragma unroll
-                for (int t = 0; t < T::KEYS / 32; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int in = 32 * t + 8 * (i / 4) + 4 * half + i % 4, key = base + in;
-                        if (key < lo || key >= hi || (missing >> (in / 16) & 1)) z[t][i] = -INFINITY;
-                    }
-            }
+            for (int c = 0; c < D / 16; ++c)
+                z[t] = M::mma32(read_row(here + key_at + 32 * t * T::ROW + 16 * T::key_place(n, 2 * c + half)), q[c],
+                                z[t]);
+        }
+        if (edge) {
 #pragma unroll
             for (int t = 0; t < T::KEYS / 32; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, z[t][i]);
-            top *= factor;
-            if (__any(top > m + 8.0f)) {
-                const float up = fmaxf(max_of_halves(top), m), keep = __builtin_amdgcn_exp2f(m - up);
-                m = up;
-                l *= keep;
-#pragma unroll
-                for (int t = 0; t < D / 32; ++t) o[t] *= keep;
-            }
-            u4 w[T::KEYS / 16];
-#pragma unroll
-            for (int t = 0; t < T::KEYS / 32; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i], factor, -m));
-                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i + 1], factor, -m));
-                    l += x0 + x1;
-                    w[2 * t + i / 8][i % 8 / 2] = M::pack(x0, x1);
+                for (int i = 0; i < 16; ++i) {
+                    const int in = 32 * t + 8 * (i / 4) + 4 * half + i % 4, key = base + in;
+                    z[t][i] = key >= lo && key < hi && !(now_missing >> (in / 16) & 1) ? z[t][i] : -INFINITY;
                 }
-            auto value = [&](int k, int t) {
-                const uint32_t from = here + value_at + 16 * k * T::ROW +
-                                      16 * T::value_place(value_row, 4 * t + value_piece);
-                const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
-                return u4{x0.x, x0.y, x1.x, x1.y};
-            };
-            if (full) {
+        }
+        float top = z[0][0];
 #pragma unroll
-                for (int k = 0; k < T::KEYS / 16; ++k)
+        for (int t = 0; t < T::KEYS / 32; ++t)
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = M::mma32(value(k, t), w[k], o[t]);
-            } else {
-                // a weight of zero times an infinity is NaN: what no row of the wave sees is cleared, and values that are
-                // not finite are left out of the product and reach the rows that see them as infinities (a NaN as both)
-                int from_key = base;
-                auto slots = [&](int k, int from, int to) {  // the lane's 8 keys of 16: 4 half + 0..3 and 8 more
-                    u4 x;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, z[t][i]);
+        top *= factor;
+        if (__any(top > m + 8.0f)) {
+            const float up = fmaxf(max_of_halves(top), m), keep = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) o[t] *= keep;
+        }
+        auto value = [&](int k, int t) {
+            const uint32_t from =
+                here + value_at + 16 * k * T::ROW + 16 * T::value_place(value_row, 4 * t + value_piece);
+            const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
+            return u4{x0.x, x0.y, x1.x, x1.y};
+        };
+        u4 w[T::KEYS / 16];
+#pragma unroll
+        for (int t = 0; t < T::KEYS / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i], factor, -m));
+                const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i + 1], factor, -m));
+                l += x0 + x1;
+                w[2 * t + i / 8][i % 8 / 2] = M::pack(x0, x1);
+            }
+#pragma unroll
+        for (int k = 0; k < T::KEYS / 16; ++k)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) o[t] = M::mma32(value(k, t), w[k], o[t]);
+
+        if (odd) {
+            // the values that are not finite reach the rows that see them as infinities (a NaN as both)
+            wait_for_copies();
+            __syncthreads();
+            again(base, buffer, now_missing);
+            __syncthreads();
+            for (int t = 0; t < D / 32; ++t) {
+                fx16 plus, minus;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) plus[i] = minus[i] = 0.0f;
+                for (int k = 0; k < T::KEYS / 16; ++k) {
+                    u4 sees;
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int key = from_key + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
-                        x[p] = missing >> k & 1 ? 0u
-                                                : (key >= from && key < to ? 0xFFFFu : 0u) |
-                                                      (key + 1 >= from && key + 1 < to ? 0xFFFF0000u : 0u);
+                        const int key = base + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
+                        sees[p] = now_missing >> k & 1 ? 0u
+                                                       : ((key >= lo && key < hi ? 0xFFFFu : 0u) |
+                                                          (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u)) & M::ONES;
                     }
-                    return x;
-                };
-                uint32_t odd = 0;
-#pragma unroll
-                for (int k = 0; k < T::KEYS / 16; ++k) {
-                    const u4 some = slots(k, some_lo, some_hi);
-#pragma unroll
-                    for (int t = 0; t < D / 32; ++t) {
-                        const u4 v = value(k, t) & some, f = M::finite(v), x = v ^ f;
-                        odd |= x.x | x.y | x.z | x.w;
-                        o[t] = M::mma32(f, w[k], o[t]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    const u4 v = value(k, t);
+                    plus = M::mma32(M::above(v), sees, plus);
+                    minus = M::mma32(M::below(v), sees, minus);
                 }
-                if (__any(odd != 0)) {
-                    // anew, so that the compiler does not keep the pass above's for it
-                    asm volatile("" : "+s"(from_key)::"memory");
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) {
-                        fx16 plus, minus;
+                for (int u = 0; u < D / 32; ++u)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) plus[i] = minus[i] = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < T::KEYS / 16; ++k) {
-                            const u4 v = value(k, t) & slots(k, some_lo, some_hi), sees = slots(k, lo, hi) & M::ONES;
-                            plus = M::mma32(M::above(v), sees, plus);
-                            minus = M::mma32(M::below(v), sees, minus);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            if (plus[i] > 0.0f) o[t][i] += INFINITY;
-                            if (minus[i] > 0.0f) o[t][i] -= INFINITY;
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        if (u == t && plus[i] > 0.0f) o[u][i] += INFINITY;
+                        if (u == t && minus[i] > 0.0f) o[u][i] -= INFINITY;
                     }
-                }
             }
         }
         if constexpr (CODES) {
