@@ -121,6 +121,10 @@ struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
     static __device__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
     }
+    static __device__ uint32_t scaled(uint32_t x, float by) {
+        const h2 v = __builtin_bit_cast(h2, x);
+        return pack((float)v.x * by, (float)v.y * by);
+    }
 };
 template <>
 struct Matrix<__bf16> : Pairs<0x7F80u, 0x3F803F80u> {
@@ -133,6 +137,9 @@ struct Matrix<__bf16> : Pairs<0x7F80u, 0x3F803F80u> {
     static __device__ uint32_t pack(float x, float y) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    }
+    static __device__ uint32_t scaled(uint32_t x, float by) {
+        return pack(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xFFFF0000u) * by);
     }
 };
 

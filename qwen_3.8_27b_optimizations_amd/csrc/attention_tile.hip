@@ -51,7 +51,7 @@ __device__ inline u2 read_column(uint32_t lds) {
 // Geometry of a tile in LDS: KEYS rows of 2 * D bytes, 16-byte pieces exchanged within a row.
 template <int D>
 struct Tile {
-    static constexpr int KEYS = D == 256 ? 32 : 64;
+    static constexpr int KEYS = 64;
     static constexpr int ROW = 2 * D, BYTES = KEYS * ROW;
     static constexpr int PIECES = D / 8;               // of a row
     static constexpr int ROWS = 64 / PIECES;           // of 64 pieces
@@ -147,14 +147,12 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     float m = -FLT_MAX, l = 0.0f;
 
     const uint32_t at = lds_address(lds);
-    // a tile's rows on their way: wave w brings rows [w KEYS / 4, (w + 1) KEYS / 4), which lie in one page; a page that
-    // is not in the cache, or past the keys, is read as page 0 and masked
-    const int bring = wave * (T::KEYS / 4), piece = lane % T::PIECES, in_load = lane / T::PIECES;
-    u2 code[2][CODES ? T::LOADS : 1];
-    _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    // wave w brings a tile's rows 16 w to 16 w + 15, which lie in one page; a page that is not in the cache, or past the
+    // keys, is read as page 0 and masked
+    const int bring = 16 * wave, piece = lane % T::PIECES, in_load = lane / T::PIECES;
     constexpr int PARTS = T::KEYS / 16;
     typedef int i4 __attribute__((ext_vector_type(4)));
-    i4 pages{-1, -1, -1, -1};  // of the tile to fetch next, looked up a tile before; -1: none, or not in the cache
+    i4 pages{-1, -1, -1, -1};  // of a tile, looked up a tile before they are wanted; -1: none, or not in the cache
     auto look_up = [&](int base) {
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
@@ -162,56 +160,53 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             pages[i] = key < k1 ? s.pages[key >> a.c.shift] : -1;
         }
     };
-    // which 16 keys of the tile that was looked up are not there
-    auto lacking = [&]() {
-        uint32_t out = 0;
+    // of the tile at `base`, which was looked up: which 16 keys are not there, and where this wave's rows begin
+    auto locate = [&](int base, uint32_t& lacking) {
+        lacking = 0;
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
-            if (pages[i] < 0 || pages[i] >= a.c.pages) out |= 1u << i;
-        return out;
-    };
-    auto fetch = [&](int base, int buffer) {
-        const int key = base + bring;
+            if (pages[i] < 0 || pages[i] >= a.c.pages) lacking |= 1u << i;
         int page = pages[0];
 #pragma unroll
         for (int i = 1; i < PARTS; ++i)
-            if (bring / 16 == i) page = pages[i];
+            if (wave == i) page = pages[i];
         const bool there = page >= 0 && page < a.c.pages;
-        const int64_t row = page_row(a.c, there ? page : 0, head, there ? key & ((1 << a.c.shift) - 1) : 0);
+        return page_row(a.c, there ? page : 0, head, there ? (base + bring) & ((1 << a.c.shift) - 1) : 0);
+    };
+    // rows of one side (0 keys, 1 values) on their way to a buffer; of an 8-bit cache into registers, from which `put`
+    // takes them
+    u2 code[2][CODES ? T::LOADS : 1];
+    _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    auto fetch = [&](int side, int64_t row, int buffer) {
+        const void* from = side ? a.c.v : a.c.k;
         if constexpr (CODES) {
-            const int8_t* kp = static_cast<const int8_t*>(a.c.k) + row * D;
-            const int8_t* vp = static_cast<const int8_t*>(a.c.v) + row * D;
-            const _Float16 *ks = a.c.ks + row * (D / 32), *vs = a.c.vs + row * (D / 32);
+            const int8_t* p = static_cast<const int8_t*>(from) + row * D;
+            const _Float16* sc = (side ? a.c.vs : a.c.ks) + row * (D / 32);
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
                 const int rr = i * T::ROWS + in_load;
-                code[0][i] = *reinterpret_cast<const u2*>(kp + rr * D + 8 * piece);
-                code[1][i] = *reinterpret_cast<const u2*>(vp + rr * D + 8 * piece);
-                code_scale[0][i] = ks[rr * (D / 32) + piece / 4];
-                code_scale[1][i] = vs[rr * (D / 32) + piece / 4];
+                code[side][i] = *reinterpret_cast<const u2*>(p + rr * D + 8 * piece);
+                code_scale[side][i] = sc[rr * (D / 32) + piece / 4];
             }
         } else {
-            const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + row * T::ROW;
-            const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + row * T::ROW;
+            const uint8_t* p = static_cast<const uint8_t*>(from) + row * T::ROW;
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
                 const int rr = i * T::ROWS + in_load;
-                const uint32_t to = at + buffer * 2 * T::BYTES + (bring + i * T::ROWS) * T::ROW;
-                copy_to_lds(kp, rr * T::ROW + 16 * T::key_place(bring + rr, piece), to);
-                copy_to_lds(vp, rr * T::ROW + 16 * T::value_place(bring + rr, piece), to + T::BYTES);
+                copy_to_lds(p + i * T::ROWS * T::ROW,
+                            in_load * T::ROW + 16 * (side ? T::value_place(rr, piece) : T::key_place(rr, piece)),
+                            at + (buffer * 2 + side) * T::BYTES + (bring + i * T::ROWS) * T::ROW);
             }
         }
     };
-    // an 8-bit tile goes through registers: fetched before a tile's products, put down after them
-    auto put = [&](int buffer) {
+    auto put = [&](int side, int buffer) {
         if constexpr (CODES) {
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
-                const int rr = bring + i * T::ROWS + in_load;
-                uint8_t* to = &lds[buffer][0][rr * T::ROW];
-                *reinterpret_cast<u4*>(to + 16 * T::key_place(rr, piece)) = codes_to_f16(code[0][i], code_scale[0][i]);
-                *reinterpret_cast<u4*>(to + T::BYTES + 16 * T::value_place(rr, piece)) =
-                    codes_to_f16(code[1][i], code_scale[1][i]);
+                const int rr = i * T::ROWS + in_load;
+                const int place = side ? T::value_place(rr, piece) : T::key_place(rr, piece);
+                *reinterpret_cast<u4*>(&lds[buffer][side][(bring + rr) * T::ROW + 16 * place]) =
+                    codes_to_f16(code[side][i], code_scale[side][i]);
             }
         }
     };
@@ -234,23 +229,124 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     };
 
     // where this lane reads: keys by rows n, values by columns
-    const uint32_t key_at = at + n * T::ROW;
-    const int column = lane % 16;
-    const int value_row = 4 * half + column / 4;
-    const uint32_t value_at = at + T::BYTES + value_row * T::ROW + 8 * (column % 2);
-    const int value_piece = 2 * ((lane / 16) % 2) + (column % 4) / 2;
+    const int column = lane % 16, value_row = 4 * half + column / 4;
+    uint32_t key_at = at + n * T::ROW + 16 * T::key_place(n, half);
+    uint32_t value_at = at + T::BYTES + value_row * T::ROW + 8 * (column % 2) +
+                        16 * T::value_place(value_row, 2 * ((lane / 16) % 2) + (column % 4) / 2);
+    // pieces 2 c further along a row of keys, 4 t of values, and `more` bytes on: the exchange of pieces is an exclusive
+    // or within 16 (8 with heads of 64)
+    auto key_piece = [&](uint32_t from, int c, int more) {
+        return read_row((from ^ (32 * c & (T::ROW < 256 ? 127 : 255))) + (32 * c & ~255) + more);
+    };
+    auto value_piece = [&](uint32_t from, int t, int more) {
+        const uint32_t to = (from ^ (64 * t & (T::ROW < 256 ? 127 : 255))) + (64 * t & ~255) + more;
+        const u2 x0 = read_column(to), x1 = read_column(to + 8 * T::ROW);
+        return u4{x0.x, x0.y, x1.x, x1.y};
+    };
 
+    // `z` are scores of 32 keys at `base`: hidden ones go, the running maximum moves if it must, and with it the sums and the weights `w` still to be used.
+    auto raise = [&](fx16& z, int base, uint32_t lacking, bool edge, u4(&w)[2]) {
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int in = 8 * (i / 4) + 4 * half + i % 4, key = base + in;
+                z[i] = key >= lo && key < hi && !(lacking >> (in / 16) & 1) ? z[i] : -INFINITY;
+            }
+        }
+        float top = z[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
+        top *= factor;
+        if (__any(top > m + 8.0f)) {
+            // whole powers of two, so that scaling the 16-bit weights is exact
+            const float up = fmaxf(ceilf(max_of_halves(top)), m), keep = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) o[t] *= keep;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) w[k][p] = M::scaled(w[k][p], keep);
+        }
+    };
+    // A pair of weights of the scores z.
+    auto weigh = [&](const fx16& z, int i, u4(&w)[2]) {
+        const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], factor, -m));
+        const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i + 1], factor, -m));
+        l += x0 + x1;
+        uint32_t pair = M::pack(x0, x1);
+        asm volatile("" : "+v"(pair), "+v"(l));  // here, not where they are used
+        w[i / 8][i % 8 / 2] = pair;
+    };
+    // A step's products in turn, those of the scores (place c of the queries) between those of the values (16 keys k,
+    // channels t); its operands from LDS are read AHEAD products before.
+    constexpr int PRODUCTS = D / 8, AHEAD = 4;
+    auto piece_of = [&](int i, uint32_t keys, uint32_t values) {
+        const int j = i / 2;
+        return i % 2 == 0 ? key_piece(keys, j, 0) : value_piece(values, j % (D / 32), 16 * (j / (D / 32)) * T::ROW);
+    };
+    auto begin = [&](uint32_t keys, uint32_t values, u4(&f)[AHEAD]) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) f[i] = piece_of(i, keys, values);
+    };
+    // The scores `next` of 32 keys, the weights of the scores `z`, and the product of the weights `w` before them with
+    // their values.  The order is kept as written: beside each product its share of the weights.
+    auto step = [&](uint32_t keys, uint32_t values, u4(&f)[AHEAD], fx16& next, const fx16& z, const u4(&w)[2],
+                    u4(&w_next)[2]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PRODUCTS; ++i) {
+            const int j = i / 2;
+            if (i % 2 == 0)
+                next = M::mma32(f[i % AHEAD], q[j], next);
+            else
+                o[j % (D / 32)] = M::mma32(f[i % AHEAD], w[j / (D / 32)], o[j % (D / 32)]);
+            if (i + AHEAD < PRODUCTS) f[i % AHEAD] = piece_of(i + AHEAD, keys, values);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e * PRODUCTS / 8 == i || (PRODUCTS == 8 && e == i)) weigh(z, 2 * e, w_next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // Tile T in steps 2 T and 2 T + 1 of 32 keys.  A step computes the scores of the step after it and the weights of its
+    // own beside the product of the weights before it: keys are wanted a tile ahead of values.  The barrier of tile T
+    // comes before step 2 T + 1: keys of tile T and values of tile T - 1 are done with, those of T + 1 and T are there.
+    uint32_t lacking, next_lacking = (1u << PARTS) - 1;
     look_up(k0);
-    fetch(k0, 0);
-    uint32_t missing = lacking(), next_missing = 0;
+    int64_t row = locate(k0, lacking);
+    fetch(0, row, 0);
+    fetch(1, row, 0);
+    put(0, 0);
+    put(1, 0);
     look_up(k0 + T::KEYS);
-    put(0);
+    wait_for_copies();
+    __syncthreads();
+    fx16 even, odd_step;
+    u4 w_even[2] = {}, w_odd[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) even[i] = odd_step[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+        even = M::mma32(key_piece(key_at, c, 0), q[c], even);
+        odd_step = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], odd_step);
+    }
+    bool edge = lacking != 0 || k0 < all_lo || k0 + T::KEYS > all_hi;
+    raise(even, k0, lacking, edge, w_even);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) weigh(even, i, w_even);
+    if (k0 + T::KEYS < k1) {
+        row = locate(k0 + T::KEYS, next_lacking);
+        fetch(0, row, 1);
+        put(0, 1);
+        look_up(k0 + 2 * T::KEYS);
+    }
     int buffer = 0;
-    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1, missing = next_missing) {
+    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
         wait_for_copies();
         __syncthreads();
-        const uint32_t here = buffer * 2 * T::BYTES;
-        const bool edge = missing != 0 || base < all_lo || base + T::KEYS > all_hi;
         // A weight of zero times an infinity is NaN.  Where rows differ in what they see, values that no row sees and
         // values that are not finite are cleared in LDS; the latter come again after the tile's products.
         bool odd = false;
@@ -258,78 +354,39 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
                 const int key = base + i / T::PIECES;
                 u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
-                const bool seen = key >= any_lo && key < any_hi && !(missing >> (i / T::PIECES / 16) & 1);
+                const bool seen = key >= any_lo && key < any_hi && !(lacking >> (i / T::PIECES / 16) & 1);
                 const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
                 odd = odd || (seen && (x.x | x.y | x.z | x.w) != 0);
                 *p = f;
             }
             odd = __syncthreads_or(odd);
         }
-        const uint32_t now_missing = missing;
-        if (base + T::KEYS < k1) {
-            fetch(base + T::KEYS, buffer ^ 1);
-            next_missing = lacking();
-            look_up(base + 2 * T::KEYS);
+        const uint32_t was_lacking = lacking;
+        lacking = next_lacking;
+        next_lacking = (1u << PARTS) - 1;
+        if (base + T::KEYS < k1) fetch(1, row, buffer ^ 1);
+        if (base + 2 * T::KEYS < k1) {
+            row = locate(base + 2 * T::KEYS, next_lacking);
+            fetch(0, row, buffer);
+            look_up(base + 3 * T::KEYS);
         }
-
-        fx16 z[T::KEYS / 32];
-#pragma unroll
-        for (int t = 0; t < T::KEYS / 32; ++t) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[t][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-                z[t] = M::mma32(read_row(here + key_at + 32 * t * T::ROW + 16 * T::key_place(n, 2 * c + half)), q[c],
-                                z[t]);
-        }
-        if (edge) {
-#pragma unroll
-            for (int t = 0; t < T::KEYS / 32; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int in = 32 * t + 8 * (i / 4) + 4 * half + i % 4, key = base + in;
-                    z[t][i] = key >= lo && key < hi && !(now_missing >> (in / 16) & 1) ? z[t][i] : -INFINITY;
-                }
-        }
-        float top = z[0][0];
-#pragma unroll
-        for (int t = 0; t < T::KEYS / 32; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, z[t][i]);
-        top *= factor;
-        if (__any(top > m + 8.0f)) {
-            const float up = fmaxf(max_of_halves(top), m), keep = __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= keep;
-#pragma unroll
-            for (int t = 0; t < D / 32; ++t) o[t] *= keep;
-        }
-        auto value = [&](int k, int t) {
-            const uint32_t from =
-                here + value_at + 16 * k * T::ROW + 16 * T::value_place(value_row, 4 * t + value_piece);
-            const u2 x0 = read_column(from), x1 = read_column(from + 8 * T::ROW);
-            return u4{x0.x, x0.y, x1.x, x1.y};
-        };
-        u4 w[T::KEYS / 16];
-#pragma unroll
-        for (int t = 0; t < T::KEYS / 32; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i], factor, -m));
-                const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i + 1], factor, -m));
-                l += x0 + x1;
-                w[2 * t + i / 8][i % 8 / 2] = M::pack(x0, x1);
-            }
-#pragma unroll
-        for (int k = 0; k < T::KEYS / 16; ++k)
-#pragma unroll
-            for (int t = 0; t < D / 32; ++t) o[t] = M::mma32(value(k, t), w[k], o[t]);
+        asm volatile("" : "+v"(key_at), "+v"(value_at));  // the places along a row are cheaper computed than kept
+        const uint32_t here = buffer * 2 * T::BYTES, there = 2 * T::BYTES - here;
+        u4 f[AHEAD];
+        begin(key_at + there, value_at + here, f);
+        raise(odd_step, base + 32, was_lacking >> 2, edge, w_even);
+        step(key_at + there, value_at + here, f, even, odd_step, w_even, w_odd);
+        // past the last tile these are scores of whatever lies in LDS, all masked
+        edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
+        begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
+        raise(even, base + T::KEYS, lacking, edge, w_odd);
+        step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, odd_step, even, w_odd, w_even);
 
         if (odd) {
             // the values that are not finite reach the rows that see them as infinities (a NaN as both)
             wait_for_copies();
             __syncthreads();
-            again(base, buffer, now_missing);
+            again(base, buffer, was_lacking);
             __syncthreads();
             for (int t = 0; t < D / 32; ++t) {
                 fx16 plus, minus;
@@ -340,11 +397,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const int key = base + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
-                        sees[p] = now_missing >> k & 1 ? 0u
+                        sees[p] = was_lacking >> k & 1 ? 0u
                                                        : ((key >= lo && key < hi ? 0xFFFFu : 0u) |
                                                           (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u)) & M::ONES;
                     }
-                    const u4 v = value(k, t);
+                    const u4 v = value_piece(value_at + here, t, 16 * k * T::ROW);
                     plus = M::mma32(M::above(v), sees, plus);
                     minus = M::mma32(M::below(v), sees, minus);
                 }
@@ -357,9 +414,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
                     }
             }
         }
-        if constexpr (CODES) {
-            if (base + T::KEYS < k1) put(buffer ^ 1);
-        }
+        if (base + T::KEYS < k1) put(1, buffer ^ 1);
+        if (base + 2 * T::KEYS < k1) put(0, buffer);
     }
 
     if (wave0 + n > last) return;
