@@ -248,11 +248,12 @@ struct Step<D, int8_t> {
 
 // The lane's 8 keys of a step as word masks: pairs of 16-bit slots whose key lies in [lo, hi).
 __device__ inline u4 slots_in(int base, int j, int lo, int hi) {
+    const int from = lo - base - 4 * j, to = hi - base - 4 * j;
     u4 m;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const int key = base + (p < 2 ? 0 : 16) + 4 * j + 2 * (p % 2);
-        m[p] = (key >= lo && key < hi ? 0xFFFFu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+        const int in = (p < 2 ? 0 : 16) + 2 * (p % 2);
+        m[p] = (in >= from && in < to ? 0xFFFFu : 0u) | (in + 1 >= from && in + 1 < to ? 0xFFFF0000u : 0u);
     }
     return m;
 }
@@ -371,14 +372,14 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void strea
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float top = -INFINITY;
+            const int from = lo[i] - base - 4 * j, to = hi[i] - base - 4 * j;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     z[i][t][r] *= factor[i];
                     if (!full) {
-                        const int key = base + 16 * t + 4 * j + r;
-                        if (!there[t] || key < lo[i] || key >= hi[i]) z[i][t][r] = -INFINITY;
+                        if (!there[t] || 16 * t + r < from || 16 * t + r >= to) z[i][t][r] = -INFINITY;
                     }
                     top = fmaxf(top, z[i][t][r]);
                 }

@@ -56,6 +56,8 @@ struct Tile {
     static constexpr int PIECES = D / 8;               // of a row
     static constexpr int ROWS = 64 / PIECES;           // of 64 pieces
     static constexpr int LOADS = KEYS * PIECES / 256;  // for each lane
+    // Places are exclusive ors: place(row, piece) = place(row', piece) ^ place(row - row', 0) where row' are the row's
+    // bits within a load.
     // keys are read by rows: 16 rows' pieces of one place lie in 16 places
     static __device__ int key_place(int row, int piece) {
         return piece ^ (D == 64 ? (row >> 1) & 7 : row & 15);
@@ -177,37 +179,39 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // takes them
     u2 code[2][CODES ? T::LOADS : 1];
     _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    uint32_t load_at[2] = {(uint32_t)(in_load * T::ROW + 16 * T::key_place(in_load, piece)),
+                           (uint32_t)(in_load * T::ROW + 16 * T::value_place(in_load, piece))};
+    auto turn = [&](int side, int i) {
+        return 16u * (side ? T::value_place(i * T::ROWS, 0) : T::key_place(i * T::ROWS, 0));
+    };
     auto fetch = [&](int side, int64_t row, int buffer) {
+        asm volatile("" : "+v"(load_at[side]));  // a load's place is cheaper computed than kept
         const void* from = side ? a.c.v : a.c.k;
         if constexpr (CODES) {
             const int8_t* p = static_cast<const int8_t*>(from) + row * D;
             const _Float16* sc = (side ? a.c.vs : a.c.ks) + row * (D / 32);
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
-                const int rr = i * T::ROWS + in_load;
-                code[side][i] = *reinterpret_cast<const u2*>(p + rr * D + 8 * piece);
-                code_scale[side][i] = sc[rr * (D / 32) + piece / 4];
+                const int rr = i * T::ROWS;
+                code[side][i] = *reinterpret_cast<const u2*>(p + rr * D + 8 * (unsigned)lane);
+                code_scale[side][i] = sc[rr * (D / 32) + (unsigned)lane / 4];
             }
         } else {
             const uint8_t* p = static_cast<const uint8_t*>(from) + row * T::ROW;
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
-                const int rr = i * T::ROWS + in_load;
-                copy_to_lds(p + i * T::ROWS * T::ROW,
-                            in_load * T::ROW + 16 * (side ? T::value_place(rr, piece) : T::key_place(rr, piece)),
+                copy_to_lds(p + i * T::ROWS * T::ROW, load_at[side] ^ turn(side, i),
                             at + (buffer * 2 + side) * T::BYTES + (bring + i * T::ROWS) * T::ROW);
             }
         }
     };
     auto put = [&](int side, int buffer) {
         if constexpr (CODES) {
+            asm volatile("" : "+v"(load_at[side]));
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) {
-                const int rr = i * T::ROWS + in_load;
-                const int place = side ? T::value_place(rr, piece) : T::key_place(rr, piece);
-                *reinterpret_cast<u4*>(&lds[buffer][side][(bring + rr) * T::ROW + 16 * place]) =
-                    codes_to_f16(code[side][i], code_scale[side][i]);
-            }
+            for (int i = 0; i < T::LOADS; ++i)
+                *reinterpret_cast<u4*>(&lds[buffer][side][(bring + i * T::ROWS) * T::ROW] +
+                                       (load_at[side] ^ turn(side, i))) = codes_to_f16(code[side][i], code_scale[side][i]);
         }
     };
 
@@ -247,10 +251,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // `z` are scores of 32 keys at `base`: hidden ones go, the running maximum moves if it must, and with it the sums and the weights `w` still to be used.
     auto raise = [&](fx16& z, int base, uint32_t lacking, bool edge, u4(&w)[2]) {
         if (edge) {
+            const int from = lo - base - 4 * half, to = hi - base - 4 * half;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int in = 8 * (i / 4) + 4 * half + i % 4, key = base + in;
-                z[i] = key >= lo && key < hi && !(lacking >> (in / 16) & 1) ? z[i] : -INFINITY;
+                const int in = 8 * (i / 4) + i % 4;
+                z[i] = in >= from && in < to && !(lacking >> (in / 16) & 1) ? z[i] : -INFINITY;
             }
         }
         float top = z[0];
@@ -263,7 +268,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             m = up;
             l *= keep;
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t) o[t] *= keep;
+            for (int t = 0; t < D / 32; ++t) {
+                o[t] *= keep;
+                if constexpr (D == 256) asm volatile("" : "+a"(o[t]));  // back where the products keep them
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -393,13 +401,14 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
                 for (int i = 0; i < 16; ++i) plus[i] = minus[i] = 0.0f;
                 for (int k = 0; k < T::KEYS / 16; ++k) {
+                    const int first = lo - base - 16 * k - 4 * half, end = hi - base - 16 * k - 4 * half;
                     u4 sees;
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int key = base + 16 * k + 8 * (p / 2) + 4 * half + 2 * (p % 2);
+                        const int in = 8 * (p / 2) + 2 * (p % 2);
                         sees[p] = was_lacking >> k & 1 ? 0u
-                                                       : ((key >= lo && key < hi ? 0xFFFFu : 0u) |
-                                                          (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u)) & M::ONES;
+                                                       : ((in >= first && in < end ? 0xFFFFu : 0u) |
+                                                          (in + 1 >= first && in + 1 < end ? 0xFFFF0000u : 0u)) & M::ONES;
                     }
                     const u4 v = value_piece(value_at + here, t, 16 * k * T::ROW);
                     plus = M::mma32(M::above(v), sees, plus);
