@@ -177,8 +177,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     };
     // rows of one side (0 keys, 1 values) on their way to a buffer; of an 8-bit cache into registers, from which `put`
     // takes them
-    u2 code[2][CODES ? T::LOADS : 1];
-    _Float16 code_scale[2][CODES ? T::LOADS : 1];
+    // heads of 256 have no registers for both sides at once: keys are fetched when the values have been put
+    constexpr bool IN_TURN = CODES && D == 256;
+    u2 code[IN_TURN ? 1 : 2][CODES ? T::LOADS : 1];
+    _Float16 code_scale[IN_TURN ? 1 : 2][CODES ? T::LOADS : 1];
     uint32_t load_at[2] = {(uint32_t)(in_load * T::ROW + 16 * T::key_place(in_load, piece)),
                            (uint32_t)(in_load * T::ROW + 16 * T::value_place(in_load, piece))};
     auto turn = [&](int side, int i) {
@@ -193,8 +195,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
                 const int rr = i * T::ROWS;
-                code[side][i] = *reinterpret_cast<const u2*>(p + rr * D + 8 * (unsigned)lane);
-                code_scale[side][i] = sc[rr * (D / 32) + (unsigned)lane / 4];
+                code[IN_TURN ? 0 : side][i] = *reinterpret_cast<const u2*>(p + rr * D + 8 * (unsigned)lane);
+                code_scale[IN_TURN ? 0 : side][i] = sc[rr * (D / 32) + (unsigned)lane / 4];
             }
         } else {
             const uint8_t* p = static_cast<const uint8_t*>(from) + row * T::ROW;
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i)
                 *reinterpret_cast<u4*>(&lds[buffer][side][(bring + i * T::ROWS) * T::ROW] +
-                                       (load_at[side] ^ turn(side, i))) = codes_to_f16(code[side][i], code_scale[side][i]);
+                                       (load_at[side] ^ turn(side, i))) = codes_to_f16(code[IN_TURN ? 0 : side][i], code_scale[IN_TURN ? 0 : side][i]);
         }
     };
 
@@ -270,7 +272,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) {
                 o[t] *= keep;
-                if constexpr (D == 256) asm volatile("" : "+a"(o[t]));  // back where the products keep them
+                if constexpr (D == 256) {  // back where the products keep them, one at a time
+                    asm volatile("" : "+a"(o[t]));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k)
@@ -326,8 +331,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     look_up(k0);
     int64_t row = locate(k0, lacking);
     fetch(0, row, 0);
+    if (IN_TURN) put(0, 0);
     fetch(1, row, 0);
-    put(0, 0);
+    if (!IN_TURN) put(0, 0);
     put(1, 0);
     look_up(k0 + T::KEYS);
     wait_for_copies();
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         if (base + T::KEYS < k1) fetch(1, row, buffer ^ 1);
         if (base + 2 * T::KEYS < k1) {
             row = locate(base + 2 * T::KEYS, next_lacking);
-            fetch(0, row, buffer);
+            if (!IN_TURN) fetch(0, row, buffer);
             look_up(base + 3 * T::KEYS);
         }
         asm volatile("" : "+v"(key_at), "+v"(value_at));  // the places along a row are cheaper computed than kept
@@ -384,6 +390,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         begin(key_at + there, value_at + here, f);
         raise(odd_step, base + 32, was_lacking >> 2, edge, w_even);
         step(key_at + there, value_at + here, f, even, odd_step, w_even, w_odd);
+        if (IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
+        if (IN_TURN && base + 2 * T::KEYS < k1) fetch(0, row, buffer);
         // past the last tile these are scores of whatever lies in LDS, all masked
         edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
         begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
                     }
             }
         }
-        if (base + T::KEYS < k1) put(1, buffer ^ 1);
+        if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
         if (base + 2 * T::KEYS < k1) put(0, buffer);
     }
 
