@@ -90,35 +90,20 @@ struct Step {
         return x;
     }
     __device__ void prepare_values() {}
-    // Whether a value in the slots of the mask is an infinity or NaN.
-    __device__ bool not_finite(u4 slots) const {
-        bool odd = false;
+    // Clears the values outside the slots of the mask and those that are not finite; whether there were such inside.
+    __device__ bool keep_finite(u4 slots) {
+        uint32_t odd = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (!(slots[e / 2] >> (16 * (e % 2)) & 1)) continue;
+            const uint32_t keep = slots[e / 2] >> (16 * (e % 2)) & 1 ? ~0u : 0u;
 #pragma unroll
-            for (int w = 0; w < OWN / 2; ++w) {
-                const uint32_t x = v[e][w / 4][w % 4];
-                odd = odd || (x & Matrix<KV>::EXPONENT) == Matrix<KV>::EXPONENT ||
-                      (x & (Matrix<KV>::EXPONENT << 16)) == Matrix<KV>::EXPONENT << 16;
+            for (int h = 0; h < (OWN / 8 ? OWN / 8 : 1); ++h) {
+                const u4 x = v[e][h] & keep, f = Matrix<KV>::finite(x), y = x ^ f;
+                odd |= y.x | y.y | y.z | y.w;
+                v[e][h] = f;
             }
         }
-        return odd;
-    }
-    // Clears the values in the slots outside the mask.
-    __device__ void keep_values(u4 slots) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int w = 0; w < OWN / 2; ++w)
-                if (!(slots[e / 2] >> (16 * (e % 2)) & 1)) v[e][w / 4][w % 4] = 0;
-    }
-    // Copies for the compiler: work on them is not moved ahead of the branch they are in.
-    __device__ void opaque() {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int h = 0; h < (OWN / 8 ? OWN / 8 : 1); ++h) asm volatile("" : "+v"(v[e][h]));
+        return odd != 0;
     }
     using Weight = KV;
 };
@@ -221,27 +206,19 @@ struct Step<D, int8_t> {
             x[p] = __builtin_bit_cast(uint32_t, code_pair(v[2 * p + 1][t / 4], v[2 * p][t / 4], t % 4) * pair[t / 8][p]);
         return x;
     }
-    __device__ bool not_finite(u4 slots) const {
+    // A code's value is not finite where its scale is not.
+    __device__ bool keep_finite(u4 slots) {
         bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-                odd = odd || ((slots[e / 2] >> (16 * (e % 2)) & 1) && (vs[e][h] & 0x7C00u) == 0x7C00u);
-        return odd;
-    }
-    __device__ void keep_values(u4 slots) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
-                pair[h][p] = __builtin_bit_cast(h2, __builtin_bit_cast(uint32_t, pair[h][p]) & slots[p]);
-    }
-    __device__ void opaque() {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int w = 0; w < WORDS; ++w) asm volatile("" : "+v"(v[e][w]));
+            for (int p = 0; p < 4; ++p) {
+                const u4 x{__builtin_bit_cast(uint32_t, pair[h][p]) & slots[p], 0, 0, 0};
+                const uint32_t f = Matrix<_Float16>::finite(x).x;
+                odd = odd || f != x.x;
+                pair[h][p] = __builtin_bit_cast(h2, f);
+            }
+        return odd;
     }
     using Weight = _Float16;
 };
@@ -259,10 +236,12 @@ __device__ inline u4 slots_in(int base, int j, int lo, int hi) {
 }
 
 template <int D, typename Q, typename KV, int NT>
-__global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void stream_attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_attention_kernel(AttentionArgs a) {
     constexpr int OWN = D / 16, PART = D == 64 ? 64 : 128;
     using W = typename Step<D, KV>::Weight;
     constexpr uint32_t ONES = Matrix<W>::ONES;
+    // values of an 8-bit cache are rounded, so weights are not: they go as two fp16 numbers, high and rest
+    constexpr bool EXACT = sizeof(KV) == 1;
     __shared__ float so[STREAM_WAVES][16][PART + 4];
     __shared__ float sm[STREAM_WAVES][16], sl[STREAM_WAVES][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -368,7 +347,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void strea
         step.scores(queries, z);
         if (next < k1) step.load_keys(a, next_row, n, j);
         const bool full = there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
-        u4 w[NT];
+        u4 w[NT], w_rest[EXACT ? NT : 1];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float top = -INFINITY;
@@ -397,53 +376,63 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D * NT > 256 ? 1 : 2) void strea
                 l[i] += p[e];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[i][e] = Matrix<W>::pack(p[2 * e], p[2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t both = Matrix<W>::pack(p[2 * e], p[2 * e + 1]);
+                w[i][e] = both;
+                if constexpr (EXACT) {
+                    const h2 high = __builtin_bit_cast(h2, both);
+                    w_rest[i][e] = Matrix<W>::pack(p[2 * e] - (float)high.x, p[2 * e + 1] - (float)high.y);
+                }
+            }
         }
         step.prepare_values();
-        // a weight of zero times an infinity is NaN: what no row sees is cleared, and where rows differ in what they see
-        // and a value is not finite, such values are left out of the product and reach the rows that see them as
-        // infinities (a NaN as both)
+        // a weight of zero times an infinity is NaN: what no row sees is cleared, and where rows differ in what they see,
+        // values that are not finite are left out of the product and reach the rows that see them after it
         bool odd = false;
+        u4 some{~0u, ~0u, ~0u, ~0u};
         if (!full) {
-            u4 some = slots_in(base, j, any_lo, any_hi);
+            some = slots_in(base, j, any_lo, any_hi);
             if (!there[0]) some.x = some.y = 0;
             if (!there[1]) some.z = some.w = 0;
-            step.keep_values(some);
-            odd = token0 != token1 && __any(step.not_finite(some));
+            odd = __any(step.keep_finite(some));
         }
-        if (!odd) {
 #pragma unroll
-            for (int t = 0; t < OWN; ++t) {
-                const u4 x = step.values(t);
+        for (int t = 0; t < OWN; ++t) {
+            const u4 x = step.values(t);
 #pragma unroll
-                for (int i = 0; i < NT; ++i) o[i][t] = Matrix<W>::mma16(x, w[i], o[i][t]);
-                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < NT; ++i) {
+                o[i][t] = Matrix<W>::mma16(x, w[i], o[i][t]);
+                if constexpr (EXACT) o[i][t] = Matrix<W>::mma16(x, w_rest[i], o[i][t]);
             }
-        } else {
-            step.opaque();
+            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (odd) {  // once more, as infinities (a NaN as both) to the rows that see them
+            step.load_values(a, row, n, j);
+            step.prepare_values();
 #pragma unroll
             for (int t = 0; t < OWN; ++t) {
-                const u4 x = step.values(t);
-                const u4 above = Matrix<W>::above(x), below = Matrix<W>::below(x), finite = Matrix<W>::finite(x);
+                const u4 x = step.values(t) & some;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const u4 sees = slots_in(base, j, lo[i], hi[i]) & ONES;
-                    const f4 plus = Matrix<W>::mma16(above, sees, f4{0, 0, 0, 0});
-                    const f4 minus = Matrix<W>::mma16(below, sees, f4{0, 0, 0, 0});
-                    o[i][t] = Matrix<W>::mma16(finite, w[i], o[i][t]);
+                    const f4 plus = Matrix<W>::mma16(Matrix<W>::above(x), sees, f4{0, 0, 0, 0});
+                    const f4 minus = Matrix<W>::mma16(Matrix<W>::below(x), sees, f4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         if (plus[r] > 0.0f) o[i][t][r] += INFINITY;
                         if (minus[r] > 0.0f) o[i][t][r] -= INFINITY;
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (next < k1) step.load_values(a, next_row, n, j);
         base = next;
-        there[0] = next_there[0];
-        there[1] = next_there[1];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            row[t] = next_row[t];
+            there[t] = next_there[t];
+        }
     }
 
     // the waves' sums join in LDS, 16 rows and up to 128 channels at a time, in the waves' order
