@@ -336,7 +336,15 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     if (base < k1) {
         find(base, row, there);
         step.load_keys(a, row, n, j);
+        __builtin_amdgcn_sched_barrier(0);  // keys first, as in the loop, or its waits count too few
         step.load_values(a, row, n, j);
+    }
+    // the queries are there before the loop begins: a wait for them inside it would be one for every load after them
+    if constexpr (D != 256) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) asm volatile("" : "+v"(queries.own[i][c]));
     }
     while (base < k1) {
         const int next = base + STEP_KEYS * STREAM_WAVES;
@@ -345,7 +353,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         find(next, next_row, next_there);
         f4 z[NT][2];
         step.scores(queries, z);
-        if (next < k1) step.load_keys(a, next_row, n, j);
+        // past the last step every lane reads one place: loads without a condition let the waits count exactly
+        const int next_n = next < k1 ? n : 0, next_j = next < k1 ? j : 0;
+        step.load_keys(a, next_row, next_n, next_j);
         const bool full = there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
         u4 w[NT], w_rest[EXACT ? NT : 1];
 #pragma unroll
@@ -426,7 +436,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 }
             }
         }
-        if (next < k1) step.load_values(a, next_row, n, j);
+        step.load_values(a, next_row, next_n, next_j);
         base = next;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
