@@ -1,5 +1,6 @@
 // attention.hip -- attention of new tokens over the paged cache: which kernel takes a call, how the keys are split, and
 // the joining of the splits.
+#include <stdlib.h>
 #include "attention_core.h"
 #include "attention_internal.h"
 #include "iq4xs_internal.h"
@@ -77,10 +78,13 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;
     if (g.window > 0 && g.window + most_q + 32 < span) span = g.window + most_q + 32;
-    // few rows: enough workgroups for three on every CU twice over, none with less than 128 keys (32 for a wave); many:
-    // for two on every CU, none with less than 512 keys
-    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, want = (p.tiles ? 6 : 2) * (int64_t)device_cu_count();
-    const int64_t least = p.tiles ? 128 : 512, most = (span + least - 1) / least;
+    // few rows: the workgroups that the CUs hold at once (by registers: 4, 2 or 1 for heads of 64, 128 or 256), in one
+    // round for one sequence, whose splits are alike, in more for several, which may differ; none with less than 128 keys
+    // (32 for a wave).  Many rows: for two on every CU, none with less than 512 keys.
+    static const int rounds = getenv("R") ? atoi(getenv("R")) : 1, rounds2 = getenv("R2") ? atoi(getenv("R2")) : 8;
+    const int64_t held = g.cache->head_dim == 64 ? 4 : g.cache->head_dim == 128 ? (getenv("H") ? atoi(getenv("H")) : 2) : 1;
+    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, least = p.tiles ? 128 : 512;
+    const int64_t want = (p.tiles ? (g.seqs == 1 ? rounds : rounds2) * held : 2) * device_cu_count(), most = (span + least - 1) / least;
     int64_t splits = (want + pairs - 1) / pairs;
     splits = splits < most ? splits : most;
     const int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;

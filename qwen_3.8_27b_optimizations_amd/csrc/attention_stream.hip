@@ -69,7 +69,7 @@ struct Step {
         }
     }
     template <int NT>
-    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2]) const {
+    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2], int) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -89,7 +89,7 @@ struct Step {
         }
         return x;
     }
-    __device__ void prepare_values() {}
+    __device__ void prepare_values(int) {}
     // Clears the values outside the slots of the mask and those that are not finite; whether there were such inside.
     __device__ bool keep_finite(u4 slots) {
         uint32_t odd = 0;
@@ -115,63 +115,72 @@ __device__ inline h2 code_pair(uint32_t hi, uint32_t lo, int b) {
     return __builtin_bit_cast(h2, w) - h2{(_Float16)1152, (_Float16)1152};
 }
 
+// Codes: a lane loads 16 of a key at once, so that a load's segments are whole 64-byte pieces, and lanes of the two halves
+// of the wave trade 8 of them, so that each product is over one group of 32.  The scales of the 32 keys and values of a
+// step are one load for the wave, lane l those of key l or value l - 32, and are handed round through LDS.
 template <int D>
 struct Step<D, int8_t> {
     static constexpr int OWN = D / 16, WORDS = D / 64, HALVES = D == 256 ? 2 : 1, GROUPS = D / 32;
-    u2 k[2][D / 32];
-    uint32_t ks[2][4 * GROUPS / 2];  // fp16 scales of this lane's four keys of a tile, all groups
+    u4 k[2][D / 64];
     uint32_t v[8][WORDS];
-    uint16_t vs[8][HALVES];
     h2 pair[HALVES][4];
+    typedef _Float16 Scales __attribute__((ext_vector_type(GROUPS)));
+    Scales scale;
+    _Float16* shared;  // [64][GROUPS], of this wave
 
     __device__ void load_keys(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
         const int8_t* p = static_cast<const int8_t*>(a.c.k);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-                k[t][c] = *reinterpret_cast<const u2*>(p + row[t] * D + n * D + 32 * c + 8 * j);
-            const u4* s = reinterpret_cast<const u4*>(a.c.ks + (row[t] + 4 * j) * GROUPS);
-#pragma unroll
-            for (int i = 0; i < GROUPS / 2; ++i) {
-                const u4 w = s[i];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) ks[t][4 * i + x] = w[x];
-            }
-        }
+            for (int c = 0; c < D / 64; ++c)
+                k[t][c] = *reinterpret_cast<const u4*>(p + row[t] * D + n * D + 64 * c + 16 * j);
+        // row[j % 2], as a sum: the compiler would index the pair in memory
+        const int64_t mine = row[0] + ((row[1] - row[0]) & -(int64_t)(j & 1));
+        const _Float16* s = (j < 2 ? a.c.ks : a.c.vs) + (mine + n) * GROUPS;
+        scale = *reinterpret_cast<const Scales*>(s);
     }
     __device__ void load_values(const AttentionArgs& a, const int64_t (&row)[2], int n, int j) {
         const int8_t* p = static_cast<const int8_t*>(a.c.v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int64_t r = row[e / 4] + 4 * j + e % 4;
+            const int8_t* r = p + row[e / 4] * D + (4 * j + e % 4) * D;
             if constexpr (OWN == 4) {
-                v[e][0] = *reinterpret_cast<const uint32_t*>(p + r * D + 4 * n);
+                v[e][0] = *reinterpret_cast<const uint32_t*>(r + 4 * n);
             } else {
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
-                    const u2 w = *reinterpret_cast<const u2*>(p + r * D + 128 * h + 8 * n);
+                    const u2 w = *reinterpret_cast<const u2*>(r + 128 * h + 8 * n);
                     v[e][2 * h] = w.x;
                     v[e][2 * h + 1] = w.y;
                 }
             }
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(a.c.vs) + r * GROUPS;
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) vs[e][h] = s[OWN == 4 ? n / 8 : 4 * h + n / 4];
         }
     }
     template <int NT>
-    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2]) const {
+    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2], int lane) const {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        *reinterpret_cast<Scales*>(shared + lane * GROUPS) = scale;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            // of the lane's four keys of the tile
+            const Scales* from = reinterpret_cast<const Scales*>(shared + (16 * t + 4 * (lane / 16)) * GROUPS);
+            const Scales ks[4] = {from[0], from[1], from[2], from[3]};
 #pragma unroll
             for (int i = 0; i < NT; ++i) s[i][t] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < GROUPS; ++c) {
+                // lanes 0 to 31 hold channels 64 (c / 2) + 0..31 of the key, the others 32..63
+                const u4 both = k[t][c / 2] ^ 0x80808080u;
+                const u2 x0 = __builtin_amdgcn_permlane32_swap(both.x, both.z, false, false);
+                const u2 x1 = __builtin_amdgcn_permlane32_swap(both.y, both.w, false, false);
                 u4 x;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const uint32_t b = (w < 2 ? k[t][c].x : k[t][c].y) ^ 0x80808080u;
+                    const uint32_t b = w < 2 ? (c % 2 ? x0.y : x0.x) : (c % 2 ? x1.y : x1.x);
                     const uint32_t z = __builtin_amdgcn_perm(b, b, w % 2 ? 0x0C030C02u : 0x0C010C00u) | 0x64006400u;
                     x[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, z) - h2{(_Float16)1152, (_Float16)1152});
                 }
@@ -180,15 +189,14 @@ struct Step<D, int8_t> {
                     const f4 part = Matrix<_Float16>::mma16(x, q.at(i, c), f4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int at = r * GROUPS + c;
-                        const _Float16 scale = __builtin_bit_cast(h2, ks[t][at / 2])[at % 2];
-                        s[i][t][r] = __builtin_fmaf((float)scale, part[r], s[i][t][r]);
+                        s[i][t][r] = __builtin_fmaf((float)ks[r][c], part[r], s[i][t][r]);
                     }
                 }
             }
         }
     }
-    __device__ void prepare_values() {
+    __device__ void prepare_values(int lane) {
+        const int n = lane % 16, j = lane / 16;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -196,8 +204,11 @@ struct Step<D, int8_t> {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
-                pair[h][p] = __builtin_bit_cast(h2, (uint32_t)vs[2 * p][h] | ((uint32_t)vs[2 * p + 1][h] << 16));
+            for (int p = 0; p < 4; ++p) {
+                const _Float16* from = shared + (32 + 16 * (p / 2) + 4 * j + 2 * (p % 2)) * GROUPS +
+                                       (OWN == 4 ? n / 8 : 4 * h + n / 4);
+                pair[h][p] = h2{from[0], from[GROUPS]};
+            }
     }
     __device__ u4 values(int t) const {
         u4 x;
@@ -278,7 +289,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         token[i] = r / a.group;
         lo[i] = least_key(a, s, total_fresh, token[i]);
         hi[i] = end_key(a, s, total_fresh, token[i]);
-        const int64_t at = (int64_t)(s.first + token[i]) * a.q_stride + (head * a.group + r % a.group) * D + 8 * j;
+        // the channels that the keys' lanes hold
+        const int channel = sizeof(KV) == 1 ? 16 * (j % 2) + 8 * (j / 2) : 8 * j;
+        const int64_t at = (int64_t)(s.first + token[i]) * a.q_stride + (head * a.group + r % a.group) * D + channel;
         const u4* p = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q) + at);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) q[i][c] = p[4 * c];
@@ -330,6 +343,10 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     };
 
     Step<D, KV> step;
+    if constexpr (sizeof(KV) == 1) {
+        __shared__ __attribute__((aligned(16))) _Float16 scales[STREAM_WAVES][64 * (D / 32)];
+        step.shared = scales[wave];
+    }
     int64_t row[2];
     bool there[2];
     int base = k0 + STEP_KEYS * wave;
@@ -352,7 +369,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         bool next_there[2];
         find(next, next_row, next_there);
         f4 z[NT][2];
-        step.scores(queries, z);
+        step.scores(queries, z, lane);
         // past the last step every lane reads one place: loads without a condition let the waits count exactly
         const int next_n = next < k1 ? n : 0, next_j = next < k1 ? j : 0;
         step.load_keys(a, next_row, next_n, next_j);
@@ -395,7 +412,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 }
             }
         }
-        step.prepare_values();
+        step.prepare_values(lane);
         // a weight of zero times an infinity is NaN: what no row sees is cleared, and where rows differ in what they see,
         // values that are not finite are left out of the product and reach the rows that see them after it
         bool odd = false;
@@ -418,7 +435,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         }
         if (odd) {  // once more, as infinities (a NaN as both) to the rows that see them
             step.load_values(a, row, n, j);
-            step.prepare_values();
+            step.prepare_values(lane);
 #pragma unroll
             for (int t = 0; t < OWN; ++t) {
                 const u4 x = step.values(t) & some;
