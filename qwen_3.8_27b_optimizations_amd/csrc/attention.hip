@@ -1,6 +1,5 @@
 // attention.hip -- attention of new tokens over the paged cache: which kernel takes a call, how the keys are split, and
 // the joining of the splits.
-#include <stdlib.h>
 #include "attention_core.h"
 #include "attention_internal.h"
 #include "iq4xs_internal.h"
@@ -70,6 +69,8 @@ struct AttentionPlan {
     int64_t grid;
 };
 
+static int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
+
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
@@ -78,15 +79,23 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;
     if (g.window > 0 && g.window + most_q + 32 < span) span = g.window + most_q + 32;
-    // few rows: the workgroups that the CUs hold at once (by registers: 4, 2 or 1 for heads of 64, 128 or 256), in one
-    // round for one sequence, whose splits are alike, in more for several, which may differ; none with less than 128 keys
-    // (32 for a wave).  Many rows: for two on every CU, none with less than 512 keys.
-    static const int rounds = getenv("R") ? atoi(getenv("R")) : 1, rounds2 = getenv("R2") ? atoi(getenv("R2")) : 8;
-    const int64_t held = g.cache->head_dim == 64 ? 4 : g.cache->head_dim == 128 ? (getenv("H") ? atoi(getenv("H")) : 2) : 1;
-    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, least = p.tiles ? 128 : 512;
-    const int64_t want = (p.tiles ? (g.seqs == 1 ? rounds : rounds2) * held : 2) * device_cu_count(), most = (span + least - 1) / least;
-    int64_t splits = (want + pairs - 1) / pairs;
-    splits = splits < most ? splits : most;
+    const int64_t pairs = g.seqs * g.cache->heads * row_tiles, cus = device_cu_count();
+    int64_t splits;
+    if (p.tiles) {
+        // One sequence, whose splits are alike: the workgroups that the CUs hold at once (by registers; one for each CU
+        // keeps enough 16-bit keys on their way), none with less than 128 keys, 32 for a wave.  Several, which may
+        // differ: that many too, or eight times as many of 512 keys at least (1024 of heads of 256), whichever is more.
+        const bool codes = g.cache->type == IQ4XS_TYPE_Q8;
+        const int64_t held = g.cache->head_dim == 64 ? 4 : g.cache->head_dim == 256 ? 1 : p.tiles == 2 ? 2 : codes ? 3 : 2;
+        const int64_t one = g.seqs == 1 && !codes && g.cache->head_dim == 128 ? 1 : held;
+        const int64_t once = at_most((one * cus + pairs - 1) / pairs, (span + 127) / 128);
+        const int64_t least = g.cache->head_dim == 256 ? 1024 : 512;
+        const int64_t more = at_most((8 * held * cus + pairs - 1) / pairs, (span + least - 1) / least);
+        splits = g.seqs > 1 && more > once ? more : once;
+    } else {
+        // two workgroups on every CU, none with less than 512 keys
+        splits = at_most((2 * cus + pairs - 1) / pairs, (span + 511) / 512);
+    }
     const int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
     p.splits = (int)((span + chunk - 1) / chunk);
     p.chunk = (int)chunk;

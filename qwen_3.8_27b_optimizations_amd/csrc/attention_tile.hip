@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 
     // `z` are scores of 32 keys at `base`: hidden ones go, the running maximum moves if it must, and with it the sums and the weights `w` still to be used.
     auto raise = [&](fx16& z, int base, uint32_t lacking, bool edge, u4(&w)[2]) {
-        if (edge) {
+        if (__builtin_expect(edge, 0)) {
             const int from = lo - base - 4 * half, to = hi - base - 4 * half;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
         top *= factor;
-        if (__any(top > m + 8.0f)) {
+        if (__builtin_expect(__any(top > m + 8.0f), 0)) {
             // whole powers of two, so that scaling the 16-bit weights is exact
             const float up = fmaxf(ceilf(max_of_halves(top)), m), keep = __builtin_amdgcn_exp2f(m - up);
             m = up;
@@ -338,14 +338,14 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     look_up(k0 + T::KEYS);
     wait_for_copies();
     __syncthreads();
-    fx16 even, odd_step;
+    fx16 even, uneven;
     u4 w_even[2] = {}, w_odd[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) even[i] = odd_step[i] = 0.0f;
+    for (int i = 0; i < 16; ++i) even[i] = uneven[i] = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
         even = M::mma32(key_piece(key_at, c, 0), q[c], even);
-        odd_step = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], odd_step);
+        uneven = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], uneven);
     }
     bool edge = lacking != 0 || k0 < all_lo || k0 + T::KEYS > all_hi;
     raise(even, k0, lacking, edge, w_even);
@@ -357,23 +357,28 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         put(0, 1);
         look_up(k0 + 2 * T::KEYS);
     }
+    if constexpr (D == 256) {  // with the sums, where the products read them and nothing else does
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) asm volatile("" : "+a"(q[c]));
+    }
+    bool odd = false;
     int buffer = 0;
     for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
         wait_for_copies();
         __syncthreads();
         // A weight of zero times an infinity is NaN.  Where rows differ in what they see, values that no row sees and
-        // values that are not finite are cleared in LDS; the latter come again after the tile's products.
-        bool odd = false;
-        if (edge) {
+        // values that are not finite are cleared in LDS; the latter come again after the last tile.
+        if (__builtin_expect(edge, 0)) {
+            bool some = false;
             for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
                 const int key = base + i / T::PIECES;
                 u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
                 const bool seen = key >= any_lo && key < any_hi && !(lacking >> (i / T::PIECES / 16) & 1);
                 const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
-                odd = odd || (seen && (x.x | x.y | x.z | x.w) != 0);
+                some = some || (seen && (x.x | x.y | x.z | x.w) != 0);
                 *p = f;
             }
-            odd = __syncthreads_or(odd);
+            odd = __syncthreads_or(some) || odd;
         }
         const uint32_t was_lacking = lacking;
         lacking = next_lacking;
@@ -388,22 +393,32 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         const uint32_t here = buffer * 2 * T::BYTES, there = 2 * T::BYTES - here;
         u4 f[AHEAD];
         begin(key_at + there, value_at + here, f);
-        raise(odd_step, base + 32, was_lacking >> 2, edge, w_even);
-        step(key_at + there, value_at + here, f, even, odd_step, w_even, w_odd);
+        raise(uneven, base + 32, was_lacking >> 2, edge, w_even);
+        step(key_at + there, value_at + here, f, even, uneven, w_even, w_odd);
         if (IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
         if (IN_TURN && base + 2 * T::KEYS < k1) fetch(0, row, buffer);
         // past the last tile these are scores of whatever lies in LDS, all masked
         edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
         begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
         raise(even, base + T::KEYS, lacking, edge, w_odd);
-        step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, odd_step, even, w_odd, w_even);
+        step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, uneven, even, w_odd, w_even);
 
-        if (odd) {
-            // the values that are not finite reach the rows that see them as infinities (a NaN as both)
-            wait_for_copies();
+        if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
+        if (base + 2 * T::KEYS < k1) put(0, buffer);
+    }
+
+    if (__builtin_expect(odd, 0)) {
+        // the values that are not finite reach the rows that see them as infinities (a NaN as both)
+        wait_for_copies();
+        for (int base = k0; base < k1; base += T::KEYS) {
+            look_up(base);
+            uint32_t out;
+            locate(base, out);
+            if (out == 0 && base >= all_lo && base + T::KEYS <= all_hi) continue;
             __syncthreads();
-            again(base, buffer, was_lacking);
+            again(base, 0, out);
             __syncthreads();
+#pragma unroll
             for (int t = 0; t < D / 32; ++t) {
                 fx16 plus, minus;
 #pragma unroll
@@ -414,27 +429,22 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const int in = 8 * (p / 2) + 2 * (p % 2);
-                        sees[p] = was_lacking >> k & 1 ? 0u
-                                                       : ((in >= first && in < end ? 0xFFFFu : 0u) |
-                                                          (in + 1 >= first && in + 1 < end ? 0xFFFF0000u : 0u)) & M::ONES;
+                        sees[p] = out >> k & 1 ? 0u
+                                               : ((in >= first && in < end ? 0xFFFFu : 0u) |
+                                                  (in + 1 >= first && in + 1 < end ? 0xFFFF0000u : 0u)) & M::ONES;
                     }
-                    const u4 v = value_piece(value_at + here, t, 16 * k * T::ROW);
+                    const u4 v = value_piece(value_at, t, 16 * k * T::ROW);
                     plus = M::mma32(M::above(v), sees, plus);
                     minus = M::mma32(M::below(v), sees, minus);
                 }
 #pragma unroll
-                for (int u = 0; u < D / 32; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (u == t && plus[i] > 0.0f) o[u][i] += INFINITY;
-                        if (u == t && minus[i] > 0.0f) o[u][i] -= INFINITY;
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    if (plus[i] > 0.0f) o[t][i] += INFINITY;
+                    if (minus[i] > 0.0f) o[t][i] -= INFINITY;
+                }
             }
         }
-        if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
-        if (base + 2 * T::KEYS < k1) put(0, buffer);
     }
-
     if (wave0 + n > last) return;
     l = sum_of_halves(l);
     const int64_t out = (int64_t)(s.first + token) * a.q_heads + query_head;
