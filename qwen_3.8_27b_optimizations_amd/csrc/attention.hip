@@ -74,7 +74,16 @@ static int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
-    p.tiles = most_q * group <= 16 ? 1 : most_q * group <= 32 ? 2 : 0;
+    // Where the kernel of few rows ends: with 16-bit caches at two 16-row tiles, beyond which reading the keys again for
+    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows (72
+    // against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys; one tile at a time where
+    // two do not fit the registers or leave the second half empty.
+    const int64_t rows = most_q * group;
+    const bool codes = g.cache->type == IQ4XS_TYPE_Q8;
+    if (rows <= 16 || (codes && rows <= 48 && (rows > 32 || g.cache->head_dim == 256)))
+        p.tiles = 1;
+    else
+        p.tiles = rows <= 32 ? 2 : 0;
     const int64_t tile = p.tiles ? 16 * p.tiles : 128, row_tiles = (most_q * group + tile - 1) / tile;
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;
@@ -85,7 +94,6 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
         // One sequence, whose splits are alike: the workgroups that the CUs hold at once (by registers; one for each CU
         // keeps enough 16-bit keys on their way), none with less than 128 keys, 32 for a wave.  Several, which may
         // differ: that many too, or eight times as many of 512 keys at least (1024 of heads of 256), whichever is more.
-        const bool codes = g.cache->type == IQ4XS_TYPE_Q8;
         const int64_t held = g.cache->head_dim == 64 ? 4 : g.cache->head_dim == 256 ? 1 : p.tiles == 2 ? 2 : codes ? 3 : 2;
         const int64_t one = g.seqs == 1 && !codes && g.cache->head_dim == 128 ? 1 : held;
         const int64_t once = at_most((one * cus + pairs - 1) / pairs, (span + 127) / 128);

@@ -89,6 +89,7 @@ struct Step {
         }
         return x;
     }
+    __device__ void share_scales(int) {}
     __device__ void prepare_values(int) {}
     // Clears the values outside the slots of the mask and those that are not finite; whether there were such inside.
     __device__ bool keep_finite(u4 slots) {
@@ -157,13 +158,15 @@ struct Step<D, int8_t> {
             }
         }
     }
-    template <int NT>
-    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2], int lane) const {
+    __device__ void share_scales(int lane) const {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         *reinterpret_cast<Scales*>(shared + lane * GROUPS) = scale;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+    }
+    template <int NT>
+    __device__ void scores(const Queries<D, NT>& q, f4 (&s)[NT][2], int lane) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             // of the lane's four keys of the tile
@@ -342,6 +345,15 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         }
     };
 
+    // the lane's slots of a step whose keys some row sees
+    auto seen = [&](int base, const bool(&there)[2]) {
+        u4 some = slots_in(base, j, any_lo, any_hi);
+        if (!there[0]) some.x = some.y = 0;
+        if (!there[1]) some.z = some.w = 0;
+        return some;
+    };
+
+    bool odd = false;
     Step<D, KV> step;
     if constexpr (sizeof(KV) == 1) {
         __shared__ __attribute__((aligned(16))) _Float16 scales[STREAM_WAVES][64 * (D / 32)];
@@ -369,6 +381,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         bool next_there[2];
         find(next, next_row, next_there);
         f4 z[NT][2];
+        step.share_scales(lane);
         step.scores(queries, z, lane);
         // past the last step every lane reads one place: loads without a condition let the waits count exactly
         const int next_n = next < k1 ? n : 0, next_j = next < k1 ? j : 0;
@@ -384,12 +397,12 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     z[i][t][r] *= factor[i];
-                    if (!full) {
+                    if (__builtin_expect(!full, 0)) {
                         if (!there[t] || 16 * t + r < from || 16 * t + r >= to) z[i][t][r] = -INFINITY;
                     }
                     top = fmaxf(top, z[i][t][r]);
                 }
-            if (__any(top > m[i] + 8.0f)) {
+            if (__builtin_expect(__any(top > m[i] + 8.0f), 0)) {
                 const float up = fmaxf(max_of_quarters(top), m[i]), keep = __builtin_amdgcn_exp2f(m[i] - up);
                 m[i] = up;
                 l[i] *= keep;
@@ -413,16 +426,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
             }
         }
         step.prepare_values(lane);
-        // a weight of zero times an infinity is NaN: what no row sees is cleared, and where rows differ in what they see,
-        // values that are not finite are left out of the product and reach the rows that see them after it
-        bool odd = false;
-        u4 some{~0u, ~0u, ~0u, ~0u};
-        if (!full) {
-            some = slots_in(base, j, any_lo, any_hi);
-            if (!there[0]) some.x = some.y = 0;
-            if (!there[1]) some.z = some.w = 0;
-            odd = __any(step.keep_finite(some));
-        }
+        // a weight of zero times an infinity is NaN: where rows differ in what they see, what no row sees and what is not
+        // finite is cleared; the latter comes again after the last step
+        if (__builtin_expect(!full, 0)) odd = step.keep_finite(seen(base, there)) || odd;
 #pragma unroll
         for (int t = 0; t < OWN; ++t) {
             const u4 x = step.values(t);
@@ -433,12 +439,24 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
             }
             if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        if (odd) {  // once more, as infinities (a NaN as both) to the rows that see them
+        step.load_values(a, next_row, next_n, next_j);
+        base = next;
+        there[0] = next_there[0];
+        there[1] = next_there[1];
+    }
+
+    if (__builtin_expect(__any(odd), 0)) {
+        // values that are not finite reach the rows that see them as infinities (a NaN as both)
+        for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
+            find(base, row, there);
+            if (there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi) continue;
+            step.load_keys(a, row, n, j);
             step.load_values(a, row, n, j);
+            step.share_scales(lane);
             step.prepare_values(lane);
 #pragma unroll
             for (int t = 0; t < OWN; ++t) {
-                const u4 x = step.values(t) & some;
+                const u4 x = step.values(t) & seen(base, there);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const u4 sees = slots_in(base, j, lo[i], hi[i]) & ONES;
@@ -452,13 +470,6 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        }
-        step.load_values(a, next_row, next_n, next_j);
-        base = next;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            row[t] = next_row[t];
-            there[t] = next_there[t];
         }
     }
 
@@ -526,6 +537,8 @@ void launch_types(const AttentionArgs& a, int type, int cache_type, dim3 grid, h
         hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, _Float16, NT>), grid, block, 0, stream, a);
     else if (cache_type == IQ4XS_TYPE_BF16)
         hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, __bf16, NT>), grid, block, 0, stream, a);
+    else if constexpr (D == 256 && NT == 2)
+        return;  // not asked for: two tiles of codes do not fit the registers
     else if (type == IQ4XS_TYPE_F16)
         hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, int8_t, NT>), grid, block, 0, stream, a);
     else
