@@ -333,33 +333,40 @@ _QK = struct.Struct("@PPPqqqPPPPPPPqiiiiiiif")
 _ATTENTION = struct.Struct("@PPPPPPPqqqqqqqiiiif")
 
 
+_TYPES = {}  # torch dtype -> TYPE_*, filled once a GPU has been seen
+
+
 def _types(torch):
-    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if not _TYPES:
+        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    return _TYPES
 
 
-def _rows(t, name: str, heads: int | None = None, d: int | None = None):
+def _here(torch, t) -> int:
+    """The GPU of a tensor, which must be the current one: the calls launch there.  (A tensor on a GPU says that torch is
+    initialised, so the handles below need no checks of their own: 0.3 us of a call's host time against 1.3.)"""
+    here = t.get_device()
+    if here < 0 or torch._C._cuda_getDevice() != here:
+        raise ValueError("tensors must be on the current GPU")
+    return here
+
+
+def _rows(t, name: str):
     """Shape and token stride of [tokens][heads][head] whose heads lie one after another."""
-    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
-        raise ValueError(f"{name} must be [tokens, heads, head] with a token's heads one after another")
-    if (heads is not None and t.size(1) != heads) or (d is not None and t.size(2) != d):
-        raise ValueError(f"{name} must be [tokens, {heads}, {d}]")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head]")
+    (tokens, heads, d), (step, between, within) = t.shape, t.stride()
+    if within != 1 or between != d:
+        raise ValueError(f"{name}: a token's heads must lie one after another")
     # the stride of a single token says nothing
-    return t.size(0), t.size(1), t.size(2), t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+    return tokens, heads, d, step if tokens > 1 else heads * d
 
 
-def _whole(t, name: str, dtype, *shape) -> int:
-    """Address of a contiguous tensor of that type and shape."""
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)}")
+def _whole(t, name: str, dtype, shape, here: int) -> int:
+    """Address of a contiguous tensor of that type and shape on GPU `here`."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != here:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on the current GPU")
     return t.data_ptr()
-
-
-def _one_device(torch, *tensors) -> None:
-    """The calls launch on the current device."""
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError("every tensor must be on the current GPU")
 
 
 class KVCache:
@@ -380,18 +387,17 @@ class KVCache:
             raise ValueError("head must be 64, 128 or 256")
         if self.page < 16 or self.page & (self.page - 1) or not 0 < self.pages * self.page < 1 << 31:
             raise ValueError("page must be a power of two of at least 16, and the cache hold 1 to 2^31 - 1 tokens")
-        ptrs = [_whole(t, name, k_pages.dtype, *k_pages.shape) for t, name in ((k_pages, "k_pages"),
-                                                                              (v_pages, "v_pages"))]
+        self.device = torch.cuda.current_device()
+        ptrs = [_whole(t, name, k_pages.dtype, k_pages.shape, self.device)
+                for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"))]
         if (self.type == TYPE_Q8) != (k_scales is not None) or (k_scales is None) != (v_scales is None):
             raise ValueError("int8 pages need k_scales and v_scales, other pages take none")
         if self.type == TYPE_Q8:
             shape = (self.pages, self.heads, self.page, self.head_dim // 32)
-            ptrs += [_whole(k_scales, "k_scales", torch.float16, *shape),
-                     _whole(v_scales, "v_scales", torch.float16, *shape)]
+            ptrs += [_whole(t, name, torch.float16, shape, self.device)
+                     for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales"))]
         else:
             ptrs += [0, 0]
-        _one_device(torch, k_pages, v_pages, k_scales, v_scales)
-        self.device = k_pages.get_device()
         self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
         self._struct = ctypes.create_string_buffer(
             _CACHE.pack(*ptrs, self.pages, self.heads, self.page, self.head_dim, self.type), _CACHE.size)
@@ -399,40 +405,41 @@ class KVCache:
 
 
 def _qk(torch, q, k, v, pos, slots, cache, freqs, q_gamma, k_gamma, eps, rope, out_type):
-    """Packed arguments and outputs of the two calls below."""
+    """Packed arguments and outputs of the two calls below, and their stream."""
+    here = _here(torch, q)
     types = _types(torch)
+    kind = q.dtype
+    out_type = kind if out_type is None else out_type
+    if kind not in types or out_type not in types or k.dtype != kind:
+        raise ValueError("q and k must have one type and out_type be one: float32, float16 or bfloat16")
     tokens, hq, d, q_stride = _rows(q, "q")
-    kt, hk, _, k_stride = _rows(k, "k", None, d)
-    if kt != tokens or k.dtype != q.dtype or q.dtype not in types:
-        raise ValueError("q and k must hold the same tokens in one type (float32, float16 or bfloat16)")
-    out_type = q.dtype if out_type is None else out_type
-    if out_type not in types:
-        raise ValueError("out_type must be float32, float16 or bfloat16")
+    kt, hk, kd, k_stride = _rows(k, "k")
+    if kt != tokens or kd != d or k.get_device() != here:
+        raise ValueError("q and k must hold the same tokens and head sizes, on the current GPU")
     if rope not in (ROPE_HALF, ROPE_INTERLEAVED):
         raise ValueError("rope must be ROPE_HALF or ROPE_INTERLEAVED")
     rot = 0 if freqs is None else 2 * freqs.numel()
     if rot > d or rot % 16:
         raise ValueError("freqs must hold a multiple of 8 frequencies, at most one for each two channels")
-    fp = _whole(freqs, "freqs", torch.float64, rot // 2) if rot else 0
-    gq = 0 if q_gamma is None else _whole(q_gamma, "q_gamma", torch.float32, d)
-    gk = 0 if k_gamma is None else _whole(k_gamma, "k_gamma", torch.float32, d)
-    _one_device(torch, q, k, v, pos, slots, freqs, q_gamma, k_gamma)
-    q_out = torch.empty((tokens, hq, d), dtype=out_type, device=q.device)
-    k_out, vp, v_stride, sp = None, 0, 0, 0
+    fp = _whole(freqs, "freqs", torch.float64, (rot // 2,), here) if rot else 0
+    gq = 0 if q_gamma is None else _whole(q_gamma, "q_gamma", torch.float32, (d,), here)
+    gk = 0 if k_gamma is None else _whole(k_gamma, "k_gamma", torch.float32, (d,), here)
+    q_out = q.new_empty((tokens, hq, d), dtype=out_type)
+    k_out, kp, vp, v_stride, sp = None, 0, 0, 0, 0
     if cache is None:
-        k_out = torch.empty((tokens, hk, d), dtype=out_type, device=q.device)
+        k_out = q.new_empty((tokens, hk, d), dtype=out_type)
+        kp = k_out.data_ptr()
     else:
-        if cache.device != q.get_device() or cache.heads != hk or cache.head_dim != d:
-            raise ValueError("the cache must hold k's heads, on the same GPU")
-        vt, _, _, v_stride = _rows(v, "v", hk, d)
-        if vt != tokens or v.dtype != q.dtype:
-            raise ValueError("v must hold the same tokens as k in the same type")
-        vp, sp = v.data_ptr(), _whole(slots, "slots", torch.int64, tokens)
+        if cache.device != here or cache.heads != hk or cache.head_dim != d:
+            raise ValueError("the cache must hold k's heads, on the current GPU")
+        vt, vh, vd, v_stride = _rows(v, "v")
+        if (vt, vh, vd) != (tokens, hk, d) or v.dtype != kind or v.get_device() != here:
+            raise ValueError("v must be as k")
+        vp, sp = v.data_ptr(), _whole(slots, "slots", torch.int64, (tokens,), here)
     args = _QK.pack(q.data_ptr(), k.data_ptr(), vp, q_stride, k_stride, v_stride,
-                    _whole(pos, "pos", torch.int32, tokens), fp, gq, gk, sp, q_out.data_ptr(),
-                    0 if k_out is None else k_out.data_ptr(), tokens, hq, hk, d, rot, rope, types[q.dtype],
-                    types[out_type], eps)
-    return args, q_out, k_out
+                    _whole(pos, "pos", torch.int32, (tokens,), here), fp, gq, gk, sp, q_out.data_ptr(), kp, tokens, hq,
+                    hk, d, rot, rope, types[kind], types[out_type], eps)
+    return args, q_out, k_out, torch._C._cuda_getCurrentRawStream(here)
 
 
 def qk_norm_rope(q, k, pos, freqs=None, q_gamma=None, k_gamma=None, eps: float = 1e-6, rope: int = ROPE_HALF,
@@ -442,8 +449,8 @@ def qk_norm_rope(q, k, pos, freqs=None, q_gamma=None, k_gamma=None, eps: float =
 
     A token's heads lie one after another; tokens may be strided (views of a fused projection)."""
     torch = _torch()
-    args, q_out, k_out = _qk(torch, q, k, None, pos, None, None, freqs, q_gamma, k_gamma, eps, rope, out_type)
-    lib().check("iq4xs_qk_norm_rope", args, _stream(torch))
+    args, q_out, k_out, stream = _qk(torch, q, k, None, pos, None, None, freqs, q_gamma, k_gamma, eps, rope, out_type)
+    lib().check("iq4xs_qk_norm_rope", args, stream)
     return q_out, k_out
 
 
@@ -452,8 +459,8 @@ def qk_norm_rope_append(q, k, v, pos, slots, cache, freqs=None, q_gamma=None, k_
     """qk_norm_rope with k and v written to the cache at slots [tokens] (int64; negative or past the cache: the token is
     not stored).  Returns the new q."""
     torch = _torch()
-    args, q_out, _ = _qk(torch, q, k, v, pos, slots, cache, freqs, q_gamma, k_gamma, eps, rope, out_type)
-    lib().check("iq4xs_qk_norm_rope_append", args, cache._address, _stream(torch))
+    args, q_out, _, stream = _qk(torch, q, k, v, pos, slots, cache, freqs, q_gamma, k_gamma, eps, rope, out_type)
+    lib().check("iq4xs_qk_norm_rope_append", args, cache._address, stream)
     return q_out
 
 
@@ -467,13 +474,17 @@ def kv_gather(cache, table, starts, total: int, out_type=None):
         out_type = torch.float16 if cache.type == TYPE_Q8 else cache.k_pages.dtype
     if out_type not in types or total < 0:
         raise ValueError("out_type must be float32, float16 or bfloat16, and total not negative")
+    here = _here(torch, table)
     seqs = starts.numel() - 1
     width = table.size(1) if table.dim() == 2 else 0
-    tp, sp = _whole(table, "table", torch.int32, seqs, width), _whole(starts, "starts", torch.int32, seqs + 1)
-    _one_device(torch, cache.k_pages, table, starts)
-    k, v = (torch.empty((total, cache.heads, cache.head_dim), dtype=out_type, device=table.device) for _ in "kv")
+    tp = _whole(table, "table", torch.int32, (seqs, width), here)
+    sp = _whole(starts, "starts", torch.int32, (seqs + 1,), here)
+    if cache.device != here:
+        raise ValueError("the cache must be on the current GPU")
+    shape = (total, cache.heads, cache.head_dim)
+    k, v = table.new_empty(shape, dtype=out_type), table.new_empty(shape, dtype=out_type)
     lib().check("iq4xs_kv_gather", cache._address, tp, width, sp, seqs, k.data_ptr(), v.data_ptr(), total,
-                types[out_type], _stream(torch))
+                types[out_type], torch._C._cuda_getCurrentRawStream(here))
     return k, v
 
 
@@ -487,27 +498,30 @@ def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, 
     0).  scale defaults to head ** -0.5, out_type to q's.  Returns out, or (out, log-sum-exp of the scores [total,
     q_heads] in fp32) with lse; a row that sees nothing gives zeros and -inf."""
     torch = _torch()
+    here = _here(torch, q)
     types = _types(torch)
-    total, hq, d, q_stride = _rows(q, "q", None, cache.head_dim)
+    total, hq, d, q_stride = _rows(q, "q")
     out_type = q.dtype if out_type is None else out_type
     kind = types.get(q.dtype, TYPE_F32)
     if kind == TYPE_F32 or (cache.type != TYPE_Q8 and cache.type != kind) or out_type not in types:
         raise ValueError("q must have the cache's type (float16 or bfloat16 for codes), out_type be a float type")
-    if hq % cache.heads:
-        raise ValueError("q's heads must be a multiple of the cache's")
+    if d != cache.head_dim or hq % cache.heads or cache.device != here:
+        raise ValueError("q must have the cache's head size, a multiple of its heads, and both be on the current GPU")
     seqs = starts.numel() - 1
     width = table.size(1) if table.dim() == 2 else 0
-    tp, sp = _whole(table, "table", torch.int32, seqs, width), _whole(starts, "starts", torch.int32, seqs + 1)
-    lp = _whole(kv_len, "kv_len", torch.int32, seqs)
-    _one_device(torch, cache.k_pages, q, table, starts, kv_len)
-    out = torch.empty((total, hq, d), dtype=out_type, device=q.device)
-    sums = torch.empty((total, hq), dtype=torch.float32, device=q.device) if lse else None
+    tp = _whole(table, "table", torch.int32, (seqs, width), here)
+    sp = _whole(starts, "starts", torch.int32, (seqs + 1,), here)
+    lp = _whole(kv_len, "kv_len", torch.int32, (seqs,), here)
+    out = q.new_empty((total, hq, d), dtype=out_type)
+    sums = q.new_empty((total, hq), dtype=torch.float32) if lse else None
     args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), sums.data_ptr() if lse else 0, cache._address, tp, sp, lp,
                            q_stride, width, seqs, total, most_q, most_kv, window, hq, kind, types[out_type],
                            bool(causal), d ** -0.5 if scale is None else scale)
-    nbytes = lib().iq4xs_paged_attention_workspace_bytes(args)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    lib().check("iq4xs_paged_attention", args, ws.data_ptr() if nbytes else 0, nbytes, _stream(torch))
+    L = lib()
+    nbytes = L.iq4xs_paged_attention_workspace_bytes(args)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    L.check("iq4xs_paged_attention", args, ws.data_ptr() if nbytes else 0, nbytes,
+            torch._C._cuda_getCurrentRawStream(here))
     return (out, sums) if lse else out
 
 
