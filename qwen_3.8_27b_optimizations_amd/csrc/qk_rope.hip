@@ -101,18 +101,29 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_norm_rope_kernel(QkArgs a) {
         if (slot >= ((int64_t)a.c.pages << a.c.shift)) slot = -1;
     }
 
+    // a step's heads are loaded a step ahead
+    auto fetch = [&](int head, f4& u, f4& w) {
+        if (head >= heads) return;
+        const bool query = head < a.q_heads, key = head < a.q_heads + a.k_heads;
+        const int h = head - (query ? 0 : key ? a.q_heads : a.q_heads + a.k_heads);
+        const In* x = (query ? static_cast<const In*>(a.q) + token * a.q_stride
+                       : key ? static_cast<const In*>(a.k) + token * a.k_stride
+                             : static_cast<const In*>(a.v) + token * a.v_stride) + h * D;
+        u = load4(x + 4 * (key ? ca : 2 * l));
+        w = load4(x + 4 * (key ? cb : 2 * l + 1));
+    };
+    f4 u_next, w_next;
+    fetch(first + sub, u_next, w_next);
     for (int step = 0; step < a.steps; ++step) {
         const int head = first + step * HEADS + sub;
         if (head >= heads) return;  // a head's lanes leave together
+        f4 u = u_next, w = w_next;
+        if (step + 1 < a.steps) fetch(head + HEADS, u_next, w_next);
         const int kind = head < a.q_heads ? 0 : head < a.q_heads + a.k_heads ? 1 : 2;
         const int h = head - (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + a.k_heads);
-        const In* x = (kind == 0 ? static_cast<const In*>(a.q) + token * a.q_stride
-                       : kind == 1 ? static_cast<const In*>(a.k) + token * a.k_stride
-                                   : static_cast<const In*>(a.v) + token * a.v_stride) + h * D;
         if (kind == 2) {
             if (slot < 0) continue;
             const int64_t row = page_row(a.c, (int)(slot >> a.c.shift), h, (int)slot & ((1 << a.c.shift) - 1));
-            const f4 u = load4(x + 8 * l), w = load4(x + 8 * l + 4);
             if (a.cache_type == IQ4XS_TYPE_Q8) {
                 store_q8(static_cast<int8_t*>(a.c.v), a.c.vs, row, D, l, u, w);
             } else {
@@ -121,7 +132,6 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_norm_rope_kernel(QkArgs a) {
             }
             continue;
         }
-        f4 u = load4(x + 4 * ca), w = load4(x + 4 * cb);
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss += u[i] * u[i] + w[i] * w[i];
@@ -187,8 +197,10 @@ hipError_t launch_qk_norm_rope(const iq4xs_qk_norm_rope_args& g, const iq4xs_kv_
              g.out_type, 1, 1, g.eps, cache ? cache_pages(*cache) : CachePages{}, cache ? cache->type : 0};
     const int at_once = 512 / g.head_dim;
     const int steps = (g.q_heads + g.k_heads * (cache ? 2 : 1) + at_once - 1) / at_once;
-    // few tokens: a step of heads for each wave; many: a token for each wave
-    a.splits = (int)(g.tokens * steps <= 16 * (int64_t)device_cu_count() ? steps : 1);
+    // a token's heads go to as many waves as give every CU 16: fewer leave it idle (256 tokens of 64 + 8 heads of 128 22.6
+    // us in one wave each, 11.2 so), more compute more cosines (1024 tokens: 21.7 us with 64 waves, 15.2 so)
+    const int64_t splits = (16 * (int64_t)device_cu_count() + g.tokens - 1) / g.tokens;
+    a.splits = (int)(splits < steps ? splits : steps);
     a.steps = (steps + a.splits - 1) / a.splits;
     a.units = g.tokens * a.splits;
     const int64_t grid = (a.units + QK_WAVES - 1) / QK_WAVES;
