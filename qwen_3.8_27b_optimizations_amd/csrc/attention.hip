@@ -75,15 +75,17 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
     // Where the kernel of few rows ends: with 16-bit caches at two 16-row tiles, beyond which reading the keys again for
-    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows (72
-    // against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys; one tile at a time where
-    // two do not fit the registers or leave the second half empty.
+    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows for
+    // bf16 queries (72 against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys, and at 64
+    // for fp16 queries, whose keys neither rounds (64 rows of 64, 128, 256 channels: 66, 72, 114 against 99, 79, 125 us;
+    // 128 rows: 110, 118, 218 against 107, 87, 133).  One tile at a time where two do not fit the registers or leave most
+    // of the second empty.
     const int64_t rows = most_q * group;
-    const bool codes = g.cache->type == IQ4XS_TYPE_Q8;
-    if (rows <= 16 || (codes && rows <= 48 && (rows > 32 || g.cache->head_dim == 256)))
-        p.tiles = 1;
+    const bool codes = g.cache->type == IQ4XS_TYPE_Q8, wide = g.cache->head_dim == 256;
+    if (rows > (codes ? g.type == IQ4XS_TYPE_F16 ? 64 : 48 : 32))
+        p.tiles = 0;
     else
-        p.tiles = rows <= 32 ? 2 : 0;
+        p.tiles = rows <= 16 || (codes && (wide || (rows > 32 && rows <= 48))) ? 1 : 2;
     const int64_t tile = p.tiles ? 16 * p.tiles : 128, row_tiles = (most_q * group + tile - 1) / tile;
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;

@@ -13,8 +13,12 @@
 //   that lane: weights stay in registers;
 // - two workgroups share a CU, so that one's products run beside the other's exponentials;
 // - the running maximum of a row moves only when a key passes it by 2^8 (in powers of two).
-// An 8-bit cache becomes fp16 on its way into LDS (half a step of 2^-11 for each key and value); bf16 queries for it
-// become fp16 with a power of two taken out of each row.
+// An 8-bit cache with bf16 queries: keys and values become fp16 on their way into LDS (half a step of 2^-11 each, an
+// eighth of what bf16 outputs show), the queries fp16 with a power of two taken out of each row.  With fp16 queries
+// that would be 1.7 to 2.4 times the error of the outputs' own rounding, so there keys stay codes, exact in fp16, whose
+// scales multiply the parts of a score in fp32, and weights go as two fp16 numbers: half as many products again and as
+// many vector operations.  2048 tokens over 16384 keys of 128 channels: 1324 us with rounded keys, 1860 with exact ones
+// (of 64 channels 1513 and 2200, of 256 1712 and 2560); the kernel of few rows takes 2690 (2917, 4553).
 #include <type_traits>
 
 #include "attention_core.h"
@@ -68,15 +72,16 @@ struct Tile {
     }
 };
 
-// 16-byte piece of 8 codes as fp16, times the scale of their group.
+// 16-byte piece of 8 codes as fp16, times the scale of their group or (SCALED false) as they are.
+template <bool SCALED>
 __device__ inline u4 codes_to_f16(u2 w, _Float16 scale) {
     u4 x;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const uint32_t b = (p < 2 ? w.x : w.y) ^ 0x80808080u;
         const uint32_t z = __builtin_amdgcn_perm(b, b, p % 2 ? 0x0C030C02u : 0x0C010C00u) | 0x64006400u;
-        x[p] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(h2, z) - h2{(_Float16)1152, (_Float16)1152}) *
-                                                h2{scale, scale});
+        const h2 v = __builtin_bit_cast(h2, z) - h2{(_Float16)1152, (_Float16)1152};
+        x[p] = __builtin_bit_cast(uint32_t, SCALED ? v * h2{scale, scale} : v);
     }
     return x;
 }
@@ -85,9 +90,13 @@ template <int D, typename Q, typename KV>
 __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attention_kernel(AttentionArgs a) {
     using T = Tile<D>;
     constexpr bool CODES = sizeof(KV) == 1;
+    // fp16 queries of an 8-bit cache: scores of the exact codes, weights in two parts
+    constexpr bool EXACT = CODES && __is_same(Q, _Float16);
     using W = typename std::conditional<CODES, _Float16, KV>::type;
     using M = Matrix<W>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][T::BYTES];  // [buffer][keys, values]
+    // of exact keys, in the order in which a lane's scores want them: the 4 keys of every 8, half by half
+    __shared__ __attribute__((aligned(16))) _Float16 key_scales[EXACT ? 2 : 1][D / 32][T::KEYS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int n = lane % 32, half = lane / 32;
 
@@ -153,26 +162,21 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // keys, is read as page 0 and masked
     const int bring = 16 * wave, piece = lane % T::PIECES, in_load = lane / T::PIECES;
     constexpr int PARTS = T::KEYS / 16;
-    typedef int i4 __attribute__((ext_vector_type(4)));
-    i4 pages{-1, -1, -1, -1};  // of a tile, looked up a tile before they are wanted; -1: none, or not in the cache
+    // Pages of a tile, looked up a tile before they are wanted: of its 16 keys i in lane i.  A load without a condition,
+    // waited for where `locate` uses it; waiting at once would be waiting for the tiles on their way (2048 tokens over
+    // 16384 keys: 1116 us, and 1032 so).
+    int looked_up;
     auto look_up = [&](int base) {
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-            const int key = base + 16 * i;
-            pages[i] = key < k1 ? s.pages[key >> a.c.shift] : -1;
-        }
+        const int key = base + 16 * (lane % PARTS);
+        const int32_t* p = key < k1 ? s.pages + (key >> a.c.shift) : a.starts;
+        looked_up = *p;
     };
     // of the tile at `base`, which was looked up: which 16 keys are not there, and where this wave's rows begin
     auto locate = [&](int base, uint32_t& lacking) {
-        lacking = 0;
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i)
-            if (pages[i] < 0 || pages[i] >= a.c.pages) lacking |= 1u << i;
-        int page = pages[0];
-#pragma unroll
-        for (int i = 1; i < PARTS; ++i)
-            if (wave == i) page = pages[i];
-        const bool there = page >= 0 && page < a.c.pages;
+        const bool held = base + 16 * (lane % PARTS) < k1 && looked_up >= 0 && looked_up < a.c.pages;
+        lacking = ~(uint32_t)__ballot(held) & ((1u << PARTS) - 1);
+        const int page = __builtin_amdgcn_readlane(looked_up, wave);
+        const bool there = !(lacking >> wave & 1);
         return page_row(a.c, there ? page : 0, head, there ? (base + bring) & ((1 << a.c.shift) - 1) : 0);
     };
     // rows of one side (0 keys, 1 values) on their way to a buffer; of an 8-bit cache into registers, from which `put`
@@ -207,13 +211,43 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             }
         }
     };
-    auto put = [&](int side, int buffer) {
+    // An infinity times a weight's second part is NaN: exact products want none in LDS; `odd` says that there were such.
+    int odd = 0;
+    auto put = [&](int side, int buffer, int base = 0, uint32_t missing = 0) {
         if constexpr (CODES) {
             asm volatile("" : "+v"(load_at[side]));
+            bool large = false;  // scales past 65504 / 127, whose values may not be finite
+            if (EXACT && side == 1) {
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i)
-                *reinterpret_cast<u4*>(&lds[buffer][side][(bring + i * T::ROWS) * T::ROW] +
-                                       (load_at[side] ^ turn(side, i))) = codes_to_f16(code[IN_TURN ? 0 : side][i], code_scale[IN_TURN ? 0 : side][i]);
+                for (int i = 0; i < T::LOADS; ++i) {
+                    const _Float16 by = code_scale[IN_TURN ? 0 : 1][i];
+                    large = large || (__builtin_bit_cast(uint16_t, by) & 0x7FFFu) > 0x6007u;
+                }
+                large = __any(large);
+            }
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) {
+                const u2 c = code[IN_TURN ? 0 : side][i];
+                const _Float16 by = code_scale[IN_TURN ? 0 : side][i];
+                u4* to = reinterpret_cast<u4*>(&lds[buffer][side][(bring + i * T::ROWS) * T::ROW] +
+                                               (load_at[side] ^ turn(side, i)));
+                if (EXACT && side == 0) {
+                    const int rr = bring + i * T::ROWS + in_load;
+                    *to = codes_to_f16<false>(c, by);
+                    if (piece % 4 == 0)
+                        key_scales[buffer][piece / 4][rr / 32 * 32 + rr / 4 % 2 * 16 + rr % 32 / 8 * 4 + rr % 4] = by;
+                } else {
+                    u4 v = codes_to_f16<true>(c, by);
+                    if (__builtin_expect(large, 0)) {
+                        const int rr = bring + i * T::ROWS + in_load, key = base + rr;
+                        const u4 f = M::finite(v), x = v ^ f;
+                        odd |= key >= any_lo && key < any_hi && !(missing >> (rr / 16) & 1) &&
+                               (x.x | x.y | x.z | x.w) != 0;
+                        v = f;
+                    }
+                    *to = v;
+                }
+            }
         }
     };
 
@@ -225,7 +259,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             if (key >= any_lo && key < any_hi && !(missing >> (rr / 16) & 1)) {
                 const int64_t row = page_row(a.c, s.pages[key >> a.c.shift], head, key & ((1 << a.c.shift) - 1));
                 if constexpr (CODES)
-                    v = codes_to_f16(*reinterpret_cast<const u2*>(static_cast<const int8_t*>(a.c.v) + row * D + 8 * p),
+                    v = codes_to_f16<true>(*reinterpret_cast<const u2*>(static_cast<const int8_t*>(a.c.v) + row * D + 8 * p),
                                      a.c.vs[row * (D / 32) + p / 4]);
                 else
                     v = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.c.v) + row * D + 8 * p);
@@ -324,97 +358,178 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         }
     };
 
-    // Tile T in steps 2 T and 2 T + 1 of 32 keys.  A step computes the scores of the step after it and the weights of its
-    // own beside the product of the weights before it: keys are wanted a tile ahead of values.  The barrier of tile T
-    // comes before step 2 T + 1: keys of tile T and values of tile T - 1 are done with, those of T + 1 and T are there.
-    uint32_t lacking, next_lacking = (1u << PARTS) - 1;
-    look_up(k0);
-    int64_t row = locate(k0, lacking);
-    fetch(0, row, 0);
-    if (IN_TURN) put(0, 0);
-    fetch(1, row, 0);
-    if (!IN_TURN) put(0, 0);
-    put(1, 0);
-    look_up(k0 + T::KEYS);
-    wait_for_copies();
-    __syncthreads();
-    fx16 even, uneven;
-    u4 w_even[2] = {}, w_odd[2];
+    // A weight of zero times an infinity is NaN.  Where rows differ in what they see, values that no row sees and values
+    // that are not finite are cleared in LDS; the latter come again after the last tile.
+    auto clear = [&](int base, int buffer, uint32_t missing) {
+        uint32_t some = 0;
+        for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
+            const int key = base + i / T::PIECES;
+            u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
+            const bool seen = key >= any_lo && key < any_hi && !(missing >> (i / T::PIECES / 16) & 1);
+            const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
+            some |= seen ? x.x | x.y | x.z | x.w : 0u;
+            *p = f;
+        }
+        odd = __syncthreads_or(odd | (some != 0));
+    };
+
+    if constexpr (EXACT) {
+        // A tile's 32 keys in turn: their scores, weights and product with the values; the next tile's codes are on their
+        // way meanwhile.
+        uint32_t lacking;
+        look_up(k0);
+        int64_t row = locate(k0, lacking);
+        fetch(0, row, 0);
+        if (IN_TURN) put(0, 0);
+        fetch(1, row, 0);
+        if (!IN_TURN) put(0, 0);
+        put(1, 0, k0, lacking);
+        look_up(k0 + T::KEYS);
+        int buffer = 0;
+        for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+            asm volatile("" : "+v"(looked_up));
+            __syncthreads();
+            const bool edge = lacking != 0 || base < all_lo || base + T::KEYS > all_hi, more = base + T::KEYS < k1;
+            if (__builtin_expect(edge, 0)) clear(base, buffer, lacking);
+            const uint32_t was_lacking = lacking;
+            if (more) {
+                row = locate(base + T::KEYS, lacking);
+                fetch(0, row, buffer ^ 1);
+                if (!IN_TURN) fetch(1, row, buffer ^ 1);
+                look_up(base + 2 * T::KEYS);
+            }
+            asm volatile("" : "+v"(key_at), "+v"(value_at));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) even[i] = uneven[i] = 0.0f;
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t from = buffer * 2 * T::BYTES + s * 32 * T::ROW;
+                fx16 z;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-        even = M::mma32(key_piece(key_at, c, 0), q[c], even);
-        uneven = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], uneven);
-    }
-    bool edge = lacking != 0 || k0 < all_lo || k0 + T::KEYS > all_hi;
-    raise(even, k0, lacking, edge, w_even);
+                for (int i = 0; i < 16; ++i) z[i] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) weigh(even, i, w_even);
-    if (k0 + T::KEYS < k1) {
-        row = locate(k0 + T::KEYS, next_lacking);
-        fetch(0, row, 1);
-        put(0, 1);
-        look_up(k0 + 2 * T::KEYS);
-    }
-    if constexpr (D == 256) {  // with the sums, where the products read them and nothing else does
+                for (int g = 0; g < D / 32; ++g) {
+                    fx16 part;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) asm volatile("" : "+a"(q[c]));
-    }
-    bool odd = false;
-    int buffer = 0;
-    for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+                    for (int i = 0; i < 16; ++i) part[i] = 0.0f;
+                    part = M::mma32(key_piece(key_at + from, 2 * g, 0), q[2 * g], part);
+                    part = M::mma32(key_piece(key_at + from, 2 * g + 1, 0), q[2 * g + 1], part);
+                    const h8* sc = reinterpret_cast<const h8*>(&key_scales[buffer][g][32 * s + 16 * half]);
+                    const h8 s0 = sc[0], s1 = sc[1];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = __builtin_fmaf(part[i], (float)(i < 8 ? s0[i] : s1[i - 8]), z[i]);
+                }
+                u4 w[2] = {}, rest[2];
+                raise(z, base + 32 * s, was_lacking >> 2 * s, edge, w);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], factor, -m));
+                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i + 1], factor, -m));
+                    l += x0 + x1;
+                    const h2 high{(_Float16)x0, (_Float16)x1};
+                    w[i / 8][i % 8 / 2] = __builtin_bit_cast(uint32_t, high);
+                    rest[i / 8][i % 8 / 2] = M::pack(x0 - (float)high.x, x1 - (float)high.y);
+                }
+                if (IN_TURN && s == 0 && more) {
+                    put(0, buffer ^ 1);
+                    fetch(1, row, buffer ^ 1);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int t0 = 0; t0 < D / 32; t0 += 2) {
+                        const u4 v0 = value_piece(value_at + from, t0, 16 * k * T::ROW);
+                        const u4 v1 = value_piece(value_at + from, t0 + 1, 16 * k * T::ROW);
+                        o[t0] = M::mma32(v0, w[k], o[t0]);
+                        o[t0 + 1] = M::mma32(v1, w[k], o[t0 + 1]);
+                        o[t0] = M::mma32(v0, rest[k], o[t0]);
+                        o[t0 + 1] = M::mma32(v1, rest[k], o[t0 + 1]);
+                    }
+            }
+            if (more) {
+                if (!IN_TURN) put(0, buffer ^ 1);
+                put(1, buffer ^ 1, base + T::KEYS, lacking);
+            }
+        }
+    } else {
+        // Tile T in steps 2 T and 2 T + 1 of 32 keys.  A step computes the scores of the step after it and the weights of its
+        // own beside the product of the weights before it: keys are wanted a tile ahead of values.  The barrier of tile T
+        // comes before step 2 T + 1: keys of tile T and values of tile T - 1 are done with, those of T + 1 and T are there.
+        uint32_t lacking, next_lacking = (1u << PARTS) - 1;
+        look_up(k0);
+        int64_t row = locate(k0, lacking);
+        fetch(0, row, 0);
+        if (IN_TURN) put(0, 0);
+        fetch(1, row, 0);
+        if (!IN_TURN) put(0, 0);
+        put(1, 0);
+        look_up(k0 + T::KEYS);
         wait_for_copies();
         __syncthreads();
-        // A weight of zero times an infinity is NaN.  Where rows differ in what they see, values that no row sees and
-        // values that are not finite are cleared in LDS; the latter come again after the last tile.
-        if (__builtin_expect(edge, 0)) {
-            bool some = false;
-            for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
-                const int key = base + i / T::PIECES;
-                u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
-                const bool seen = key >= any_lo && key < any_hi && !(lacking >> (i / T::PIECES / 16) & 1);
-                const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
-                some = some || (seen && (x.x | x.y | x.z | x.w) != 0);
-                *p = f;
+        fx16 even, uneven;
+        u4 w_even[2] = {}, w_odd[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) even[i] = uneven[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+            even = M::mma32(key_piece(key_at, c, 0), q[c], even);
+            uneven = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], uneven);
+        }
+        bool edge = lacking != 0 || k0 < all_lo || k0 + T::KEYS > all_hi;
+        raise(even, k0, lacking, edge, w_even);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) weigh(even, i, w_even);
+        if (k0 + T::KEYS < k1) {
+            row = locate(k0 + T::KEYS, next_lacking);
+            fetch(0, row, 1);
+            put(0, 1);
+            look_up(k0 + 2 * T::KEYS);
+        }
+        if constexpr (D == 256) {  // with the sums, where the products read them and nothing else does
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) asm volatile("" : "+a"(q[c]));
+        }
+        int buffer = 0;
+        for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+            wait_for_copies();
+            asm volatile("" : "+v"(looked_up));  // there now, as far as the compiler's own waits go
+            __syncthreads();
+            if (__builtin_expect(edge, 0)) clear(base, buffer, lacking);
+            const uint32_t was_lacking = lacking;
+            lacking = next_lacking;
+            next_lacking = (1u << PARTS) - 1;
+            if (base + T::KEYS < k1) fetch(1, row, buffer ^ 1);
+            if (base + 2 * T::KEYS < k1) {
+                row = locate(base + 2 * T::KEYS, next_lacking);
+                if (!IN_TURN) fetch(0, row, buffer);
+                look_up(base + 3 * T::KEYS);
             }
-            odd = __syncthreads_or(some) || odd;
-        }
-        const uint32_t was_lacking = lacking;
-        lacking = next_lacking;
-        next_lacking = (1u << PARTS) - 1;
-        if (base + T::KEYS < k1) fetch(1, row, buffer ^ 1);
-        if (base + 2 * T::KEYS < k1) {
-            row = locate(base + 2 * T::KEYS, next_lacking);
-            if (!IN_TURN) fetch(0, row, buffer);
-            look_up(base + 3 * T::KEYS);
-        }
-        asm volatile("" : "+v"(key_at), "+v"(value_at));  // the places along a row are cheaper computed than kept
-        const uint32_t here = buffer * 2 * T::BYTES, there = 2 * T::BYTES - here;
-        u4 f[AHEAD];
-        begin(key_at + there, value_at + here, f);
-        raise(uneven, base + 32, was_lacking >> 2, edge, w_even);
-        step(key_at + there, value_at + here, f, even, uneven, w_even, w_odd);
-        if (IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
-        if (IN_TURN && base + 2 * T::KEYS < k1) fetch(0, row, buffer);
-        // past the last tile these are scores of whatever lies in LDS, all masked
-        edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
-        begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
-        raise(even, base + T::KEYS, lacking, edge, w_odd);
-        step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, uneven, even, w_odd, w_even);
+            asm volatile("" : "+v"(key_at), "+v"(value_at));  // the places along a row are cheaper computed than kept
+            const uint32_t here = buffer * 2 * T::BYTES, there = 2 * T::BYTES - here;
+            u4 f[AHEAD];
+            begin(key_at + there, value_at + here, f);
+            raise(uneven, base + 32, was_lacking >> 2, edge, w_even);
+            step(key_at + there, value_at + here, f, even, uneven, w_even, w_odd);
+            if (IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
+            if (IN_TURN && base + 2 * T::KEYS < k1) fetch(0, row, buffer);
+            // past the last tile these are scores of whatever lies in LDS, all masked
+            edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
+            begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
+            raise(even, base + T::KEYS, lacking, edge, w_odd);
+            step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, uneven, even, w_odd, w_even);
 
-        if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
-        if (base + 2 * T::KEYS < k1) put(0, buffer);
+            if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
+            if (base + 2 * T::KEYS < k1) put(0, buffer);
+        }
     }
 
-    if (__builtin_expect(odd, 0)) {
+    if (EXACT) odd = __syncthreads_or(odd);
+    if (__builtin_expect(odd != 0, 0)) {
         // the values that are not finite reach the rows that see them as infinities (a NaN as both)
         wait_for_copies();
         for (int base = k0; base < k1; base += T::KEYS) {
             look_up(base);
             uint32_t out;
             locate(base, out);
-            if (out == 0 && base >= all_lo && base + T::KEYS <= all_hi) continue;
+            if (!EXACT && out == 0 && base >= all_lo && base + T::KEYS <= all_hi) continue;
             __syncthreads();
             again(base, 0, out);
             __syncthreads();
