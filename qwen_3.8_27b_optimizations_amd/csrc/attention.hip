@@ -14,7 +14,7 @@ template <int D>
 __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(AttentionArgs a) {
     constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / LANES;
     __shared__ f4 so[GROUPS][LANES];
-    __shared__ float sm[GROUPS], sl[GROUPS];
+    __shared__ float sm[GROUPS], sl[GROUPS], sr[GROUPS];
     const int head = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
     const int seq = sequence_of(a.starts, a.seqs, row, threadIdx.x % 64);
     if (seq < 0 || seq >= a.seqs) return;
@@ -27,37 +27,40 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(AttentionArgs
     const int from = (lo - s.seen_from) / a.chunk, to = hi > lo ? (hi - 1 - s.seen_from) / a.chunk : from - 1;
     const int g = threadIdx.x / LANES, c = threadIdx.x % LANES;
     const int64_t out = (int64_t)row * a.q_heads + head, step = (int64_t)a.total * a.q_heads;
-    float m = -FLT_MAX, l = 0.0f;
+    float m = -FLT_MAX, l = 0.0f, rounded = 0.0f;
     f4 o{0, 0, 0, 0};
 #pragma unroll 4
     for (int i = from + g; i <= to; i += GROUPS) {
         const int64_t at = i * step + out;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+        const float4 ml = *reinterpret_cast<const float4*>(a.part_ml + 4 * at);
         const f4 v = *reinterpret_cast<const f4*>(a.part + at * D + 4 * c);
         const float up = fmaxf(m, ml.x), old = __builtin_amdgcn_exp2f(m - up), now = __builtin_amdgcn_exp2f(ml.x - up);
         m = up;
         l = l * old + ml.y * now;
+        rounded = rounded * old + ml.z * now;
         o = o * old + v * now;
     }
     so[g][c] = o;
     if (c == 0) {
         sm[g] = m;
         sl[g] = l;
+        sr[g] = rounded;
     }
     __syncthreads();
     if (g > 0) return;
     float best = sm[0];
 #pragma unroll
     for (int i = 1; i < GROUPS; ++i) best = fmaxf(best, sm[i]);
-    float sum = 0.0f;
+    float sum = 0.0f, weights = 0.0f;
     f4 v{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
         const float f = __builtin_amdgcn_exp2f(sm[i] - best);
         sum += sl[i] * f;
+        weights += sr[i] * f;
         v += so[i][c] * f;
     }
-    store4(a.out, out * D + 4 * c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / sum);
+    store4(a.out, out * D + 4 * c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / weights);
     if (a.lse && c == 0) a.lse[out] = sum == 0.0f ? -INFINITY : (best + __log2f(sum)) * 0.69314718056f;
 }
 
@@ -125,7 +128,7 @@ static size_t part_bytes(const iq4xs_paged_attention_args& g, int splits) {
 
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& g) {
     const int splits = plan_of(g).splits;
-    return part_bytes(g, splits) + part_bytes(g, splits) / g.cache->head_dim * 2;
+    return part_bytes(g, splits) + part_bytes(g, splits) / g.cache->head_dim * 4;
 }
 
 hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws, hipStream_t stream) {

@@ -18,7 +18,7 @@ struct AttentionArgs {
     float* lse;
     const int32_t *table, *starts, *kv_len;
     float* part;      // [splits][total][q_heads][D] unnormalised sums, with splits > 1
-    float* part_ml;   // [splits][total][q_heads][2] their maxima (in powers of two) and sums of weights
+    float* part_ml;   // [splits][total][q_heads][4] their maxima (in powers of two), sums of weights, and of rounded ones
     int64_t q_stride, width;
     int total, most_q, most_kv, window;  // window 0: none
     int seqs, q_heads, group, out_type, causal;
@@ -121,6 +121,12 @@ struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
     static __device__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
     }
+    // A pair of weights onto a sum, exact products and one fp32 sum (fp16 below its normal range too).  What the values'
+    // sum is divided by has to be the sum of the weights as they are rounded, or a row of one key is off by its
+    // weight's rounding: over short rows, 1.5 times the error.
+    static __device__ float add(uint32_t pair, float sum) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), h2{(_Float16)1, (_Float16)1}, sum, false);
+    }
     static __device__ uint32_t scaled(uint32_t x, float by) {
         const h2 v = __builtin_bit_cast(h2, x);
         return pack((float)v.x * by, (float)v.y * by);
@@ -137,6 +143,10 @@ struct Matrix<__bf16> : Pairs<0x7F80u, 0x3F803F80u> {
     static __device__ uint32_t pack(float x, float y) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    }
+    static __device__ float add(uint32_t pair, float sum) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), b2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
     }
     static __device__ uint32_t scaled(uint32_t x, float by) {
         return pack(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xFFFF0000u) * by);

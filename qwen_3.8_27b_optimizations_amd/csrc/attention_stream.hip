@@ -257,7 +257,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     // values of an 8-bit cache are rounded, so weights are not: they go as two fp16 numbers, high and rest
     constexpr bool EXACT = sizeof(KV) == 1;
     __shared__ float so[STREAM_WAVES][16][PART + 4];
-    __shared__ float sm[STREAM_WAVES][16], sl[STREAM_WAVES][16];
+    __shared__ float sm[STREAM_WAVES][16], sl[STREAM_WAVES][16], sr[STREAM_WAVES][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int n = lane % 16, j = lane / 16;
     unsigned x = blockIdx.x;
@@ -325,11 +325,11 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     }
 
     f4 o[NT][OWN];
-    float m[NT], l[NT];
+    float m[NT], l[NT], rounded[NT];  // of the weights as they are and, where they are rounded, so
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         m[i] = -FLT_MAX;
-        l[i] = 0.0f;
+        l[i] = rounded[i] = 0.0f;
 #pragma unroll
         for (int t = 0; t < OWN; ++t) o[i][t] = f4{0, 0, 0, 0};
     }
@@ -406,6 +406,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 const float up = fmaxf(max_of_quarters(top), m[i]), keep = __builtin_amdgcn_exp2f(m[i] - up);
                 m[i] = up;
                 l[i] *= keep;
+                rounded[i] *= keep;
 #pragma unroll
                 for (int t = 0; t < OWN; ++t) o[i][t] *= keep;
             }
@@ -419,6 +420,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
             for (int e = 0; e < 4; ++e) {
                 const uint32_t both = Matrix<W>::pack(p[2 * e], p[2 * e + 1]);
                 w[i][e] = both;
+                if constexpr (!EXACT) rounded[i] = Matrix<W>::add(both, rounded[i]);
                 if constexpr (EXACT) {
                     const h2 high = __builtin_bit_cast(h2, both);
                     w_rest[i][e] = Matrix<W>::pack(p[2 * e] - (float)high.x, p[2 * e + 1] - (float)high.y);
@@ -476,11 +478,12 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     // the waves' sums join in LDS, 16 rows and up to 128 channels at a time, in the waves' order
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-        const float lw = sum_of_quarters(l[i]);
+        const float lw = sum_of_quarters(l[i]), rw = EXACT ? lw : sum_of_quarters(rounded[i]);
         __syncthreads();
         if (j == 0) {
             sm[wave][n] = m[i];
             sl[wave][n] = lw;
+            sr[wave][n] = rw;
         }
         __syncthreads();
         float top = sm[0][n];
@@ -506,24 +509,26 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 float best = sm[0][y];
 #pragma unroll
                 for (int w = 1; w < STREAM_WAVES; ++w) best = fmaxf(best, sm[w][y]);
-                float sum = 0.0f;
+                float sum = 0.0f, weights = 0.0f;
                 f4 v{0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < STREAM_WAVES; ++w) {
-                    sum += sl[w][y] * __builtin_amdgcn_exp2f(sm[w][y] - best);
+                    const float f = __builtin_amdgcn_exp2f(sm[w][y] - best);
+                    sum += sl[w][y] * f;
+                    weights += sr[w][y] * f;
                     v += *reinterpret_cast<const f4*>(&so[w][y][c]);
                 }
                 const int tok = r / a.group, h = head * a.group + r % a.group;
                 const int64_t out = (int64_t)(s.first + tok) * a.q_heads + h;
                 const RowEnd end = row_end(a, s, least_key(a, s, total_fresh, tok), end_key(a, s, total_fresh, tok), split);
                 if (end == ROW_OUT) {
-                    store4(a.out, out * D + PART * part + c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / sum);
+                    store4(a.out, out * D + PART * part + c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / weights);
                     if (a.lse && part == 0 && c == 0)
                         a.lse[out] = sum == 0.0f ? -INFINITY : (best + __log2f(sum)) * 0.69314718056f;
                 } else if (end == ROW_PART) {
                     const int64_t at = (int64_t)split * a.total * a.q_heads + out;
                     *reinterpret_cast<f4*>(a.part + at * D + PART * part + c) = v;
-                    if (part == 0 && c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(best, sum);
+                    if (part == 0 && c == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * at) = make_float4(best, sum, weights, 0.0f);
                 }
             }
         }

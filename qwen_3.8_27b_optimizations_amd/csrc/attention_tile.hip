@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    float m = -FLT_MAX, l = 0.0f;
+    float m = -FLT_MAX, l = 0.0f, rounded = 0.0f;  // sums of the weights as they are and, where they are rounded, so
 
     const uint32_t at = lds_address(lds);
     // wave w brings a tile's rows 16 w to 16 w + 15, which lie in one page; a page that is not in the cache, or past the
@@ -303,6 +303,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             const float up = fmaxf(ceilf(max_of_halves(top)), m), keep = __builtin_amdgcn_exp2f(m - up);
             m = up;
             l *= keep;
+            rounded *= keep;
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) {
                 o[t] *= keep;
@@ -323,7 +324,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i + 1], factor, -m));
         l += x0 + x1;
         uint32_t pair = M::pack(x0, x1);
-        asm volatile("" : "+v"(pair), "+v"(l));  // here, not where they are used
+        rounded = M::add(pair, rounded);
+        asm volatile("" : "+v"(pair), "+v"(l), "+v"(rounded));  // here, not where they are used
         w[i / 8][i % 8 / 2] = pair;
     };
     // A step's products in turn, those of the scores (place c of the queries) between those of the values (16 keys k,
@@ -562,10 +564,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     }
     if (wave0 + n > last) return;
     l = sum_of_halves(l);
+    rounded = EXACT ? l : sum_of_halves(rounded);
     const int64_t out = (int64_t)(s.first + token) * a.q_heads + query_head;
     const RowEnd end = row_end(a, s, lo, hi, split);
     if (end == ROW_OUT) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / rounded;
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -582,7 +585,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<f4*>(a.part + part * D + 32 * t + 2 * i + 4 * half) =
                     f4{o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
-        if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
+        if (half == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * part) = make_float4(m, l, rounded, 0.0f);
     }
 }
 
