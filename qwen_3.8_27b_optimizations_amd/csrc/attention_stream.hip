@@ -91,6 +91,7 @@ struct Step {
     }
     __device__ void share_scales(int) {}
     __device__ void prepare_values(int) {}
+    __device__ bool some_odd() const { return false; }
     // Clears the values outside the slots of the mask and those that are not finite; whether there were such inside.
     __device__ bool keep_finite(u4 slots) {
         uint32_t odd = 0;
@@ -220,6 +221,16 @@ struct Step<D, int8_t> {
             x[p] = __builtin_bit_cast(uint32_t, code_pair(v[2 * p + 1][t / 4], v[2 * p][t / 4], t % 4) * pair[t / 8][p]);
         return x;
     }
+    // Whether a scale of the step, of a key or a value, is not finite.
+    __device__ bool some_odd() const {
+        bool odd = false;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const _Float16 x = scale[g];
+            odd = odd || (__builtin_bit_cast(uint16_t, x) & 0x7C00u) == 0x7C00u;
+        }
+        return __any(odd);
+    }
     // A code's value is not finite where its scale is not.
     __device__ bool keep_finite(u4 slots) {
         bool odd = false;
@@ -334,13 +345,19 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         for (int t = 0; t < OWN; ++t) o[i][t] = f4{0, 0, 0, 0};
     }
 
-    // where tile t of the step at `base` lies; a tile past the end or on no page of the cache reads page 0 and is masked
-    auto find = [&](int base, int64_t(&row)[2], bool(&there)[2]) {
+    // Where tile t of the step at `base` lies; a tile past the end or on no page of the cache reads page 0 and is masked.
+    // Its pages are looked up a step before they are wanted, tile t's in lane t: a load without a condition, issued ahead of
+    // the step's keys, so that waiting for it is not waiting for them.
+    auto look_up = [&](int base) {
+        const int key = base + 16 * (lane % 2);
+        const int32_t* p = key < k1 ? s.pages + (key >> a.c.shift) : a.starts;
+        return *p;
+    };
+    auto find = [&](int base, int pages, int64_t(&row)[2], bool(&there)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key = base + 16 * t;
-            int page = key < k1 ? s.pages[key >> a.c.shift] : -1;
-            there[t] = page >= 0 && page < a.c.pages;
+            const int key = base + 16 * t, page = __builtin_amdgcn_readlane(pages, t);
+            there[t] = key < k1 && page >= 0 && page < a.c.pages;
             row[t] = page_row(a.c, there[t] ? page : 0, head, there[t] ? key & ((1 << a.c.shift) - 1) : 0);
         }
     };
@@ -361,9 +378,11 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     }
     int64_t row[2];
     bool there[2];
-    int base = k0 + STEP_KEYS * wave;
+    int base = k0 + STEP_KEYS * wave, pages = 0;
     if (base < k1) {
-        find(base, row, there);
+        const int first = look_up(base);
+        pages = look_up(base + STEP_KEYS * STREAM_WAVES);
+        find(base, first, row, there);
         step.load_keys(a, row, n, j);
         __builtin_amdgcn_sched_barrier(0);  // keys first, as in the loop, or its waits count too few
         step.load_values(a, row, n, j);
@@ -379,14 +398,24 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         const int next = base + STEP_KEYS * STREAM_WAVES;
         int64_t next_row[2];
         bool next_there[2];
-        find(next, next_row, next_there);
+        find(next, pages, next_row, next_there);
+        pages = look_up(next + STEP_KEYS * STREAM_WAVES);
+        __builtin_amdgcn_sched_barrier(0);
         f4 z[NT][2];
         step.share_scales(lane);
         step.scores(queries, z, lane);
+        // an infinity times a weight's second part is NaN: with codes, what is not finite is always cleared
+        const bool finite = !step.some_odd();
         // past the last step every lane reads one place: loads without a condition let the waits count exactly
         const int next_n = next < k1 ? n : 0, next_j = next < k1 ? j : 0;
         step.load_keys(a, next_row, next_n, next_j);
-        const bool full = there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
+        // Scores of heads of 256 come out in accumulation registers; they leave them here.  Left to itself the compiler
+        // read them in the blocks below, the last 6 wait states after its product, which takes 8, and got it unfinished.
+        if constexpr (D == 256 && !EXACT) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(z[i][0]), "+v"(z[i][1]));
+        }
+        const bool full = finite && there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
         u4 w[NT], w_rest[EXACT ? NT : 1];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -450,8 +479,8 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     if (__builtin_expect(__any(odd), 0)) {
         // values that are not finite reach the rows that see them as infinities (a NaN as both)
         for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
-            find(base, row, there);
-            if (there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi) continue;
+            find(base, look_up(base), row, there);
+            if (!EXACT && there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi) continue;
             step.load_keys(a, row, n, j);
             step.load_values(a, row, n, j);
             step.share_scales(lane);
