@@ -308,7 +308,8 @@ int iq4xs_mul_mat_fused(const void* W, const float* X, float* Y, int64_t K, int6
                         int32_t* S, void* stream);
 
 /* ===================== the attention half of a layer =====================
- * What runs between the q/k/v projections and o: norm and position rotation of
+ * What runs between the q/k/v projections and o (examples/attention_block.py
+ * runs them together): norm and position rotation of
  * queries and keys, a paged key/value cache, and attention over it.  No
  * counterpart in the reference, which leaves these ops to stock ggml.  The
  * calls allocate nothing, never synchronise and may be captured.
@@ -412,10 +413,16 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * and sees key j < kv_len if j <= p (causal) and j > p - window (window > 0).  A
  * row that sees nothing gives zeros and -Inf.  Keys and values that a row does
  * not see (and all that lies past kv_len) do not reach it, whatever they hold.
- * Scores, statistics and sums are fp32; weights are rounded to the type of q, or
- * fp16 for a Q8 cache, for their product with the values.  Tokens on a page that is
- * not in the cache are as masked ones.  Where kv_len is above most_kv or the
- * table, the first keys count; rows past most_q are not written.  The same call gives the same bits. */
+ * Scores, statistics and sums are fp32.  For their product with the values,
+ * weights are rounded to the cache's 16-bit type; the sum they are divided by is
+ * that of the rounded ones.  A Q8 cache: values become fp16 (their magnitudes
+ * must be within its range).  With F16 queries keys are exact and weights two
+ * fp16 numbers, high and rest.  BF16 queries become fp16 with a power of two taken
+ * out of each row; up to 48 rows of a cache head (new tokens times q_heads / heads)
+ * the rest is as with F16, above, keys become fp16 too and weights are one.
+ * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
+ * above most_kv or the table, the first keys count.  Rows past most_q, and those
+ * of no sequence, are not written.  The same call gives the same bits. */
 int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
 /* ================================ debug exports ================================

@@ -14,8 +14,16 @@
 //   splits in a second launch.
 // The running maximum of a row moves only when a key passes it by 2^8 (in powers of two): weights up to 2^8 are as exact
 // in 16 bits as weights up to 1, and the sums need no rescaling in most steps.
-// An 8-bit cache's codes become fp16 (exact); a key's four or so scales multiply the parts of its score in fp32, the
-// values' scales multiply their codes in fp16 (half a step of 2^-11).  bf16 queries for it become fp16 with a power of
+// A step's loads are issued a step ahead, its pages looked up two ahead, and none has a condition, so that each wait is
+// for what it needs.  Registers decide how many workgroups a CU holds: 4 with heads of 64, 2 with 128 (3 of an 8-bit
+// cache), 1 with 256; staging through LDS, two steps of a wave at once and three waves a SIMD by spilling were slower.
+// Measured: 131072 keys of 8 heads of 128, one token: 96 us, 5.6 TB/s (fp16), 54 us, 5.3 TB/s (8 bits); 64 sequences of up
+// to 16384 tokens: 211 us, 5.0 TB/s.  4096 keys: 6 us, of them latency (a dependent chain of table, keys, scores and
+// values), and 4 of the joining launch.  With more rows vector work grows beside the read: 8 sequences of 40 rows over
+// 8-bit heads of 256 93 us, of which reading is 19.
+// An 8-bit cache's codes become fp16 (exact); a key's scales (one for 32 channels) multiply the parts of its score in
+// fp32, the values' scales multiply their codes in fp16 (half a step of 2^-11), and the weights go as two fp16 numbers, so
+// that only this rounding is left.  bf16 queries for it become fp16 with a power of
 // two taken out of each row, exact down to 2^-14 of the row's largest element.
 #include "attention_core.h"
 #include "attention_internal.h"
@@ -401,11 +409,11 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         find(next, pages, next_row, next_there);
         pages = look_up(next + STEP_KEYS * STREAM_WAVES);
         __builtin_amdgcn_sched_barrier(0);
+        // an infinity times a weight's second part is NaN: with codes, what is not finite is always cleared
+        const bool finite = !step.some_odd();
         f4 z[NT][2];
         step.share_scales(lane);
         step.scores(queries, z, lane);
-        // an infinity times a weight's second part is NaN: with codes, what is not finite is always cleared
-        const bool finite = !step.some_odd();
         // past the last step every lane reads one place: loads without a condition let the waits count exactly
         const int next_n = next < k1 ? n : 0, next_j = next < k1 ? j : 0;
         step.load_keys(a, next_row, next_n, next_j);

@@ -3,7 +3,8 @@
 //   y = x * rsqrt(mean(x^2) + eps) * gain;  pair i of the first rot channels, (a, b):
 //   (a cos t - b sin t, b cos t + a sin t),  t = pos * freq[i]
 //
-// One pass over the data, bound by HBM at many tokens and by latency at few.  A head is held by head_dim / 8 lanes of 8
+// One pass over the data, bound by HBM at many tokens (4096 tokens of 64 + 8 heads of 128 in fp32: 64 us, 4.7 TB/s; 2048
+// into an 8-bit cache 34 us, 4.3 TB/s) and by latency at few.  A head is held by head_dim / 8 lanes of 8
 // channels, as two chunks of 4 picked so that both channels of every pair lie in one lane (half layout: chunk l and
 // chunk l + rot/8; interleaved: neighbours), so the rotation needs no exchange, and cosine and sine are computed once
 // for a lane's four pairs and used for every head it takes.  The angle is reduced to turns in 64 bits (positions reach
