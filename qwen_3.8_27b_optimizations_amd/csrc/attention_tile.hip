@@ -15,7 +15,7 @@
 // - the running maximum of a row moves only when a key passes it by 2^8 (in powers of two);
 // - the scores of the next 32 keys, the weights of these and the value products of those before are one stream of
 //   instructions, in the order written.
-// Measured: 2048 tokens over 16384 keys of 128 channels, 64 query heads on 8: 1040 us, 990 TFLOP/s of fp16 (1440 is what
+// Measured: 2048 tokens over 16384 keys of 128 channels, 64 query heads on 8: 1050 us, 980 TFLOP/s of fp16 (1440 is what
 // a large library product reaches), 1000 us in bf16; of 64 channels 1250 us, of 256 1130.  Matrix units are busy about
 // half of the time and vector units as long, with little overlap; LDS has no conflicts.
 // An 8-bit cache with bf16 queries: keys and values become fp16 on their way into LDS (half a step of 2^-11 each, an
