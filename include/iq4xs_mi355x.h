@@ -416,10 +416,10 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * Scores, statistics and sums are fp32.  For their product with the values,
  * weights are rounded to the cache's 16-bit type; the sum they are divided by is
  * that of the rounded ones.  A Q8 cache: values become fp16 (their magnitudes
- * must be within its range).  With F16 queries keys are exact and weights two
- * fp16 numbers, high and rest.  BF16 queries become fp16 with a power of two taken
- * out of each row; up to 48 rows of a cache head (new tokens times q_heads / heads)
- * the rest is as with F16, above, keys become fp16 too and weights are one.
+ * must be within its range), BF16 queries too, with a power of two taken out of
+ * each row; keys are exact and weights two fp16 numbers, high and rest.  Only where
+ * nothing but BF16 outputs is asked for, and more than 48 rows of a cache head (new
+ * tokens times q_heads / heads), keys become fp16 and weights are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
  * above most_kv or the table, the first keys count.  Rows past most_q, and those
  * of no sequence, are not written.  The same call gives the same bits. */

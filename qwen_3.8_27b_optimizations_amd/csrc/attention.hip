@@ -64,6 +64,71 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(AttentionArgs
     if (a.lse && c == 0) a.lse[out] = sum == 0.0f ? -INFINITY : (best + __log2f(sum)) * 0.69314718056f;
 }
 
+// The same with a wave for JOIN_EACH consecutive pairs of row and head: head_dim / 64 channels in a lane, the splits one
+// after another.
+constexpr int JOIN_EACH = 4;
+
+template <int D>
+__global__ __launch_bounds__(JOIN_THREADS) void join_splits_of_many_kernel(AttentionArgs a) {
+    typedef float Part __attribute__((ext_vector_type(D / 64)));
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t pairs = (int64_t)a.total * a.q_heads, step = pairs;
+    int64_t out = ((int64_t)blockIdx.x * (JOIN_THREADS / 64) + wave) * JOIN_EACH;
+    int before = -1, from = 0, to = -1;
+    bool skip = true;
+    for (int e = 0; e < JOIN_EACH && out < pairs; ++e, ++out) {
+        const int row = (int)(out / a.q_heads);
+        if (row != before) {
+            before = row;
+            const int seq = sequence_of(a.starts, a.seqs, row, lane);
+            skip = seq < 0 || seq >= a.seqs;
+            if (!skip) {
+                int total_fresh;
+                const Sequence s = sequence(a, seq, total_fresh);
+                const int token = row - s.first;
+                skip = token >= s.fresh;
+                if (!skip) {
+                    const int lo = least_key(a, s, total_fresh, token), hi = end_key(a, s, total_fresh, token);
+                    skip = one_split(a, s, lo, hi);
+                    from = (lo - s.seen_from) / a.chunk;
+                    to = hi > lo ? (hi - 1 - s.seen_from) / a.chunk : from - 1;
+                }
+            }
+        }
+        if (skip) continue;
+        float m = -FLT_MAX, l = 0.0f, rounded = 0.0f;
+        Part o = (Part)(0.0f);
+#pragma unroll 4
+        for (int i = from; i <= to; ++i) {
+            const int64_t at = i * step + out;
+            const float4 ml = *reinterpret_cast<const float4*>(a.part_ml + 4 * at);
+            const Part v = *reinterpret_cast<const Part*>(a.part + at * D + D / 64 * lane);
+            const float up = fmaxf(m, ml.x), old = __builtin_amdgcn_exp2f(m - up), now = __builtin_amdgcn_exp2f(ml.x - up);
+            m = up;
+            l = l * old + ml.y * now;
+            rounded = rounded * old + ml.z * now;
+            o = o * old + v * now;
+        }
+        const Part y = l == 0.0f ? (Part)(0.0f) : o / rounded;
+        const int64_t at = out * D + D / 64 * lane;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            float z;
+            if constexpr (D == 64)
+                z = y[0];
+            else
+                z = y[c];
+            if (a.out_type == IQ4XS_TYPE_F32)
+                static_cast<float*>(a.out)[at + c] = z;
+            else if (a.out_type == IQ4XS_TYPE_F16)
+                static_cast<_Float16*>(a.out)[at + c] = (_Float16)z;
+            else
+                static_cast<__bf16*>(a.out)[at + c] = (__bf16)z;
+        }
+        if (a.lse && lane == 0) a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718056f;
+    }
+}
+
 // What a call launches.
 struct AttentionPlan {
     int tiles;      // 16-row tiles of a workgroup that streams the cache, or 0: the kernel of many rows
@@ -72,20 +137,23 @@ struct AttentionPlan {
     int64_t grid;
 };
 
+// Whether the outputs show a rounding of an 8-bit cache's keys to fp16: all but bf16 ones do.
+static bool exact_keys(const iq4xs_paged_attention_args& g) { return g.out_type != IQ4XS_TYPE_BF16 || g.lse; }
+
 static int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
     // Where the kernel of few rows ends: with 16-bit caches at two 16-row tiles, beyond which reading the keys again for
-    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows for
-    // bf16 queries (72 against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys, and at 64
-    // for fp16 queries, whose keys neither rounds (64 rows of 64, 128, 256 channels: 66, 72, 114 against 99, 79, 125 us;
+    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows
+    // (72 against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys, and at 64 where
+    // neither may (64 rows of 64, 128, 256 channels: 66, 72, 114 against 99, 79, 125 us;
     // 128 rows: 110, 118, 218 against 107, 87, 133).  One tile at a time where two do not fit the registers or leave most
     // of the second empty.
     const int64_t rows = most_q * group;
     const bool codes = g.cache->type == IQ4XS_TYPE_Q8, wide = g.cache->head_dim == 256;
-    if (rows > (codes ? g.type == IQ4XS_TYPE_F16 ? 64 : 48 : 32))
+    if (rows > (codes ? exact_keys(g) ? 64 : 48 : 32))
         p.tiles = 0;
     else
         p.tiles = rows <= 16 || (codes && (wide || (rows > 32 && rows <= 48))) ? 1 : 2;
@@ -111,8 +179,12 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
             splits = at_most(round * (rounds > 1 ? rounds : 1), (span + 127) / 128);
         }
     } else {
-        // two workgroups on every CU, none with less than 512 keys
-        splits = at_most((2 * cus + pairs - 1) / pairs, (span + 511) / 512);
+        // the workgroups that the CUs hold at once, none with less than 512 keys: one with heads of 256 (1024-token
+        // prompt 94 us with two, 50 with one), two with 128, and of 64, where they hold three, two for one sequence and
+        // four for several, whose lengths differ (16 tokens over 32768 keys 43 us with two, 50 with four; 8 x 8 tokens 65
+        // and 54)
+        const int64_t held = wide ? 1 : g.cache->head_dim == 64 && g.seqs > 1 ? 4 : 2;
+        splits = at_most((held * cus + pairs - 1) / pairs, (span + 511) / 512);
     }
     const int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
     p.splits = (int)((span + chunk - 1) / chunk);
@@ -147,10 +219,21 @@ hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws,
     if (p.tiles)
         launch_stream_attention(a, D, p.tiles, g.type, g.cache->type, p.grid, stream);
     else
-        launch_tile_attention(a, D, g.type, g.cache->type, p.grid, stream);
+        launch_tile_attention(a, D, g.type, g.cache->type, exact_keys(g), p.grid, stream);
     if (p.splits > 1) {
-        const dim3 blocks((unsigned)join), threads(JOIN_THREADS);
-        if (D == 64)
+        const dim3 threads(JOIN_THREADS);
+        // a workgroup for each costs 1.3 ns; a wave for four is slower while there are few, whose splits then wait for
+        // each other (4 x 64 tokens, 16384 pairs: 84 us of a call in all, 78 so; 8 x 8 tokens, 4096 pairs: 47 and 50)
+        const bool many = join >= 16384;
+        const int64_t each = JOIN_THREADS / 64 * JOIN_EACH;
+        const dim3 blocks((unsigned)(many ? (join + each - 1) / each : join));
+        if (many && D == 64)
+            hipLaunchKernelGGL((join_splits_of_many_kernel<64>), blocks, threads, 0, stream, a);
+        else if (many && D == 128)
+            hipLaunchKernelGGL((join_splits_of_many_kernel<128>), blocks, threads, 0, stream, a);
+        else if (many)
+            hipLaunchKernelGGL((join_splits_of_many_kernel<256>), blocks, threads, 0, stream, a);
+        else if (D == 64)
             hipLaunchKernelGGL((join_splits_kernel<64>), blocks, threads, 0, stream, a);
         else if (D == 128)
             hipLaunchKernelGGL((join_splits_kernel<128>), blocks, threads, 0, stream, a);

@@ -19,7 +19,7 @@ struct AttentionArgs;
 void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
                              hipStream_t stream);
 // Rows of many, 128 for each workgroup.
-void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, int64_t grid,
+void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
                            hipStream_t stream);
 
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& args);

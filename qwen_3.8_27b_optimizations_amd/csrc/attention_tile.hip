@@ -18,11 +18,11 @@
 // Measured: 2048 tokens over 16384 keys of 128 channels, 64 query heads on 8: 1050 us, 980 TFLOP/s of fp16 (1440 is what
 // a large library product reaches), 1000 us in bf16; of 64 channels 1250 us, of 256 1130.  Matrix units are busy about
 // half of the time and vector units as long, with little overlap; LDS has no conflicts.
-// An 8-bit cache with bf16 queries: keys and values become fp16 on their way into LDS (half a step of 2^-11 each, an
-// eighth of what bf16 outputs show), the queries fp16 with a power of two taken out of each row.  With fp16 queries
-// that would be 1.7 to 2.4 times the error of the outputs' own rounding, so there keys stay codes, exact in fp16, whose
-// scales multiply the parts of a score in fp32, and weights go as two fp16 numbers: half as many products again and as
-// many vector operations.  2048 tokens over 16384 keys of 128 channels: 1324 us with rounded keys, 1860 with exact ones
+// An 8-bit cache whose outputs are bf16 alone: keys and values become fp16 on their way into LDS (half a step of 2^-11
+// each, an eighth of what such outputs show).  In fp16 outputs that would be 1.7 to 2.4 times the error of their own
+// rounding, and log-sum-exps would be off by 1e-5, so for these (EXACT) keys stay codes, exact in fp16, whose scales
+// multiply the parts of a score in fp32, and weights go as two fp16 numbers: half as many products again and as many
+// vector operations.  bf16 queries become fp16 with a power of two taken out of each row.  2048 tokens over 16384 keys of 128 channels: 1324 us with rounded keys, 1860 with exact ones
 // (of 64 channels 1513 and 2200, of 256 1712 and 2560); the kernel of few rows takes 2690 (2917, 4553).
 #include <type_traits>
 
@@ -91,12 +91,10 @@ __device__ inline u4 codes_to_f16(u2 w, _Float16 scale) {
     return x;
 }
 
-template <int D, typename Q, typename KV>
+template <int D, typename Q, typename KV, bool EXACT>
 __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attention_kernel(AttentionArgs a) {
     using T = Tile<D>;
     constexpr bool CODES = sizeof(KV) == 1;
-    // fp16 queries of an 8-bit cache: scores of the exact codes, weights in two parts
-    constexpr bool EXACT = CODES && __is_same(Q, _Float16);
     using W = typename std::conditional<CODES, _Float16, KV>::type;
     using M = Matrix<W>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][T::BYTES];  // [buffer][keys, values]
@@ -595,27 +593,31 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 }
 
 template <int D>
-void launch_types(const AttentionArgs& a, int type, int cache_type, dim3 grid, hipStream_t stream) {
+void launch_types(const AttentionArgs& a, int type, int cache_type, bool exact, dim3 grid, hipStream_t stream) {
     const dim3 block(64 * TILE_WAVES);
     if (cache_type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, _Float16>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, _Float16, false>), grid, block, 0, stream, a);
     else if (cache_type == IQ4XS_TYPE_BF16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, __bf16>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, __bf16, false>), grid, block, 0, stream, a);
+    else if (type == IQ4XS_TYPE_F16 && exact)
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, true>), grid, block, 0, stream, a);
     else if (type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, false>), grid, block, 0, stream, a);
+    else if (exact)
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, true>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, false>), grid, block, 0, stream, a);
 }
 
-void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, int64_t grid,
+void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
                            hipStream_t stream) {
     const dim3 blocks((unsigned)grid);
     if (head_dim == 64)
-        launch_types<64>(a, type, cache_type, blocks, stream);
+        launch_types<64>(a, type, cache_type, exact, blocks, stream);
     else if (head_dim == 128)
-        launch_types<128>(a, type, cache_type, blocks, stream);
+        launch_types<128>(a, type, cache_type, exact, blocks, stream);
     else
-        launch_types<256>(a, type, cache_type, blocks, stream);
+        launch_types<256>(a, type, cache_type, exact, blocks, stream);
 }
 
 }  // namespace iq4xs

@@ -54,3 +54,25 @@ def test_infinite_scales_among_keys_that_all_see(pkg, dev, new, d, value):  # no
     keep = torch.ones_like(got, dtype=torch.bool)
     keep[:, 4:, 32:64] = False
     assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("d,heads", [(64, 16), (128, 8), (256, 4)])
+@pytest.mark.parametrize("kv,new", [([1500, 40, 2100], [130, 40, 120]), ([1400], [300])])
+def test_many_rows_in_several_splits(pkg, dev, d, heads, kv, new):  # noqa: F811
+    """Enough rows that a wave joins several: equal to the sequences on their own, where fewer are joined another way."""
+    print(f"[many rows] {d} {kv} {new}", flush=True)
+    p = Problem(kv, new, heads, 8, d, 16, "f16", seed=d)
+    q, c, table, starts, kv_len = p.on(pkg, dev)
+    for window in (0, 700):
+        out, lse = pkg.paged_attention(q, c, table, starts, kv_len, max(new), max(kv), window=window, lse=True)
+        for s in range(len(kv)):
+            for lo in range(0, new[s], 16):  # rows of 16 tokens at a time, as drafts at the end of what they see
+                n = min(16, new[s] - lo)
+                first, end = int(starts[s]) + lo, kv[s] - new[s] + lo + n
+                one, l1 = pkg.paged_attention(q[first:first + n], c, table[s:s + 1],
+                                              torch.tensor([0, n], dtype=torch.int32, device=dev),
+                                              torch.tensor([end], dtype=torch.int32, device=dev), n, end, window=window,
+                                              lse=True)
+                # both are within two half steps of fp16 (weights, output) of the same sum, of values below 6
+                assert bool(((one - out[first:first + n]).abs() <= 2 * 2 * 2.0 ** -11 * 6).all()), (s, lo)
+                assert bool(((l1 - lse[first:first + n]).abs() <= 2.0 ** -14).all()), (s, lo)
