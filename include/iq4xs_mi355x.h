@@ -418,7 +418,7 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * that of the rounded ones.  A Q8 cache: values become fp16 (their magnitudes
  * must be within its range), BF16 queries too, with a power of two taken out of
  * each row; keys are exact and weights two fp16 numbers, high and rest.  Only where
- * nothing but BF16 outputs is asked for, and more than 48 rows of a cache head (new
+ * nothing but BF16 outputs is asked for, of more than 32 rows of a cache head (new
  * tokens times q_heads / heads), keys become fp16 and weights are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
  * above most_kv or the table, the first keys count.  Rows past most_q, and those

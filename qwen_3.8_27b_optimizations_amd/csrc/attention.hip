@@ -145,15 +145,15 @@ static int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
-    // Where the kernel of few rows ends: with 16-bit caches at two 16-row tiles, beyond which reading the keys again for
-    // the third costs more than the other kernel's idle rows (40 rows: 75 against 54 us).  With 8-bit ones at 48 rows
-    // (72 against 64 us of heads of 128, 103 against 92 of 256), since it does not round the keys, and at 64 where
-    // neither may (64 rows of 64, 128, 256 channels: 66, 72, 114 against 99, 79, 125 us;
-    // 128 rows: 110, 118, 218 against 107, 87, 133).  One tile at a time where two do not fit the registers or leave most
-    // of the second empty.
+    // Where the kernel of few rows ends: at two 16-row tiles, beyond which reading the keys again for the third costs more
+    // than the other kernel's idle rows (40 rows: 75 against 54 us with 16-bit caches, 48 rows of an 8-bit one for bf16
+    // outputs 94 against 72 of 256 channels, 64 against 57 of 128).  With exact 8-bit keys, which cost the other kernel
+    // more, at 64 rows, with heads of 256 at 48 (64 rows of 64, 128, 256 channels: 66, 70, 121 against 99, 79, 115 us; 128
+    // rows: 110, 118, 218 against 93, 87, 116).  One tile at a time where two do not fit the registers or leave most of the
+    // second empty.
     const int64_t rows = most_q * group;
     const bool codes = g.cache->type == IQ4XS_TYPE_Q8, wide = g.cache->head_dim == 256;
-    if (rows > (codes ? exact_keys(g) ? 64 : 48 : 32))
+    if (rows > (codes && exact_keys(g) ? wide ? 48 : 64 : 32))
         p.tiles = 0;
     else
         p.tiles = rows <= 16 || (codes && (wide || (rows > 32 && rows <= 48))) ? 1 : 2;
