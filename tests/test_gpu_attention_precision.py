@@ -76,3 +76,17 @@ def test_many_rows_in_several_splits(pkg, dev, d, heads, kv, new):  # noqa: F811
                 # both are within two half steps of fp16 (weights, output) of the same sum, of values below 6
                 assert bool(((one - out[first:first + n]).abs() <= 2 * 2 * 2.0 ** -11 * 6).all()), (s, lo)
                 assert bool(((l1 - lse[first:first + n]).abs() <= 2.0 ** -14).all()), (s, lo)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("new", [1, 3, 30])
+def test_calls_repeat_bit_for_bit(pkg, dev, new, cache, d):  # noqa: F811
+    """Lengths of one step, of several and of several splits, the call again and again: nothing is read unfinished."""
+    p = Problem([1, 33, 64, 65, 130, 700, 1500, 9000], [1] * 5 + [new] * 3, 1, 8, d, 16, cache, seed=d)
+    q, c, table, starts, kv_len = p.on(pkg, dev)
+    first = None
+    for _ in range(12):
+        got = pkg.paged_attention(q, c, table, starts, kv_len, max(p.new), max(p.kv), lse=True)
+        first = first or got
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
