@@ -142,6 +142,9 @@ static bool exact_keys(const iq4xs_paged_attention_args& g) { return g.out_type 
 
 static int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 
+// Positions are below 2^31: a window of that many and more hides nothing, and sums with it could pass 64 bits.
+static int64_t window_of(const iq4xs_paged_attention_args& g) { return g.window < 0x7FFFFFFF ? g.window : 0; }
+
 static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
@@ -160,7 +163,8 @@ static AttentionPlan plan_of(const iq4xs_paged_attention_args& g) {
     const int64_t tile = p.tiles ? 16 * p.tiles : 128, row_tiles = (most_q * group + tile - 1) / tile;
     // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
     int64_t span = g.most_kv;
-    if (g.window > 0 && g.window + most_q + 32 < span) span = g.window + most_q + 32;
+    const int64_t window = window_of(g);
+    if (window > 0 && window + most_q + 32 < span) span = window + most_q + 32;
     const int64_t pairs = g.seqs * g.cache->heads * row_tiles, cus = device_cu_count();
     int64_t splits;
     if (p.tiles) {
@@ -208,10 +212,9 @@ hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws,
     const AttentionPlan p = plan_of(g);
     const int D = g.cache->head_dim;
     float* part = static_cast<float*>(ws);
-    const int64_t window = g.window < 0x7FFFFFFF ? g.window : 0;  // past every key: none
     const AttentionArgs a{cache_pages(*g.cache), g.q, g.out, g.lse, g.table, g.starts, g.kv_len, part,
                           p.splits > 1 ? part + part_bytes(g, p.splits) / sizeof(float) : nullptr, g.q_stride,
-                          g.table_width, (int)g.total, (int)g.most_q, (int)g.most_kv, (int)window, (int)g.seqs,
+                          g.table_width, (int)g.total, (int)g.most_q, (int)g.most_kv, (int)window_of(g), (int)g.seqs,
                           g.q_heads, g.q_heads / g.cache->heads, g.out_type, g.causal, p.splits, p.chunk, p.row_tiles,
                           g.scale * 1.44269504089f};
     const int64_t join = g.total * g.q_heads;
