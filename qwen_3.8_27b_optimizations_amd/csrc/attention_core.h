@@ -1,11 +1,11 @@
-// attention_core.h -- what the two attention kernels share: which keys a row sees, how the keys are split over
-// workgroups, matrix products, and the outputs.
+// attention_core.h -- what the two attention kernels share: their arguments, matrix products, and the outputs.
 #pragma once
 
 #include <float.h>
 #include <math.h>
 
 #include "attention_device.h"
+#include "attention_plan.h"
 
 namespace iq4xs {
 
@@ -26,53 +26,6 @@ struct AttentionArgs {
     int row_tiles;
     float scale;  // times log2(e)
 };
-
-// One sequence of the call, cut to what the arguments allow.
-struct Sequence {
-    int first, fresh;  // its rows in q: first row, count
-    int keys;          // cached tokens
-    int seen_from;     // first key that the first row sees, a multiple of 32: where split 0 begins
-    const int32_t* pages;
-};
-
-__device__ inline int least_key(const AttentionArgs& a, const Sequence& s, int total_fresh, int token) {
-    const int64_t lo = (int64_t)s.keys - total_fresh + token + 1 - a.window;
-    return a.window > 0 && lo > 0 ? (lo < s.keys ? (int)lo : s.keys) : 0;
-}
-__device__ inline int end_key(const AttentionArgs& a, const Sequence& s, int total_fresh, int token) {
-    const int64_t hi = (int64_t)s.keys - total_fresh + token + 1;
-    return !a.causal || hi > s.keys ? s.keys : hi > 0 ? (int)hi : 0;
-}
-
-// total_fresh: the new tokens as the positions count them; s.fresh of them are rows to compute.
-__device__ inline Sequence sequence(const AttentionArgs& a, int seq, int& total_fresh) {
-    Sequence s;
-    s.first = a.starts[seq];
-    total_fresh = a.starts[seq + 1] - s.first;
-    s.fresh = total_fresh < a.most_q ? total_fresh : a.most_q;
-    if (s.first < 0) s.fresh = 0;
-    if (s.fresh > a.total - s.first) s.fresh = a.total - s.first;
-    int64_t keys = a.kv_len[seq];
-    keys = keys < a.most_kv ? keys : a.most_kv;
-    keys = keys < (a.width << a.c.shift) ? keys : a.width << a.c.shift;
-    s.keys = keys > 0 ? (int)keys : 0;
-    s.seen_from = least_key(a, s, total_fresh, 0) & ~31;
-    s.pages = a.table + (int64_t)seq * a.width;
-    return s;
-}
-
-// Where the sums of a row that sees the keys [lo, hi) go: with one split, to the outputs, from the workgroup of that
-// split; with several, to its place in the workspace, from every workgroup that has them, and the joining kernel writes
-// the outputs, as it does for a row that sees nothing.
-enum RowEnd { ROW_OUT, ROW_PART, ROW_NONE };
-
-__device__ inline bool one_split(const AttentionArgs& a, const Sequence& s, int lo, int hi) {
-    return a.splits == 1 || (hi > lo && (lo - s.seen_from) / a.chunk == (hi - 1 - s.seen_from) / a.chunk);
-}
-__device__ inline RowEnd row_end(const AttentionArgs& a, const Sequence& s, int lo, int hi, int split) {
-    if (!one_split(a, s, lo, hi)) return ROW_PART;
-    return a.splits == 1 || (lo - s.seen_from) / a.chunk == split ? ROW_OUT : ROW_NONE;
-}
 
 // Pairs of 16-bit numbers as masks: 0xFFFF where a number is an infinity or NaN and `which` says so of its sign (0 or 1)
 // and of being NaN.

@@ -120,12 +120,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // keys that some row sees, and those that all see
     const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
     const int all_lo = least_key(a, s, total_fresh, token1), all_hi = end_key(a, s, total_fresh, token0);
-    int k0 = s.seen_from + split * a.chunk, k1 = any_hi;
-    if (a.splits > 1) {
-        k1 = any_hi < k0 + a.chunk ? any_hi : k0 + a.chunk;
-        if (k1 <= k0 || k0 + a.chunk <= any_lo) return;
-    }
-    if (k0 < (any_lo & ~31)) k0 = any_lo & ~31;
+    int k0, k1;
+    if (!split_keys(a, s, any_lo, any_hi, split, k0, k1)) return;
 
     // this lane's row (lanes without one repeat the last)
     const int wave0 = row0 + 32 * wave;

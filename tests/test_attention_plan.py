@@ -1,0 +1,56 @@
+"""How attention splits keys over workgroups (csrc/attention_plan.h), compiled for the host and asked about many calls:
+every key that a row sees reaches it exactly once, and the sums that are joined are those that were written."""
+import os
+import random
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CXX = os.environ.get("CXX", "g++")
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    if shutil.which(CXX) is None:
+        pytest.skip("needs a host C++ compiler")
+    exe = str(tmp_path_factory.mktemp("plan") / "attention_plan")
+    subprocess.run([CXX, "-std=c++17", "-O2", "-I" + os.path.join(ROOT, "qwen_3.8_27b_optimizations_amd", "csrc"),
+                    "-I" + os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "arith", "attention_plan.cpp"),
+                    "-o", exe], check=True)
+
+    def wrong(calls):
+        r = subprocess.run([exe], input="\n".join(calls) + "\n", capture_output=True, text=True, check=True)
+        out = [int(x) for x in r.stdout.split()]
+        assert len(out) == len(calls)
+        return [(c, n) for c, n in zip(calls, out) if n]
+
+    return wrong
+
+
+def call(new, kv, most_q=None, most_kv=None, window=0, causal=True, heads=1, group=1, d=128, kind=1, out=1, lse=0,
+         total=None, width=1 << 20):
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    total = sum(new) if total is None else total
+    return " ".join(str(int(x)) for x in (total, max(new) if most_q is None else most_q,
+                                          max(kv) if most_kv is None else most_kv, window, causal, heads, group, d, kind,
+                                          out, lse, width, 4, len(kv), *starts, *kv))
+
+
+def drawn(rng, over):
+    """A call; `over`: with sequences of more new tokens, and more cached ones, than it was told."""
+    seqs = rng.choice([1, 1, 2, 5])
+    spread = lambda n: int(n ** rng.random())  # noqa: E731
+    new = [spread(900) for _ in range(seqs)]
+    kv = [max(0, rng.choice([n, n + spread(20000), n + spread(300), n - spread(50)])) for n in new]
+    most_q = max(1, spread(max(new))) if over else max(new) + rng.choice([0, 0, 3])
+    most_kv = max(1, max(kv) - spread(max(kv) + 1)) if over else max(1, max(kv)) + rng.choice([0, 0, 1000])
+    return call(new, kv, most_q, most_kv, rng.choice([0, 1, spread(2000), spread(2000)]), rng.random() < 0.5,
+                rng.choice([1, 2, 8]), rng.choice([1, 3, 8]), rng.choice([64, 128, 256]), rng.choice([1, 3]),
+                rng.choice([0, 1, 2]), rng.random() < 0.5)
+
+
+def test_calls_as_described(ask):
+    rng = random.Random(1)
+    assert not ask([drawn(rng, False) for _ in range(3000)])
