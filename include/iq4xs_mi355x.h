@@ -421,8 +421,10 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * nothing but BF16 outputs is asked for, of more than 32 rows of a cache head (new
  * tokens times q_heads / heads), keys become fp16 and weights are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
- * above most_kv or the table, the first keys count.  Rows past most_q, and those
- * of no sequence, are not written.  The same call gives the same bits. */
+ * above most_kv or the table, the first keys count.  A sequence of more new tokens
+ * than most_q has its first most_q rows computed, at the places that starts gives
+ * them; rows past most_q, and those of no sequence, are not written.  The same call
+ * gives the same bits. */
 int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
 /* ================================ debug exports ================================

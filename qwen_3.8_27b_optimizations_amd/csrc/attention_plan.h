@@ -53,25 +53,32 @@ IQ4XS_BOTH inline Sequence sequence(const Args& a, int seq, int& total_fresh) {
     return s;
 }
 
+// The split that a key belongs to.  The last one goes on to the end: lengths are read on the device, and a sequence of more
+// new tokens than most_q may see more keys than the splits were planned for (with a window, its first row's lies further
+// back).
+template <typename Args>
+IQ4XS_BOTH inline int split_of(const Args& a, const Sequence& s, int key) {
+    const int split = (key - s.seen_from) / a.chunk;
+    return split < a.splits ? split : a.splits - 1;
+}
+
 // The keys [k0, k1) that a workgroup of rows that see some of [lo, hi) takes as its split; false: none, and no rows to
 // write either.
 template <typename Args>
 IQ4XS_BOTH inline bool split_keys(const Args& a, const Sequence& s, int lo, int hi, int split, int& k0, int& k1) {
-    k0 = s.seen_from + split * a.chunk;
-    k1 = hi;
-    if (a.splits > 1) {
-        k1 = hi < k0 + a.chunk ? hi : k0 + a.chunk;
-        if (k1 <= k0 || k0 + a.chunk <= lo) return false;
-    }
-    if (k0 < (lo & ~31)) k0 = lo & ~31;
+    const int64_t from = s.seen_from + (int64_t)split * a.chunk, to = from + a.chunk;
+    const bool last = split + 1 == a.splits;
+    if (a.splits > 1 && (hi <= from || (!last && to <= lo))) return false;
+    k0 = from < (lo & ~31) ? lo & ~31 : (int)from;
+    k1 = last || hi < to ? hi : (int)to;
     return true;
 }
 
 // The splits that hold keys of a row that sees [lo, hi): first and last, which is before the first if there are none.
 template <typename Args>
 IQ4XS_BOTH inline void splits_of(const Args& a, const Sequence& s, int lo, int hi, int& first, int& last) {
-    first = (lo - s.seen_from) / a.chunk;
-    last = hi > lo ? (hi - 1 - s.seen_from) / a.chunk : first - 1;
+    first = split_of(a, s, lo);
+    last = hi > lo ? split_of(a, s, hi - 1) : first - 1;
 }
 
 // Where the sums of a row that sees the keys [lo, hi) go: with one split, to the outputs, from the workgroup of that
@@ -81,12 +88,12 @@ enum RowEnd { ROW_OUT, ROW_PART, ROW_NONE };
 
 template <typename Args>
 IQ4XS_BOTH inline bool one_split(const Args& a, const Sequence& s, int lo, int hi) {
-    return a.splits == 1 || (hi > lo && (lo - s.seen_from) / a.chunk == (hi - 1 - s.seen_from) / a.chunk);
+    return a.splits == 1 || (hi > lo && split_of(a, s, lo) == split_of(a, s, hi - 1));
 }
 template <typename Args>
 IQ4XS_BOTH inline RowEnd row_end(const Args& a, const Sequence& s, int lo, int hi, int split) {
     if (!one_split(a, s, lo, hi)) return ROW_PART;
-    return a.splits == 1 || (lo - s.seen_from) / a.chunk == split ? ROW_OUT : ROW_NONE;
+    return a.splits == 1 || split_of(a, s, lo) == split ? ROW_OUT : ROW_NONE;
 }
 
 // What a call launches.

@@ -36,3 +36,24 @@ def test_results_with_a_window_past_every_key(pkg, new, cache):
         for window in (2**31 - 2, 2**31, sys.maxsize):
             got = p.run(pkg, torch.device("cuda:0"), causal, window)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (causal, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [0, 900])
+@pytest.mark.parametrize("most_q,d", [(1, 128), (3, 256), (40, 64), (40, 128)])
+def test_sequences_of_more_new_tokens_than_most_q(pkg, most_q, d, window, causal):
+    """Their first most_q rows against a call that is told how many there are."""
+    import test_gpu_attention as t
+
+    dev, new, kv = torch.device("cuda:0"), [1200, 2, 50], [2600, 30, 700]
+    print(f"[more than most_q] {most_q} {d} {window} {causal}", flush=True)
+    p = t.Problem(kv, new, 2, 4, d, 16, "f16", seed=d)
+    q, c, table, starts, kv_len = p.on(pkg, dev)
+    at = [s + i for s, n in zip((0, 1200, 1202), new) for i in range(min(n, most_q))]
+    want, want_lse = p.run(pkg, dev, causal, window)
+    got, lse = pkg.paged_attention(q, c, table, starts, kv_len, most_q, 2600, causal=causal, window=window, lse=True,
+                                   scale=p.scale)
+    # two ways to split the same sums, each within weights' and output's half steps (2^-11) of values below 6
+    assert bool(((got[at].double() - want[at].double()).abs() <= 2 * 2 * 2.0 ** -11 * 6).all())
+    assert bool(((lse[at] - want_lse[at]).abs() <= 2.0 ** -14).all())

@@ -54,3 +54,14 @@ def drawn(rng, over):
 def test_calls_as_described(ask):
     rng = random.Random(1)
     assert not ask([drawn(rng, False) for _ in range(3000)])
+
+
+def test_sequences_of_more_new_tokens_than_most_q(ask):
+    """Their first most_q rows are computed, and see what they would with a larger most_q: without causal masking that is
+    up to the last key, further than a window of most_q rows reaches."""
+    assert not ask([call([8000], [9000], most_q=4, window=1024, causal=False),
+                    call([600], [600], most_q=1, window=1000, causal=False),
+                    call([600, 2, 600], [5000, 30, 600], most_q=3, window=900, causal=False, heads=8, group=8),
+                    call([8000], [9000], most_q=300, window=1024, causal=False, heads=2)])
+    rng = random.Random(2)
+    assert not ask([drawn(rng, True) for _ in range(3000)])
