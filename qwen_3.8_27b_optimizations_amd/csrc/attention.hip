@@ -21,7 +21,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(AttentionArgs
     int total_fresh;
     const Sequence s = sequence(a, seq, total_fresh);
     const int token = row - s.first;
-    if (token >= s.fresh) return;
+    if (token < 0 || token >= s.fresh) return;  // below zero: starts that fall
     const int lo = least_key(a, s, total_fresh, token), hi = end_key(a, s, total_fresh, token);
     if (one_split(a, s, lo, hi)) return;
     int from, to;
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_of_many_kernel(Atten
                 int total_fresh;
                 const Sequence s = sequence(a, seq, total_fresh);
                 const int token = row - s.first;
-                skip = token >= s.fresh;
+                skip = token < 0 || token >= s.fresh;
                 if (!skip) {
                     const int lo = least_key(a, s, total_fresh, token), hi = end_key(a, s, total_fresh, token);
                     skip = one_split(a, s, lo, hi);

@@ -70,7 +70,8 @@ __global__ __launch_bounds__(64 * GATHER_WAVES) void kv_gather_kernel(GatherArgs
     if (seq >= 0 && seq < a.seqs) {
         const int64_t j = row - a.starts[seq];
         off = (int)j & ((1 << a.c.shift) - 1);
-        if ((j >> a.c.shift) < a.width) page = a.table[seq * a.width + (j >> a.c.shift)];
+        // j below zero: starts that fall
+        if (j >= 0 && (j >> a.c.shift) < a.width) page = a.table[seq * a.width + (j >> a.c.shift)];
     }
     const bool there = page >= 0 && page < a.c.pages;
     for (int head = sub; head < 2 * a.c.heads; head += HEADS) {

@@ -57,3 +57,40 @@ def test_sequences_of_more_new_tokens_than_most_q(pkg, most_q, d, window, causal
     # two ways to split the same sums, each within weights' and output's half steps (2^-11) of values below 6
     assert bool(((got[at].double() - want[at].double()).abs() <= 2 * 2 * 2.0 ** -11 * 6).all())
     assert bool(((lse[at] - want_lse[at]).abs() <= 2.0 ** -14).all())
+
+
+def rising(starts, rows):
+    """For each row the sequence whose start is the last at or below it, counted as the kernels count."""
+    return [sum(s <= r for s in starts) - 1 for r in rows]
+
+
+FALLING = [[100, 200, 300, 5], [700, 900, 1000, 0], [0, 50, 20, 60]]
+
+
+def test_starts_that_fall_put_rows_before_their_sequence():
+    """The count of starts at or below a row then names a sequence that begins after it: what the kernels must look for."""
+    for starts in FALLING[:2]:
+        seq = rising(starts, range(60))
+        assert any(0 <= s < 3 and starts[s] > r and starts[s + 1] > starts[s] for r, s in enumerate(seq))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", FALLING)
+def test_starts_that_fall_stay_in_bounds(pkg, starts):
+    """Not a call that has an answer: rows of no sequence are zero where the cache is read back, and nothing else is read
+    than tables and pages."""
+    import test_gpu_attention as t
+
+    dev = torch.device("cuda:0")
+    print(f"[falling starts] {starts}", flush=True)
+    p = t.Problem([3000, 2000, 1000], [20] * 3, 2, 4, 128, 16, "f16")
+    q, c, table, _, kv_len = p.on(pkg, dev)
+    fall = torch.tensor(starts, dtype=torch.int32, device=dev)
+    k, v = pkg.kv_gather(c, table, fall, 60)
+    seq = rising(starts, range(60))
+    for r, s in enumerate(seq):
+        if not (0 <= s < 3) or starts[s] > r:
+            assert not bool(k[r].any()) and not bool(v[r].any())
+    out, lse = pkg.paged_attention(q, c, table, fall, kv_len, 20, 3000, window=1500, lse=True)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape
