@@ -405,7 +405,8 @@ struct iq4xs_paged_attention_args {
     float scale;
 };
 
-/* Bytes of workspace iq4xs_paged_attention needs; 0 also for arguments it refuses. */
+/* Bytes of workspace iq4xs_paged_attention needs; 0 also for arguments it refuses
+ * (IQ4XS_ERROR_INVALID_CONFIG: total * q_heads, or its workgroups, past 2^31 - 1). */
 size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args);
 
 /* out = softmax(scale * q k^T over the visible keys) v, lse = log(sum(exp(scale
@@ -421,7 +422,7 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * nothing but BF16 outputs is asked for, of more than 32 rows of a cache head (new
  * tokens times q_heads / heads), keys become fp16 and weights are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
- * above most_kv or the table, the first keys count.  A sequence of more new tokens
+ * above most_kv, the table or 2^31 - 4096, the first keys count.  A sequence of more new tokens
  * than most_q has its first most_q rows computed, at the places that starts gives
  * them; rows past most_q, and those of no sequence, are not written.  The same call
  * gives the same bits. */

@@ -129,6 +129,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_of_many_kernel(Atten
     }
 }
 
+bool paged_attention_fits(const iq4xs_paged_attention_args& g) {
+    return rows_fit(g) && plan_of(g, device_cu_count()).grid <= MAX_GRID;
+}
+
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& g) {
     const int splits = plan_of(g, device_cu_count()).splits;
     return part_bytes(g, splits) + part_bytes(g, splits) / g.cache->head_dim * 4;
@@ -141,11 +145,10 @@ hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws,
     float* part = static_cast<float*>(ws);
     const AttentionArgs a{cache_pages(*g.cache), g.q, g.out, g.lse, g.table, g.starts, g.kv_len, part,
                           p.splits > 1 ? part + part_bytes(g, p.splits) / sizeof(float) : nullptr, g.q_stride,
-                          g.table_width, (int)g.total, (int)g.most_q, (int)g.most_kv, (int)window_of(g), (int)g.seqs,
+                          g.table_width, (int)g.total, (int)g.most_q, most_kv_of(g), (int)window_of(g), (int)g.seqs,
                           g.q_heads, g.q_heads / g.cache->heads, g.out_type, g.causal, p.splits, p.chunk, p.row_tiles,
                           g.scale * 1.44269504089f};
     const int64_t join = g.total * g.q_heads;
-    if (p.grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     if (p.tiles)
         launch_stream_attention(a, D, p.tiles, g.type, g.cache->type, p.grid, stream);
     else

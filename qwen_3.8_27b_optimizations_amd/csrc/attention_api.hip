@@ -58,12 +58,12 @@ int check_attention(const iq4xs_paged_attention_args* a) {
     if (!plain_type(a->out_type) || (a->type != IQ4XS_TYPE_F16 && a->type != IQ4XS_TYPE_BF16))
         return hipErrorInvalidValue;
     if (c.type != IQ4XS_TYPE_Q8 && c.type != a->type) return hipErrorInvalidValue;
-    if (a->total < 0 || a->total >= MAX_COUNT || a->seqs < 0 || a->seqs >= MAX_COUNT) return hipErrorInvalidValue;
+    if (a->total < 0 || a->total >= MAX_COUNT || a->seqs < 0 || a->seqs >= MAX_COUNT - 64) return hipErrorInvalidValue;
     if (a->total == 0 || a->seqs == 0) return hipSuccess;
     if (!given(a->q) || !given(a->out) || !a->table || !a->starts || !a->kv_len) return hipErrorInvalidValue;
     if (!count(a->table_width) || !count(a->most_q) || !count(a->most_kv)) return hipErrorInvalidValue;
     if (!stride_of(a->q_stride, a->q_heads, c.head_dim)) return hipErrorInvalidValue;
-    return hipSuccess;
+    return paged_attention_fits(*a) ? hipSuccess : hipErrorInvalidConfiguration;
 }
 
 }  // namespace

@@ -22,6 +22,8 @@ void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, in
 void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
                            hipStream_t stream);
 
+// Whether the launches of a call, whose arguments hold otherwise, are not too large.
+bool paged_attention_fits(const iq4xs_paged_attention_args& args);
 size_t paged_attention_workspace(const iq4xs_paged_attention_args& args);
 hipError_t launch_paged_attention(const iq4xs_paged_attention_args& args, void* ws, hipStream_t stream);
 

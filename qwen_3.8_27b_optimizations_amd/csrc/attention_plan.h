@@ -112,6 +112,17 @@ inline int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 // Positions are below 2^31: a window of that many and more hides nothing, and sums with it could pass 64 bits.
 inline int64_t window_of(const iq4xs_paged_attention_args& g) { return g.window < 0x7FFFFFFF ? g.window : 0; }
 
+// Keys of a sequence that count: their places, and those of a few steps past the end, are ints in the kernels.
+inline int most_kv_of(const iq4xs_paged_attention_args& g) {
+    return (int)at_most(g.most_kv, ((int64_t)1 << 31) - 4096);
+}
+
+// Workgroups of a launch.
+constexpr int64_t MAX_GRID = 0x7FFFFFFF;
+
+// Whether a workgroup for each row and head is a launch, without which the plan's products could pass 64 bits.
+inline bool rows_fit(const iq4xs_paged_attention_args& g) { return g.total <= MAX_GRID / g.q_heads; }
+
 inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;

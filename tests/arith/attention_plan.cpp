@@ -2,6 +2,8 @@
 // input is a call; the answer is the number of its rows that something goes wrong with.
 //   total most_q most_kv window causal heads group head_dim type out_type lse table_width shift seqs
 //       then seqs + 1 starts and seqs lengths
+// or the word keys, the key that the kernels' places must stay below, and a call as above; the answer is 1 if some
+// sequence has more keys than that.
 #include <iostream>
 #include <sstream>
 #include <string>
@@ -76,6 +78,10 @@ int main() {
     std::string line;
     while (std::getline(std::cin, line)) {
         std::istringstream in(line);
+        const bool ask_keys = line.compare(0, 5, "keys ") == 0;
+        int64_t below = 0;
+        std::string word;
+        if (ask_keys) in >> word >> below;
         iq4xs_kv_cache cache = {};
         iq4xs_paged_attention_args g = {};
         int64_t heads, group, head_dim, type, out_type, lse, causal, shift;
@@ -96,7 +102,16 @@ int main() {
         g.lse = lse ? &some : nullptr;
         const iq4xs::AttentionPlan p = iq4xs::plan_of(g, 256);
         const Args a{nullptr, starts.data(), kv.data(), g.table_width, {(int)shift}, (int)g.total, (int)g.most_q,
-                     (int)g.most_kv, (int)iq4xs::window_of(g), g.causal, p.splits, p.chunk};
+                     iq4xs::most_kv_of(g), (int)iq4xs::window_of(g), g.causal, p.splits, p.chunk};
+        if (ask_keys) {
+            bool more = false;
+            for (int seq = 0; seq < g.seqs; ++seq) {
+                int total_fresh;
+                more = more || iq4xs::sequence(a, seq, total_fresh).keys > below;
+            }
+            std::cout << more << "\n";
+            continue;
+        }
         int64_t wrong = p.splits < 1 || p.chunk < 1 || p.grid < 1;
         for (int seq = 0; seq < g.seqs && !wrong; ++seq) wrong += wrong_rows(a, p, seq, (int)group);
         std::cout << wrong << "\n";

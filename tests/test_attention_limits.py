@@ -94,3 +94,16 @@ def test_starts_that_fall_stay_in_bounds(pkg, starts):
     out, lse = pkg.paged_attention(q, c, table, fall, kv_len, 20, 3000, window=1500, lse=True)
     torch.cuda.synchronize()
     assert out.shape == q.shape
+
+
+@pytest.mark.parametrize("over,heads,code", [
+    (dict(seqs=2**30, total=2**30, most_q=2**30, hq=2**20, qs=2**27), 2**20, 9),  # the plan's products wrap to zero
+    (dict(seqs=2**30, total=2**30, most_q=2**30, hq=2**20, qs=2**27), 1, 9),
+    (dict(total=2**28, most_q=2**28, hq=8, qs=1024), 8, 9),                       # a workgroup for each row and head
+    (dict(seqs=2**30, total=100, most_q=100, hq=8, qs=1024), 8, 9),               # for each sequence and head
+    (dict(seqs=2**31 - 64), 2, 1), (dict(seqs=2**31 - 1), 2, 1)])
+def test_calls_too_large_to_launch_are_refused(pkg, over, heads, code):
+    cache = cache_of(pkg, heads=heads)
+    args = attention_args(pkg, cache, **over)
+    assert pkg.lib().iq4xs_paged_attention_workspace_bytes(args) == 0
+    assert pkg.lib().iq4xs_paged_attention(args, FAKE, 1 << 62, None) == code

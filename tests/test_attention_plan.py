@@ -65,3 +65,10 @@ def test_sequences_of_more_new_tokens_than_most_q(ask):
                     call([8000], [9000], most_q=300, window=1024, causal=False, heads=2)])
     rng = random.Random(2)
     assert not ask([drawn(rng, True) for _ in range(3000)])
+
+
+def test_places_past_the_longest_sequence_are_ints(ask):
+    """Up to two steps of four waves, or three tiles, past a sequence's end are looked at: 256 keys."""
+    below = 2**31 - 1 - 256
+    assert not ask([f"keys {below} " + call([1], [kv], most_kv=2**31 - 1, width=1 << 27, window=w)
+                    for kv in (2**31 - 1, 2**31 - 200, 2**31 - 4096, 5) for w in (0, 1000)])
