@@ -65,6 +65,12 @@ template <typename T>
 struct Matrix;
 template <>
 struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
+    // Weights are 2^(z - m), in 16 bits for their product with the values.  m is set so that the row's largest weight is
+    // 2^LARGEST then, and moves when one passes 2^(LARGEST + 8).  fp16 holds 2^15, and has its full bits down to 2^-14: as
+    // far up as it goes, since a key that takes nearly all of the weight may have a value of nothing, and then the
+    // small weights make the output.  At 2^0 weights 17 nats below the largest were two fifths off or zero, at 2^7 half a
+    // hundredth.
+    static constexpr float LARGEST = 7.0f;
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
@@ -87,6 +93,7 @@ struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
 };
 template <>
 struct Matrix<__bf16> : Pairs<0x7F80u, 0x3F803F80u> {
+    static constexpr float LARGEST = 0.0f;  // fp32's range
     static __device__ f4 mma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }

@@ -12,8 +12,8 @@
 //   are the right operand of O^T as they stand;
 // - the four waves of a workgroup and the splits of a long cache go through different keys; the waves join in LDS, the
 //   splits in a second launch.
-// The running maximum of a row moves only when a key passes it by 2^8 (in powers of two): weights up to 2^8 are as exact
-// in 16 bits as weights up to 1, and the sums need no rescaling in most steps.
+// The running maximum of a row moves only when a key passes it by 2^8 (in powers of two): weights up to 2^8 times the
+// largest are as exact in 16 bits, and the sums need no rescaling in most steps.
 // A step's loads are issued a step ahead, its pages looked up two ahead, and none has a condition, so that each wait is
 // for what it needs.  Registers decide how many workgroups a CU holds: 4 with heads of 64, 2 with 128 (3 of an 8-bit
 // cache), 1 with 256; staging through LDS, two steps of a wave at once and three waves a SIMD by spilling were slower.
@@ -23,7 +23,8 @@
 // 8-bit heads of 256 93 us, of which reading is 19.
 // An 8-bit cache's codes become fp16 (exact); a key's scales (one for 32 channels) multiply the parts of its score in
 // fp32, the values' scales multiply their codes in fp16 (half a step of 2^-11), and the weights go as two fp16 numbers, so
-// that only this rounding is left.  bf16 queries for it become fp16 with a power of
+// that this rounding is left, and that of weights below 2^-21 of the largest, whose second part is below fp16's normal
+// range (2^-32 of the largest each).  bf16 queries for it become fp16 with a power of
 // two taken out of each row, exact down to 2^-14 of the row's largest element.
 #include "attention_core.h"
 #include "attention_internal.h"
@@ -435,8 +436,8 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                     }
                     top = fmaxf(top, z[i][t][r]);
                 }
-            if (__builtin_expect(__any(top > m[i] + 8.0f), 0)) {
-                const float up = fmaxf(max_of_quarters(top), m[i]), keep = __builtin_amdgcn_exp2f(m[i] - up);
+            if (__builtin_expect(__any(top > m[i] + (Matrix<W>::LARGEST + 8.0f)), 0)) {
+                const float up = fmaxf(max_of_quarters(top) - Matrix<W>::LARGEST, m[i]), keep = __builtin_amdgcn_exp2f(m[i] - up);
                 m[i] = up;
                 l[i] *= keep;
                 rounded[i] *= keep;

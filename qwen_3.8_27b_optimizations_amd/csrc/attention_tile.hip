@@ -299,9 +299,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
         top *= factor;
-        if (__builtin_expect(__any(top > m + 8.0f), 0)) {
+        if (__builtin_expect(__any(top > m + (M::LARGEST + 8.0f)), 0)) {
             // whole powers of two, so that scaling the 16-bit weights is exact
-            const float up = fmaxf(ceilf(max_of_halves(top)), m), keep = __builtin_amdgcn_exp2f(m - up);
+            const float up = fmaxf(ceilf(max_of_halves(top)) - M::LARGEST, m), keep = __builtin_amdgcn_exp2f(m - up);
             m = up;
             l *= keep;
             rounded *= keep;
