@@ -416,9 +416,10 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * not see (and all that lies past kv_len) do not reach it, whatever they hold.
  * Scores, statistics and sums are fp32.  For their product with the values,
  * weights are rounded to the cache's 16-bit type; the sum they are divided by is
- * that of the rounded ones.  A Q8 cache: values become fp16 (their magnitudes
- * must be within its range), BF16 queries too, with a power of two taken out of
- * each row; keys are exact and weights two fp16 numbers, high and rest.  Only where
+ * that of the rounded ones.  A Q8 cache: values become fp16 (codes times scale past
+ * its range an infinity, of the rows that see them), BF16 queries too, with a power
+ * of two taken out of each row; keys are exact and weights two fp16 numbers, high and
+ * rest.  Only where
  * nothing but BF16 outputs is asked for, of more than 32 rows of a cache head (new
  * tokens times q_heads / heads), keys become fp16 and weights are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is

@@ -209,11 +209,17 @@ struct Step<D, int8_t> {
         }
     }
     __device__ void prepare_values(int lane) {
-        const int n = lane % 16, j = lane / 16;
+        flip_codes();
+        take_scales(lane);
+    }
+    __device__ void flip_codes() {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int w = 0; w < WORDS; ++w) v[e][w] ^= 0x80808080u;
+    }
+    __device__ void take_scales(int lane) {
+        const int n = lane % 16, j = lane / 16;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
@@ -230,29 +236,49 @@ struct Step<D, int8_t> {
             x[p] = __builtin_bit_cast(uint32_t, code_pair(v[2 * p + 1][t / 4], v[2 * p][t / 4], t % 4) * pair[t / 8][p]);
         return x;
     }
-    // Whether a scale of the step, of a key or a value, is not finite.
+    // Whether a scale of the step, of a key or a value, is not finite, or so large that codes may pass fp16: above 515.5,
+    // 127 times which is the last that rounds to one.
     __device__ bool some_odd() const {
         bool odd = false;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
             const _Float16 x = scale[g];
-            odd = odd || (__builtin_bit_cast(uint16_t, x) & 0x7C00u) == 0x7C00u;
+            odd = odd || (__builtin_bit_cast(uint16_t, x) & 0x7FFFu) > 0x6007u;
         }
         return __any(odd);
     }
-    // A code's value is not finite where its scale is not.
+    // Clears the scales outside the slots of the mask, and those that are not finite or large; whether there were such
+    // inside.
     __device__ bool keep_finite(u4 slots) {
         bool odd = false;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                const u4 x{__builtin_bit_cast(uint32_t, pair[h][p]) & slots[p], 0, 0, 0};
-                const uint32_t f = Matrix<_Float16>::finite(x).x;
-                odd = odd || f != x.x;
-                pair[h][p] = __builtin_bit_cast(h2, f);
+                const uint32_t x = __builtin_bit_cast(uint32_t, pair[h][p]) & slots[p], over = large_halves(x);
+                odd = odd || over != 0;
+                pair[h][p] = __builtin_bit_cast(h2, x & ~over);
             }
         return odd;
+    }
+    // Puts in the scales' place the large ones among them that are finite, times 2^-12, so that no code makes an infinity
+    // of them; whether there are any.
+    __device__ bool large_scales(u4 slots, int lane) {
+        take_scales(lane);
+        uint32_t some = 0;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const uint32_t x = __builtin_bit_cast(uint32_t, pair[h][p]) & slots[p];
+                const uint32_t f = Matrix<_Float16>::finite(u4{x & large_halves(x), 0, 0, 0}).x;
+                some |= f;
+                pair[h][p] = __builtin_bit_cast(h2, f) * h2{(_Float16)0x1p-12f, (_Float16)0x1p-12f};
+            }
+        return __any(some != 0);
+    }
+    static __device__ uint32_t large_halves(uint32_t x) {
+        return ((x & 0x7FFFu) > 0x6007u ? 0xFFFFu : 0u) | ((x >> 16 & 0x7FFFu) > 0x6007u ? 0xFFFF0000u : 0u);
     }
     using Weight = _Float16;
 };
@@ -406,7 +432,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
         find(next, pages, next_row, next_there);
         pages = look_up(next + STEP_KEYS * STREAM_WAVES);
         __builtin_amdgcn_sched_barrier(0);
-        // an infinity times a weight's second part is NaN: with codes, what is not finite is always cleared
+        // an infinity times a weight's second part may be NaN: with codes, what may not be finite is always cleared
         const bool finite = !step.some_odd();
         f4 z[NT][2];
         step.share_scales(lane);
@@ -482,6 +508,50 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     }
 
     if (__builtin_expect(__any(odd), 0)) {
+        if constexpr (EXACT) {
+            // values of large scales come with the weights as they are now, and may be infinities too: those after them
+            for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
+                find(base, look_up(base), row, there);
+                step.load_keys(a, row, n, j);
+                step.share_scales(lane);
+                if (!step.large_scales(seen(base, there), lane)) continue;
+                f4 z[NT][2];
+                u4 w[NT], w_rest[NT];
+                step.scores(queries, z, lane);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    u4 sees = slots_in(base, j, lo[i], hi[i]);
+                    if (!there[0]) sees.x = sees.y = 0;
+                    if (!there[1]) sees.z = sees.w = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float p[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float x = z[i][e / 2][2 * (e % 2) + h] * factor[i] - m[i];
+                            p[h] = sees[e] >> (16 * h) & 1 ? __builtin_amdgcn_exp2f(x) : 0.0f;
+                        }
+                        const uint32_t both = Matrix<W>::pack(p[0], p[1]);
+                        const h2 high = __builtin_bit_cast(h2, both);
+                        w[i][e] = both;
+                        w_rest[i][e] = Matrix<W>::pack(p[0] - (float)high.x, p[1] - (float)high.y);
+                    }
+                }
+                step.load_values(a, row, n, j);
+                step.flip_codes();
+#pragma unroll
+                for (int t = 0; t < OWN; ++t) {
+                    const u4 x = step.values(t);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        f4 part = Matrix<W>::mma16(x, w[i], f4{0, 0, 0, 0});
+                        part = Matrix<W>::mma16(x, w_rest[i], part);
+                        o[i][t] += part * 0x1p12f;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+        }
         // values that are not finite reach the rows that see them as infinities (a NaN as both)
         for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
             find(base, look_up(base), row, there);
