@@ -372,8 +372,9 @@ int iq4xs_qk_norm_rope(const struct iq4xs_qk_norm_rope_args* args, void* stream)
 /* The same, with k and v (v as it is) written to the cache at slots; a token
  * whose slot is negative or past the cache is not stored.  Two tokens of a call
  * must not share a slot.  IQ4XS_TYPE_Q8: for each 32 channels
- * d = fp16(min(amax / 127, 65504 / 127)), codes = rint(x / d) within +-127;
- * a NaN makes its group's scale NaN. */
+ * d = fp16(min(amax / 127, 65504 / 127)), at most 515.5 where fp16 holds amax (127
+ * times the next one, 516, is past it), codes = rint(x / d) within +-127; a NaN
+ * makes its group's scale NaN. */
 int iq4xs_qk_norm_rope_append(const struct iq4xs_qk_norm_rope_args* args, const struct iq4xs_kv_cache* cache,
                               void* stream);
 

@@ -54,7 +54,10 @@ __device__ inline void store_q8(int8_t* codes, _Float16* scales, int64_t row, in
     }
     const float amax = __uint_as_float(group_umax<4>(top));
     float d = amax / 127.0f;
-    d = d > 65504.0f / 127.0f ? 65504.0f / 127.0f : d;  // code * scale stays an fp16 number; NaN passes
+    d = d > 65504.0f / 127.0f ? 65504.0f / 127.0f : d;  // NaN passes
+    // That is 516 in fp16, and 127 times it past fp16: what fp16 holds takes the scale below, whose codes it holds too, and
+    // only what it does not comes back as an infinity there.
+    if (amax < 65520.0f && d > 515.5f) d = 515.5f;
     const _Float16 dh = (_Float16)d;
     const float df = (float)dh;
     uint32_t w[2] = {0, 0};

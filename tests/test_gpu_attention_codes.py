@@ -40,3 +40,48 @@ def test_codes_past_fp16_stay_in_their_rows_and_channels(pkg, dev, scale, code, 
         keep = torch.ones_like(got, dtype=torch.bool)
         keep[first:, 4:, 37] = False
         assert torch.equal(got[keep], out[keep])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_the_largest_values_that_fp16_holds_come_back_finite(pkg, dev, d, kind):  # noqa: F811
+    """Appended, read back in fp16 and attended to.  Half a code's step (515.5 / 2), the last code standing for up to 51
+    less than 65520, and half of fp16's own step there (16); past fp16 what comes back is an infinity in fp16 and 127 * 516
+    in fp32."""
+    held = [65504.0, -65504.0, 65500.0, 65501.0, 65490.0, 65519.0, 40000.0]
+    past = [65536.0, 1e5, -1e30, math.inf]
+    values = torch.tensor(held + past)
+    n = len(values)
+    g = torch.Generator().manual_seed(d)
+    x = (torch.randn(n, 1, d, generator=g) * 3e4).clamp(-6e4, 6e4)
+    x[:, 0, 37] = values
+    x = x.to(kind)
+    if kind == torch.bfloat16:
+        held = held[6:]  # the others round to 65536
+    count = len(held)
+    first = n - len(past) - count
+    cache = pkg.KVCache(*(torch.zeros(1, 1, 16, w, dtype=t, device=dev)
+                          for w, t in ((d, torch.int8), (d, torch.int8), (d // 32, torch.float16), (d // 32, torch.float16))))
+    at = torch.arange(n, device=dev)
+    q = torch.randn(n, 4, d, generator=g).to(kind).to(dev)
+    pkg.qk_norm_rope_append(q, torch.zeros_like(x).to(dev), x.to(dev), at.int(), at, cache, out_type=torch.float16)
+    table, starts = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([0, n], dtype=torch.int32, device=dev)
+    _, v16 = pkg.kv_gather(cache, table, starts, n, out_type=torch.float16)
+    _, v32 = pkg.kv_gather(cache, table, starts, n, out_type=torch.float32)
+    v16, v32 = v16.cpu(), v32.cpu()
+    rows = slice(first, first + count)
+    assert bool(torch.isfinite(v16[rows]).all())
+    err = (v16[rows].double() - x[rows].double()).abs()
+    assert bool((err <= 515.5 / 2 + 51 + 16).all()), err.max().item()
+    over = x[first + count:, 0, 37].double()
+    assert bool((v16[first + count:, 0, 37] == over.sign() * math.inf).all())
+    assert bool((v32[first + count:, 0, 37].double() == over.sign() * 127 * 516).all())
+    # a row that sees only values that fp16 holds, as a single token and among many
+    for new in (1, 20):
+        one = lambda *i: torch.tensor(i, dtype=torch.int32, device=dev)  # noqa: E731
+        out = pkg.paged_attention(q[:1].half().expand(new, -1, -1).contiguous(), cache, table, one(0, new),
+                                  one(first + count), new, n, causal=False, window=0, out_type=torch.float32)
+        if first == 0:  # keys of zero: equal weights
+            want = v16[rows].double().mean(0)
+            # values in fp16, half a step of 32 at the most, and their mean once more
+            assert bool(((out.cpu().double() - want).abs() <= 32).all())
