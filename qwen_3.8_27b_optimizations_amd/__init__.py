@@ -356,9 +356,9 @@ def _rows(t, name: str):
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head]")
     (tokens, heads, d), (step, between, within) = t.shape, t.stride()
-    if within != 1 or between != d:
+    if within != 1 or (between != d and heads > 1):
         raise ValueError(f"{name}: a token's heads must lie one after another")
-    # the stride of a single token says nothing
+    # the stride of a single head or token says nothing
     return tokens, heads, d, step if tokens > 1 else heads * d
 
 

@@ -107,3 +107,31 @@ def test_calls_too_large_to_launch_are_refused(pkg, over, heads, code):
     args = attention_args(pkg, cache, **over)
     assert pkg.lib().iq4xs_paged_attention_workspace_bytes(args) == 0
     assert pkg.lib().iq4xs_paged_attention(args, FAKE, 1 << 62, None) == code
+
+
+def test_the_stride_between_the_heads_of_one_head_says_nothing(pkg):
+    x = torch.zeros(3, 7, 128).transpose(0, 1)  # [tokens, heads, head], a head's tokens one after another
+    assert pkg._rows(x[:, :1], "q") == (7, 1, 128, 128)
+    assert pkg._rows(torch.zeros(7, 3, 128)[:, 1:2], "q") == (7, 1, 128, 384)
+    for bad in (x, x[:, :2], torch.zeros(7, 1, 256)[..., ::2]):
+        with pytest.raises(ValueError):
+            pkg._rows(bad, "q")
+
+
+@pytest.mark.gpu
+def test_one_head_of_another_layout(pkg):
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(4, 9, 128, generator=g, device=dev).half().transpose(0, 1)  # [9 tokens, 4 heads, 128]
+    pos = torch.arange(9, dtype=torch.int32, device=dev)
+    views, copies = [x[:, i:i + 1] for i in range(3)], [x[:, i:i + 1].contiguous() for i in range(3)]
+    assert all(torch.equal(a, b) for a, b in zip(pkg.qk_norm_rope(*views[:2], pos), pkg.qk_norm_rope(*copies[:2], pos)))
+    results = []
+    for q, k, v in (views, copies):
+        cache = pkg.KVCache(*(torch.zeros(1, 1, 16, 128, dtype=torch.float16, device=dev) for _ in range(2)))
+        q = pkg.qk_norm_rope_append(q, k, v, pos, pos.long(), cache)
+        results.append((q, cache.k_pages, cache.v_pages))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    i32 = lambda *n: torch.tensor(n, dtype=torch.int32, device=dev)  # noqa: E731
+    out = [pkg.paged_attention(q, cache, i32(0)[None], i32(0, 9), i32(9), 9, 9) for q in (views[0], copies[0])]
+    assert torch.equal(*out)
