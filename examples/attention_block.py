@@ -50,7 +50,10 @@ class Sequences:
         self.lengths = [0] * count  # on the host, as of the last grow()
 
     def slots(self, seq, pos):
-        return self.table[seq, pos // self.page].long() * self.page + pos % self.page
+        """Where tokens go; past the room nowhere, -1, and they are not stored."""
+        inside = pos < self.room
+        page = self.table[seq, (pos // self.page).clamp(max=self.room // self.page - 1)]
+        return torch.where(inside, page.long() * self.page + pos % self.page, -1)
 
     def grow(self, new):
         """The new tokens of each sequence: (pos, slots, starts), one sequence after another; lengths move on."""
@@ -61,14 +64,15 @@ class Sequences:
         starts = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device=self.device)
         seq = self.rows.repeat_interleave(new_d)
         pos = torch.arange(sum(new), device=self.device) - starts[seq] + self.kv_len[seq]
-        self.kv_len += new_d.int()
+        self.kv_len.add_(new_d.int()).clamp_(max=self.room)
         self.lengths = lengths
         return pos.int(), self.slots(seq, pos), starts
 
     def step(self):
-        """One new token for each sequence, without the host: may be captured.  The caller counts the steps."""
+        """One new token for each sequence, without the host: may be captured.  The caller counts the steps; a sequence
+        whose room is full stays as it is, and its new token sees what it holds."""
         pos = self.kv_len.clone()
-        self.kv_len += 1
+        self.kv_len.add_(1).clamp_(max=self.room)
         return pos, self.slots(self.rows, pos.long()), self.each
 
 
