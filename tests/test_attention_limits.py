@@ -135,3 +135,24 @@ def test_one_head_of_another_layout(pkg):
     i32 = lambda *n: torch.tensor(n, dtype=torch.int32, device=dev)  # noqa: E731
     out = [pkg.paged_attention(q, cache, i32(0)[None], i32(0, 9), i32(9), 9, 9) for q in (views[0], copies[0])]
     assert torch.equal(*out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,d", [(1, 128), (5, 256), (60, 64)])
+def test_most_kv_off_the_truth(pkg, new, d):
+    """Below it the first keys count, as if the sequences were that long; above it the splits change and nothing else."""
+    import test_gpu_attention as t
+
+    dev = torch.device("cuda:0")
+    print(f"[most_kv] {new} {d}", flush=True)
+    p = t.Problem([3000, new + 100, 700], [new] * 3, 2, 4, d, 16, "f16", seed=d)
+    q, c, table, starts, kv_len = p.on(pkg, dev)
+    ask = lambda lens, most: pkg.paged_attention(q, c, table, starts, lens, new, most, lse=True)  # noqa: E731
+    cut = ask(kv_len, 1000)
+    assert all(torch.equal(a, b) for a, b in zip(cut, ask(kv_len.clamp(max=1000), 1000)))
+    for most in (3001, 100000, 2**31 - 1):
+        out, lse = ask(kv_len, most)
+        want, want_lse = ask(kv_len, 3000)
+        # two ways to split the same sums, each within weights' and output's half steps (2^-11) of values below 6
+        assert bool(((out.double() - want.double()).abs() <= 2 * 2 * 2.0 ** -11 * 6).all())
+        assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
