@@ -129,18 +129,23 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_splits_of_many_kernel(Atten
     }
 }
 
-bool paged_attention_fits(const iq4xs_paged_attention_args& g) {
-    return rows_fit(g) && plan_of(g, device_cu_count()).grid <= MAX_GRID;
+static size_t workspace_of(const iq4xs_paged_attention_args& g, const AttentionPlan& p) {
+    return part_bytes(g, p.splits) + part_bytes(g, p.splits) / g.cache->head_dim * 4;
 }
 
-size_t paged_attention_workspace(const iq4xs_paged_attention_args& g) {
-    const int splits = plan_of(g, device_cu_count()).splits;
-    return part_bytes(g, splits) + part_bytes(g, splits) / g.cache->head_dim * 4;
+hipError_t paged_attention_workspace(const iq4xs_paged_attention_args& g, size_t* bytes) {
+    AttentionPlan p;
+    if (!plan_fits(g, device_cu_count(), p)) return hipErrorInvalidConfiguration;
+    *bytes = workspace_of(g, p);
+    return hipSuccess;
 }
 
-hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws, hipStream_t stream) {
+hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws, size_t ws_bytes, hipStream_t stream) {
+    AttentionPlan p;
+    if (!plan_fits(g, device_cu_count(), p)) return hipErrorInvalidConfiguration;
+    const size_t need = workspace_of(g, p);
+    if (ws_bytes < need || (need && (!ws || reinterpret_cast<uintptr_t>(ws) % 256 != 0))) return hipErrorInvalidValue;
     clear_launch_error();
-    const AttentionPlan p = plan_of(g, device_cu_count());
     const int D = g.cache->head_dim;
     float* part = static_cast<float*>(ws);
     const AttentionArgs a{cache_pages(*g.cache), g.q, g.out, g.lse, g.table, g.starts, g.kv_len, part,

@@ -63,7 +63,7 @@ int check_attention(const iq4xs_paged_attention_args* a) {
     if (!given(a->q) || !given(a->out) || !a->table || !a->starts || !a->kv_len) return hipErrorInvalidValue;
     if (!count(a->table_width) || !count(a->most_q) || !count(a->most_kv)) return hipErrorInvalidValue;
     if (!stride_of(a->q_stride, a->q_heads, c.head_dim)) return hipErrorInvalidValue;
-    return paged_attention_fits(*a) ? hipSuccess : hipErrorInvalidConfiguration;
+    return hipSuccess;
 }
 
 }  // namespace
@@ -106,15 +106,14 @@ int iq4xs_kv_gather(const struct iq4xs_kv_cache* cache, const int32_t* table, in
 
 size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args) {
     if (check_attention(args) != hipSuccess || args->total == 0 || args->seqs == 0) return 0;
-    return paged_attention_workspace(*args);
+    size_t bytes = 0;
+    return paged_attention_workspace(*args, &bytes) == hipSuccess ? bytes : 0;
 }
 
 int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream) {
     const int err = check_attention(args);
     if (err != hipSuccess || args->total == 0 || args->seqs == 0) return err;
-    const size_t need = paged_attention_workspace(*args);
-    if (ws_bytes < need || (need && (!ws || reinterpret_cast<uintptr_t>(ws) % 256 != 0))) return hipErrorInvalidValue;
-    return launch_paged_attention(*args, ws, static_cast<hipStream_t>(stream));
+    return launch_paged_attention(*args, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

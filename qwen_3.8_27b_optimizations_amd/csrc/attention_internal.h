@@ -22,9 +22,9 @@ void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, in
 void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
                            hipStream_t stream);
 
-// Whether the launches of a call, whose arguments hold otherwise, are not too large.
-bool paged_attention_fits(const iq4xs_paged_attention_args& args);
-size_t paged_attention_workspace(const iq4xs_paged_attention_args& args);
-hipError_t launch_paged_attention(const iq4xs_paged_attention_args& args, void* ws, hipStream_t stream);
+// hipErrorInvalidConfiguration: a call whose launches would be too large.
+hipError_t paged_attention_workspace(const iq4xs_paged_attention_args& args, size_t* bytes);
+// The same, and hipErrorInvalidValue for a workspace that is too small or not aligned to 256 bytes.
+hipError_t launch_paged_attention(const iq4xs_paged_attention_args& args, void* ws, size_t ws_bytes, hipStream_t stream);
 
 }  // namespace iq4xs

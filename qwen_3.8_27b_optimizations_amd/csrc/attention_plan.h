@@ -117,12 +117,6 @@ inline int most_kv_of(const iq4xs_paged_attention_args& g) {
     return (int)at_most(g.most_kv, ((int64_t)1 << 31) - 4096);
 }
 
-// Workgroups of a launch.
-constexpr int64_t MAX_GRID = 0x7FFFFFFF;
-
-// Whether a workgroup for each row and head is a launch, without which the plan's products could pass 64 bits.
-inline bool rows_fit(const iq4xs_paged_attention_args& g) { return g.total <= MAX_GRID / g.q_heads; }
-
 inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
@@ -174,6 +168,15 @@ inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     p.row_tiles = (int)(row_tiles < 0x7FFFFFFF ? row_tiles : 0x7FFFFFFF);
     p.grid = pairs * p.splits;
     return p;
+}
+
+// The plan of a call, unless its launches would be too large: a workgroup for each row and head, without whose limit the
+// plan's products could pass 64 bits, and the plan's own.
+inline bool plan_fits(const iq4xs_paged_attention_args& g, int64_t cus, AttentionPlan& p) {
+    constexpr int64_t MOST = 0x7FFFFFFF;
+    if (g.total > MOST / g.q_heads) return false;
+    p = plan_of(g, cus);
+    return p.grid <= MOST;
 }
 
 inline size_t part_bytes(const iq4xs_paged_attention_args& g, int splits) {
