@@ -416,18 +416,19 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * row that sees nothing gives zeros and -Inf.  Keys and values that a row does
  * not see (and all that lies past kv_len) do not reach it, whatever they hold.
  * Scores, statistics and sums are fp32.  For their product with the values,
- * weights are rounded to the cache's 16-bit type; the sum they are divided by is
- * that of the rounded ones.  A Q8 cache: values become fp16 (codes times scale past
- * its range an infinity, of the rows that see them), BF16 queries too, with a power
- * of two taken out of each row; keys are exact and weights two fp16 numbers, high and
- * rest.  Only where
- * nothing but BF16 outputs is asked for, of more than 32 rows of a cache head (new
- * tokens times q_heads / heads), keys become fp16 and weights are one.
+ * weights are rounded to the cache's 16-bit type (fp16 ones to 2^-32 of the row's
+ * largest below 2^-21 of it); the sum they are divided by is that of the rounded
+ * ones.  A Q8 cache: values become fp16 (codes times scale past its range an
+ * infinity, of the rows that see them), BF16 queries too, with a power of two taken
+ * out of each row; keys are exact and weights two fp16 numbers, high and rest.  Only
+ * where nothing but BF16 outputs is asked for, of more than 32 rows of a cache head
+ * (new tokens times q_heads / heads), keys become fp16, within its range, and weights
+ * are one.
  * Tokens on a page that is not in the cache are as masked ones.  Where kv_len is
- * above most_kv, the table or 2^31 - 4096, the first keys count.  A sequence of more new tokens
- * than most_q has its first most_q rows computed, at the places that starts gives
- * them; rows past most_q, and those of no sequence, are not written.  The same call
- * gives the same bits. */
+ * above most_kv, the table or 2^31 - 4096, the first keys count.  A sequence of more
+ * new tokens than most_q has its first most_q rows computed, at the places that
+ * starts gives them; rows past most_q, and those of no sequence, are not written.
+ * The same call gives the same bits. */
 int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
 /* ================================ debug exports ================================

@@ -495,8 +495,9 @@ def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, 
     starts [seqs + 1] (int32): first row of each sequence; kv_len [seqs] (int32): its cached tokens, new ones included;
     table [seqs, pages of the longest] (int32).  most_q and most_kv: at least the new and the cached tokens of any
     sequence.  New token i stands at p = kv_len - new + i and sees keys up to p (causal) and after p - window (window >
-    0).  scale defaults to head ** -0.5, out_type to q's.  Returns out, or (out, log-sum-exp of the scores [total,
-    q_heads] in fp32) with lse; a row that sees nothing gives zeros and -inf."""
+    0; past every key as good as none).  scale defaults to head ** -0.5, out_type to q's.  Returns out, or (out,
+    log-sum-exp of the scores [total, q_heads] in fp32) with lse; a row that sees nothing gives zeros and -inf.  Rows of no
+    sequence, and those of a sequence past most_q, are left as they were allocated."""
     torch = _torch()
     here = _here(torch, q)
     types = _types(torch)

@@ -161,7 +161,8 @@ hipError_t launch_paged_attention(const iq4xs_paged_attention_args& g, void* ws,
     if (p.splits > 1) {
         const dim3 threads(JOIN_THREADS);
         // a workgroup for each costs 1.3 ns; a wave for four is slower while there are few, whose splits then wait for
-        // each other (4 x 64 tokens, 16384 pairs: 84 us of a call in all, 78 so; 8 x 8 tokens, 4096 pairs: 47 and 50)
+        // each other (of a call in all, 64 heads: one token over 4096 keys 12 us, 25 so; 8 x 8 tokens, 4096 pairs, 67 and
+        // 68; 4 x 64 over 8192 keys, 16384 pairs, 107 and 93)
         const bool many = join >= 16384;
         const int64_t each = JOIN_THREADS / 64 * JOIN_EACH;
         const dim3 blocks((unsigned)(many ? (join + each - 1) / each : join));

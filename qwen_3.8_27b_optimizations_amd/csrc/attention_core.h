@@ -82,7 +82,7 @@ struct Matrix<_Float16> : Pairs<0x7C00u, 0x3C003C00u> {
     }
     // A pair of weights onto a sum, exact products and one fp32 sum (fp16 below its normal range too).  What the values'
     // sum is divided by has to be the sum of the weights as they are rounded, or a row of one key is off by its
-    // weight's rounding: over short rows, 1.5 times the error.
+    // weight's rounding, and rows of few keys by most of theirs.
     static __device__ float add(uint32_t pair, float sum) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), h2{(_Float16)1, (_Float16)1}, sum, false);
     }

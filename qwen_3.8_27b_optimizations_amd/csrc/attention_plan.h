@@ -121,11 +121,12 @@ inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
     AttentionPlan p;
     // Where the kernel of few rows ends: at two 16-row tiles, beyond which reading the keys again for the third costs more
-    // than the other kernel's idle rows (40 rows: 75 against 54 us with 16-bit caches, 48 rows of an 8-bit one for bf16
-    // outputs 94 against 72 of 256 channels, 64 against 57 of 128).  With exact 8-bit keys, which cost the other kernel
-    // more, at 64 rows, with heads of 256 at 48 (64 rows of 64, 128, 256 channels: 66, 70, 121 against 99, 79, 115 us; 128
-    // rows: 110, 118, 218 against 93, 87, 116).  One tile at a time where two do not fit the registers or leave most of the
-    // second empty.
+    // than the other kernel's idle rows (8 sequences of 9001 keys, 40 rows a cache head, of 64, 128, 256 channels: 16-bit
+    // caches 90, 82, 80 us here and 70, 58, 66 there, 8-bit ones for bf16 outputs 88, 77, 96 and 72, 59, 71; 32 rows: 64,
+    // 61, 58 and 73, 57, 66, and 55, 51, 68 and 74, 57, 70).  With exact 8-bit keys, which cost the other kernel more, at 64
+    // rows, with heads of 256 at 48 (48 rows: 87, 77, 95 and 102, 82, 112; 64 rows: 91, 82, 125 and 106, 84, 115; 128 rows:
+    // 163, 150, 246 and 107, 95, 123).  One tile at a time where two do not fit the registers or leave most of the second
+    // empty.
     const int64_t rows = most_q * group;
     const bool codes = g.cache->type == IQ4XS_TYPE_Q8, wide = g.cache->head_dim == 256;
     if (rows > (codes && exact_keys(g) ? wide ? 48 : 64 : 32))
@@ -142,8 +143,8 @@ inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     if (p.tiles) {
         // One sequence, whose splits are alike: the workgroups that the CUs hold at once (by registers; one for each CU
         // keeps enough 16-bit keys on their way), none with less than 128 keys, 32 for a wave.  Several, which may
-        // differ: up to eight times as many, in whole rounds (a few more than a round cost another: 8 sequences of 9001
-        // keys of 256 channels 53 us in 9 splits, 35 in 8), while they have 512 keys (1024 of 256 channels).
+        // differ: up to eight times as many, in whole rounds (a few more than a round cost another: 8 x 2 tokens over
+        // 9001 keys of 8-bit heads of 256 40 us, 61 in one split more), while they have 512 keys (1024 of 256 channels).
         const int64_t held = g.cache->head_dim == 64 ? 4 : g.cache->head_dim == 256 ? 1 : p.tiles == 2 ? 2 : codes ? 3 : 2;
         const int64_t one = g.seqs == 1 && !codes && g.cache->head_dim == 128 ? 1 : held;
         const int64_t round = one * cus / pairs;  // splits of one
@@ -155,10 +156,10 @@ inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
             splits = at_most(round * (rounds > 1 ? rounds : 1), (span + 127) / 128);
         }
     } else {
-        // the workgroups that the CUs hold at once, none with less than 512 keys: one with heads of 256 (1024-token
-        // prompt 94 us with two, 50 with one), two with 128, and of 64, where they hold three, two for one sequence and
-        // four for several, whose lengths differ (16 tokens over 32768 keys 43 us with two, 50 with four; 8 x 8 tokens 65
-        // and 54)
+        // the workgroups that the CUs hold at once, none with less than 512 keys: one with heads of 256 (a 1024-token
+        // prompt 48 us, 60 with two), two with 128 (33, 58 with four), and of 64, where they hold three, two for one
+        // sequence (16 tokens over 32768 keys 40, 47 with four) and four for several, whose lengths differ (8 x 8 tokens
+        // over 2250 to 9001 keys 54, 65 with two; 80 and 75 over 9001 each, 106 and 87 for 32 x 16 over 1024 to 4096)
         const int64_t held = wide ? 1 : g.cache->head_dim == 64 && g.seqs > 1 ? 4 : 2;
         splits = at_most((held * cus + pairs - 1) / pairs, (span + 511) / 512);
     }

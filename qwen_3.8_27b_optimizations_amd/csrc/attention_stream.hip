@@ -20,7 +20,7 @@
 // Measured: 131072 keys of 8 heads of 128, one token: 96 us, 5.6 TB/s (fp16), 54 us, 5.3 TB/s (8 bits); 64 sequences of up
 // to 16384 tokens: 211 us, 5.0 TB/s.  4096 keys: 6 us, of them latency (a dependent chain of table, keys, scores and
 // values), and 4 of the joining launch.  With more rows vector work grows beside the read: 8 sequences of 40 rows over
-// 8-bit heads of 256 93 us, of which reading is 19.
+// 8-bit heads of 256 94 us, of which reading is 19.
 // An 8-bit cache's codes become fp16 (exact); a key's scales (one for 32 channels) multiply the parts of its score in
 // fp32, the values' scales multiply their codes in fp16 (half a step of 2^-11), and the weights go as two fp16 numbers, so
 // that this rounding is left, and that of weights below 2^-21 of the largest, whose second part is below fp16's normal

@@ -15,16 +15,17 @@
 // - the running maximum of a row moves only when a key passes it by 2^8 (in powers of two);
 // - the scores of the next 32 keys, the weights of these and the value products of those before are one stream of
 //   instructions, in the order written.
-// Measured: 2048 tokens over 16384 keys of 128 channels, 64 query heads on 8: 1050 to 1100 us, 940 to 980 TFLOP/s of
-// fp16 (1440 is what a large library product reaches), 1000 us in bf16; of 64 channels 1250 us, of 256 1130.  Matrix
-// units are busy about half of the time and vector units as long, with little overlap; LDS has no conflicts.
+// Measured: 2048 tokens over 16384 keys of 128 channels, 64 query heads on 8: 1020 to 1150 us from card to card, 900 to
+// 1010 TFLOP/s of fp16 (1440 is what a large library product reaches); on a card of 1022 bf16 took 966, 64 channels 1224,
+// 256 1127.  Matrix units are busy about half of the time and vector units as long, with little overlap; LDS has no
+// conflicts.
 // An 8-bit cache whose outputs are bf16 alone: keys and values become fp16 on their way into LDS (half a step of 2^-11
 // each, an eighth of what such outputs show).  In fp16 outputs that would be 1.7 to 2.4 times the error of their own
 // rounding, and log-sum-exps would be off by 1e-5, so for these (EXACT) keys stay codes, exact in fp16, whose scales
 // multiply the parts of a score in fp32, and weights go as two fp16 numbers: half as many products again and as many
 // vector operations.  bf16 queries become fp16 with a power of two taken out of each row.  2048 tokens over 16384 keys
-// of 128 channels: 1324 us with rounded keys, 1860 with exact ones (of 64 channels 1513 and 2200, of 256 1712 and
-// 2560); the kernel of few rows takes 2690 (2917, 4553).
+// of 128 channels on that card: 1222 us with rounded keys, 1835 with exact ones (of 64 channels 1413 and 2182, of 256
+// 1517 and 2603); the kernel of few rows takes 2428 (2911, 4960).
 #include <type_traits>
 
 #include "attention_core.h"
