@@ -431,6 +431,41 @@ size_t iq4xs_paged_attention_workspace_bytes(const struct iq4xs_paged_attention_
  * The same call gives the same bits. */
 int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
+/* The same with first tokens that stay visible beside the window: new token i also
+ * sees key j < sinks (if j <= p, causal).  With no window, or one that hides nothing,
+ * sinks change nothing.  The workspace is that of the call without them.  Any number
+ * of them is right; one workgroup of a row goes through them all, so that many
+ * thousands are slow. */
+int iq4xs_paged_attention_sinks(const struct iq4xs_paged_attention_args* args, int64_t sinks, void* ws, size_t ws_bytes,
+                                void* stream);
+
+/* Sequences that begin with the same tokens, on the same pages. */
+struct iq4xs_shared_prefix {
+    const int32_t* first; /* [groups + 1] first sequence of each group, never falling; NULL: one group of all */
+    const int32_t* len;   /* [groups] tokens that the sequences of a group share */
+    int64_t groups;
+    int64_t most_len;  /* at least the shared tokens of any group */
+    int64_t most_rows; /* at least the new tokens of a group's sequences together */
+};
+
+/* Bytes of workspace iq4xs_shared_attention needs; 0 also for arguments it refuses. */
+size_t iq4xs_shared_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args,
+                                              const struct iq4xs_shared_prefix* prefix);
+
+/* iq4xs_paged_attention of a batch whose sequences begin with the same tokens, each
+ * group's read and multiplied once for the rows of all its sequences.  Tables and
+ * kv_len are as there (the shared tokens among them); the shared tokens are read on
+ * the pages of a group's first sequence, any number of them, with or without the end
+ * of a page; a sequence of no group shares none.  args->most_kv is at least the cached
+ * tokens of any sequence after its shared ones; args->window is 0 (NOT_SUPPORTED
+ * otherwise: a window's calls read little of a prefix).  New tokens come after the
+ * shared ones (kv_len - new >= len); what a row before their end sees of them is not
+ * specified.  Where len is above most_len, the first of the shared keys count, and the
+ * sequence's own keys go on after those; rows of a group past most_rows are not
+ * written.  An 8-bit cache's keys of the prefix are rounded as there, by most_rows. */
+int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const struct iq4xs_shared_prefix* prefix,
+                           void* ws, size_t ws_bytes, void* stream);
+
 /* ================================ debug exports ================================
  * No counterpart in the reference; they exist so the Q8_1 blocks and the
  * per-32-element int32 sums can be checked bit for bit. */

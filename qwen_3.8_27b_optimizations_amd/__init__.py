@@ -88,6 +88,9 @@ SIGNATURES = {
     "iq4xs_kv_gather": (_INT, [_P, _P, _I64, _P, _I64, _P, _P, _I64, _INT, _P]),
     "iq4xs_paged_attention_workspace_bytes": (ctypes.c_size_t, [_P]),
     "iq4xs_paged_attention": (_INT, [_P, _P, ctypes.c_size_t, _P]),
+    "iq4xs_paged_attention_sinks": (_INT, [_P, _I64, _P, ctypes.c_size_t, _P]),
+    "iq4xs_shared_attention_workspace_bytes": (ctypes.c_size_t, [_P, _P]),
+    "iq4xs_shared_attention": (_INT, [_P, _P, _P, ctypes.c_size_t, _P]),
     "iq4xs_q8_1_to_blocks": (_INT, [_P, _P, _I64, _I64, _P]),
     "iq4xs_subblock_sums": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _INT, _P]),
     "iq4xs_probe_mfma_i8": (_INT, [_P, _P, _P, _P]),
@@ -331,6 +334,7 @@ def dequant(W, n_blocks: int, out=None):
 _CACHE = struct.Struct("@PPPPqiiii")
 _QK = struct.Struct("@PPPqqqPPPPPPPqiiiiiiif")
 _ATTENTION = struct.Struct("@PPPPPPPqqqqqqqiiiif")
+_SHARED = struct.Struct("@PPqqq")
 
 
 _TYPES = {}  # torch dtype -> TYPE_*, filled once a GPU has been seen
@@ -488,17 +492,8 @@ def kv_gather(cache, table, starts, total: int, out_type=None):
     return k, v
 
 
-def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, causal: bool = True, window: int = 0,
-                    lse: bool = False, scale: float | None = None, out_type=None):
-    """Attention of new tokens q [total, q_heads, head] over the paged cache, which holds their own keys and values too.
-
-    starts [seqs + 1] (int32): first row of each sequence; kv_len [seqs] (int32): its cached tokens, new ones included;
-    table [seqs, pages of the longest] (int32).  most_q and most_kv: at least the new and the cached tokens of any
-    sequence.  New token i stands at p = kv_len - new + i and sees keys up to p (causal) and after p - window (window >
-    0; past every key as good as none).  scale defaults to head ** -0.5, out_type to q's.  Returns out, or (out,
-    log-sum-exp of the scores [total, q_heads] in fp32) with lse; a row that sees nothing gives zeros and -inf.  Rows of no
-    sequence, and those of a sequence past most_q, are left as they were allocated."""
-    torch = _torch()
+def _attention(torch, q, cache, table, starts, kv_len, most_q, most_kv, causal, window, lse, scale, out_type):
+    """Packed arguments and outputs of the two calls below, and the GPU."""
     here = _here(torch, q)
     types = _types(torch)
     total, hq, d, q_stride = _rows(q, "q")
@@ -518,10 +513,56 @@ def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, 
     args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), sums.data_ptr() if lse else 0, cache._address, tp, sp, lp,
                            q_stride, width, seqs, total, most_q, most_kv, window, hq, kind, types[out_type],
                            bool(causal), d ** -0.5 if scale is None else scale)
+    return args, out, sums, here
+
+
+def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, causal: bool = True, window: int = 0,
+                    lse: bool = False, scale: float | None = None, out_type=None, sinks: int = 0):
+    """Attention of new tokens q [total, q_heads, head] over the paged cache, which holds their own keys and values too.
+
+    starts [seqs + 1] (int32): first row of each sequence; kv_len [seqs] (int32): its cached tokens, new ones included;
+    table [seqs, pages of the longest] (int32).  most_q and most_kv: at least the new and the cached tokens of any
+    sequence.  New token i stands at p = kv_len - new + i and sees keys up to p (causal) and after p - window (window >
+    0; past every key as good as none), and beside a window the first `sinks` keys.  scale defaults to head ** -0.5,
+    out_type to q's.  Returns out, or (out, log-sum-exp of the scores [total, q_heads] in fp32) with lse; a row that sees
+    nothing gives zeros and -inf.  Rows of no sequence, and those of a sequence past most_q, are left as they were
+    allocated."""
+    torch = _torch()
+    args, out, sums, here = _attention(torch, q, cache, table, starts, kv_len, most_q, most_kv, causal, window, lse, scale,
+                                       out_type)
     L = lib()
     nbytes = L.iq4xs_paged_attention_workspace_bytes(args)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    L.check("iq4xs_paged_attention", args, ws.data_ptr() if nbytes else 0, nbytes,
+    stream = torch._C._cuda_getCurrentRawStream(here)
+    if sinks:
+        L.check("iq4xs_paged_attention_sinks", args, sinks, ws.data_ptr() if nbytes else 0, nbytes, stream)
+    else:
+        L.check("iq4xs_paged_attention", args, ws.data_ptr() if nbytes else 0, nbytes, stream)
+    return (out, sums) if lse else out
+
+
+def shared_attention(q, cache, table, starts, kv_len, shared_len, most_q: int, most_own: int, most_shared: int,
+                     groups=None, most_group: int | None = None, causal: bool = True, lse: bool = False,
+                     scale: float | None = None, out_type=None):
+    """paged_attention of a batch whose sequences begin with the same tokens, on the same pages: those are read and
+    multiplied once for all of them.
+
+    groups [n + 1] (int32): first sequence of each group of sequences that share; None: one group of all.  shared_len [n]
+    (int32): the tokens that a group's sequences share, which new tokens come after.  Tables and kv_len are as in
+    paged_attention, the shared tokens among them.  most_own and most_shared: at least the cached tokens of any sequence
+    after its shared ones, and the shared ones of any group; most_group: at least the new tokens of a group's sequences
+    together (default: all rows).  Rows of a group past most_group are left as they were allocated."""
+    torch = _torch()
+    args, out, sums, here = _attention(torch, q, cache, table, starts, kv_len, most_q, most_own, causal, 0, lse, scale,
+                                       out_type)
+    n = 1 if groups is None else groups.numel() - 1
+    gp = 0 if groups is None else _whole(groups, "groups", torch.int32, (n + 1,), here)
+    prefix = _SHARED.pack(gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared,
+                          max(1, q.size(0)) if most_group is None else most_group)
+    L = lib()
+    nbytes = L.iq4xs_shared_attention_workspace_bytes(args, prefix)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    L.check("iq4xs_shared_attention", args, prefix, ws.data_ptr() if nbytes else 0, nbytes,
             torch._C._cuda_getCurrentRawStream(here))
     return (out, sums) if lse else out
 

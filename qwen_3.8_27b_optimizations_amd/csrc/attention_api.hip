@@ -66,6 +66,16 @@ int check_attention(const iq4xs_paged_attention_args* a) {
     return hipSuccess;
 }
 
+int check_shared(const iq4xs_paged_attention_args* a, const iq4xs_shared_prefix* x) {
+    const int err = check_attention(a);
+    if (err != hipSuccess) return err;
+    if (!x || x->groups <= 0 || x->groups >= MAX_COUNT - 64) return hipErrorInvalidValue;
+    if (!x->first && x->groups != 1) return hipErrorInvalidValue;
+    if (a->window != 0) return hipErrorNotSupported;
+    if (a->total == 0 || a->seqs == 0) return hipSuccess;
+    return x->len && count(x->most_len) && count(x->most_rows) ? hipSuccess : hipErrorInvalidValue;
+}
+
 }  // namespace
 
 extern "C" {
@@ -114,6 +124,29 @@ int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* w
     const int err = check_attention(args);
     if (err != hipSuccess || args->total == 0 || args->seqs == 0) return err;
     return launch_paged_attention(*args, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+int iq4xs_paged_attention_sinks(const struct iq4xs_paged_attention_args* args, int64_t sinks, void* ws, size_t ws_bytes,
+                                void* stream) {
+    const int err = check_attention(args);
+    if (err != hipSuccess) return err;
+    if (sinks < 0) return hipErrorInvalidValue;
+    if (args->total == 0 || args->seqs == 0) return hipSuccess;
+    return launch_sinks_attention(*args, sinks, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+size_t iq4xs_shared_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args,
+                                              const struct iq4xs_shared_prefix* prefix) {
+    if (check_shared(args, prefix) != hipSuccess || args->total == 0 || args->seqs == 0) return 0;
+    size_t bytes = 0;
+    return shared_attention_workspace(*args, *prefix, &bytes) == hipSuccess ? bytes : 0;
+}
+
+int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const struct iq4xs_shared_prefix* prefix,
+                           void* ws, size_t ws_bytes, void* stream) {
+    const int err = check_shared(args, prefix);
+    if (err != hipSuccess || args->total == 0 || args->seqs == 0) return err;
+    return launch_shared_attention(*args, *prefix, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -27,6 +27,16 @@ struct AttentionArgs {
     float scale;  // times log2(e)
 };
 
+// A launch of a call with first tokens or with a shared prefix.
+struct MoreArgs : AttentionArgs {
+    static constexpr bool MORE = true;
+    int pass, sinks;
+    const int32_t* group_first;  // [groups + 1] first sequence of each, or NULL
+    const int32_t* shared_len;   // [groups]
+    int groups, most_shared, all_seqs;
+    int prefix_splits, prefix_chunk, prefix_rows;  // of the prefixes' launch: rows of a group that it took
+};
+
 // Pairs of 16-bit numbers as masks: 0xFFFF where a number is an infinity or NaN and `which` says so of its sign (0 or 1)
 // and of being NaN.
 template <uint32_t EXPONENT, typename Which>

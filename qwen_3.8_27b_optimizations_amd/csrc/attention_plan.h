@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "iq4xs_mi355x.h"
 
 #ifdef __HIPCC__
@@ -16,18 +18,34 @@
 
 namespace iq4xs {
 
+// Where keys end that count.
+constexpr int KEYS_END = (int)(((int64_t)1 << 31) - 4096);
+
 // One sequence of the call, cut to what the arguments allow.
 struct Sequence {
     int first, fresh;  // its rows in q: first row, count
     int keys;          // cached tokens
     int seen_from;     // first key that the first row sees, a multiple of 32: where split 0 begins
     const int32_t* pages;
+    int skip;  // calls with first tokens or a shared prefix: keys that are not among the row's range [least, end)
 };
+
+// What a launch of a call with first tokens or a shared prefix is of: all of the former; of the latter the prefixes, a
+// group of sequences in a sequence's place, or what comes after them.
+enum Pass { PASS_SINKS, PASS_PREFIX, PASS_OWN };
+
+// Whether the arguments are those of such a launch (they say MORE).
+template <typename Args, typename = void>
+struct HasMore : std::false_type {};
+template <typename Args>
+struct HasMore<Args, std::void_t<decltype(Args::MORE)>> : std::true_type {};
 
 template <typename Args>
 IQ4XS_BOTH inline int least_key(const Args& a, const Sequence& s, int total_fresh, int token) {
     const int64_t lo = (int64_t)s.keys - total_fresh + token + 1 - a.window;
-    return a.window > 0 && lo > 0 ? (lo < s.keys ? (int)lo : s.keys) : 0;
+    const int least = a.window > 0 && lo > 0 ? (lo < s.keys ? (int)lo : s.keys) : 0;
+    if constexpr (HasMore<Args>::value) return least > s.skip ? least : s.skip;
+    return least;
 }
 template <typename Args>
 IQ4XS_BOTH inline int end_key(const Args& a, const Sequence& s, int total_fresh, int token) {
@@ -48,8 +66,68 @@ IQ4XS_BOTH inline Sequence sequence(const Args& a, int seq, int& total_fresh) {
     keys = keys < a.most_kv ? keys : a.most_kv;
     keys = keys < (a.width << a.c.shift) ? keys : a.width << a.c.shift;
     s.keys = keys > 0 ? (int)keys : 0;
+    s.skip = 0;
     s.seen_from = least_key(a, s, total_fresh, 0) & ~31;
     s.pages = a.table + (int64_t)seq * a.width;
+    return s;
+}
+
+// The group that holds a sequence, -1 if none does or it has sequences that the call has not; NULL is one group of all.
+template <typename Args>
+IQ4XS_BOTH inline int group_of(const Args& a, int seq) {
+    if (!a.group_first) return 0;
+    int from = 0, to = a.groups;  // the groups before `from` begin at seq or before it, those from `to` on after it
+    while (from < to) {
+        const int mid = (from + to) / 2;
+        if (a.group_first[mid] <= seq)
+            from = mid + 1;
+        else
+            to = mid;
+    }
+    if (from == 0 || seq >= a.group_first[from]) return -1;
+    return a.group_first[from - 1] >= 0 && a.group_first[from] <= a.all_seqs ? from - 1 : -1;
+}
+
+// Shared tokens of a group, cut to what the arguments allow.
+template <typename Args>
+IQ4XS_BOTH inline int shared_keys(const Args& a, int group) {
+    if (group < 0) return 0;
+    int64_t n = a.shared_len[group];
+    n = n < a.most_shared ? n : a.most_shared;
+    n = n < (a.width << a.c.shift) ? n : a.width << a.c.shift;
+    return n > 0 ? (int)n : 0;
+}
+
+// The sequence of a launch with first tokens or of a shared prefix's; with PASS_PREFIX `seq` is a group, whose sequences'
+// rows are one sequence's.
+template <typename Args>
+IQ4XS_BOTH inline Sequence sequence_more(const Args& a, int seq, int& total_fresh) {
+    Sequence s;
+    if (a.pass == PASS_SINKS) {
+        s = sequence(a, seq, total_fresh);
+        s.skip = a.sinks < s.keys ? a.sinks : s.keys;
+    } else if (a.pass == PASS_PREFIX) {
+        const int from = a.group_first ? a.group_first[seq] : 0, to = a.group_first ? a.group_first[seq + 1] : a.all_seqs;
+        const bool some = from >= 0 && to <= a.all_seqs && from < to;
+        s.first = some ? a.starts[from] : 0;
+        total_fresh = some ? a.starts[to] - s.first : 0;
+        s.fresh = total_fresh < a.most_q ? total_fresh : a.most_q;
+        if (s.first < 0) s.fresh = 0;
+        if (s.fresh > a.total - s.first) s.fresh = a.total - s.first;
+        s.keys = shared_keys(a, seq);
+        s.pages = a.table + (int64_t)(some ? from : 0) * a.width;
+        s.skip = 0;
+    } else {
+        s = sequence(a, seq, total_fresh);
+        const int skip = shared_keys(a, group_of(a, seq));
+        int64_t keys = a.kv_len[seq];
+        keys = keys < (int64_t)skip + a.most_kv ? keys : (int64_t)skip + a.most_kv;
+        keys = keys < (a.width << a.c.shift) ? keys : a.width << a.c.shift;
+        keys = keys < KEYS_END ? keys : KEYS_END;
+        s.keys = keys > 0 ? (int)keys : 0;
+        s.skip = skip < s.keys ? skip : s.keys;
+    }
+    s.seen_from = least_key(a, s, total_fresh, 0) & ~31;
     return s;
 }
 
@@ -71,6 +149,21 @@ IQ4XS_BOTH inline bool split_keys(const Args& a, const Sequence& s, int lo, int 
     if (a.splits > 1 && (hi <= from || (!last && to <= lo))) return false;
     k0 = from < (lo & ~31) ? lo & ~31 : (int)from;
     k1 = last || hi < to ? hi : (int)to;
+    return true;
+}
+
+// The same of a launch with first tokens: split 0 has them too, the keys [0, extra) of the rows, before those of its range,
+// which may be empty then.
+template <typename Args>
+IQ4XS_BOTH inline bool split_keys_more(const Args& a, const Sequence& s, int lo, int hi, int split, int& k0, int& k1,
+                                       int& extra) {
+    extra = a.pass == PASS_SINKS && split == 0 ? (s.skip < hi ? s.skip : hi) : 0;
+    if (!split_keys(a, s, lo, hi, split, k0, k1)) {
+        if (extra <= 0) return false;
+        k0 = k1 = 0;
+    }
+    if (extra < 0) extra = 0;
+    if (k1 < k0) k1 = k0;
     return true;
 }
 
@@ -96,6 +189,67 @@ IQ4XS_BOTH inline RowEnd row_end(const Args& a, const Sequence& s, int lo, int h
     return a.splits == 1 || split_of(a, s, lo) == split ? ROW_OUT : ROW_NONE;
 }
 
+// The same of a launch with first tokens.  A row that sees some sees key 0, in split 0, whatever its range; the parts of a
+// shared prefix's launches are always joined.
+template <typename Args>
+IQ4XS_BOTH inline bool one_split_more(const Args& a, const Sequence& s, int lo, int hi) {
+    if (a.pass != PASS_SINKS) return false;
+    if (a.splits == 1) return true;
+    if (hi <= lo) return hi > 0 && s.skip > 0;
+    return split_of(a, s, lo) == split_of(a, s, hi - 1) && (s.skip == 0 || split_of(a, s, lo) == 0);
+}
+template <typename Args>
+IQ4XS_BOTH inline RowEnd row_end_more(const Args& a, const Sequence& s, int lo, int hi, int split) {
+    if (!one_split_more(a, s, lo, hi)) return ROW_PART;
+    return a.splits == 1 || (hi > lo ? split_of(a, s, lo) : 0) == split ? ROW_OUT : ROW_NONE;
+}
+
+// Where the parts of a row lie that are joined: `before` of them from 0 on, `after` from `from` on.
+struct RowParts {
+    int before, from, after;
+    IQ4XS_BOTH int count() const { return before + after; }
+    IQ4XS_BOTH int at(int i) const { return i < before ? i : from + i - before; }
+};
+template <typename Args>
+IQ4XS_BOTH inline RowParts row_parts(const Args& a, const Sequence& s, int lo, int hi) {
+    int first, last;
+    splits_of(a, s, lo, hi, first, last);
+    if (hi <= lo) first = last + 1;
+    if (a.pass == PASS_SINKS) {
+        const int before = hi > 0 && s.skip > 0 && (first > 0 || hi <= lo);
+        return {before, first, last - first + 1};
+    }
+    // s.skip: the shared tokens, as far as the sequence reaches; the prefix's parts lie before the others
+    return {0, a.prefix_splits + first, last - first + 1};
+}
+// The parts of the prefix, of a group that shares `keys` tokens.
+template <typename Args>
+IQ4XS_BOTH inline int prefix_parts(const Args& a, int keys) {
+    if (keys <= 0) return 0;
+    const int last = (keys - 1) / a.prefix_chunk;
+    return (last < a.prefix_splits ? last : a.prefix_splits - 1) + 1;
+}
+
+// The keys that a workgroup goes through, KEYS at a time: [k0, k1), and before them as many steps as the first tokens
+// [0, extra) take.  Steps are at `base` from start on; those before k0 are of first tokens.
+template <int KEYS, bool MORE>
+struct KeySteps {
+    int k0, k1, extra, start;
+    IQ4XS_BOTH KeySteps(int k0, int k1, int extra)
+        : k0(k0), k1(k1), extra(extra), start(MORE ? k0 - (extra + KEYS - 1) / KEYS * KEYS : k0) {}
+    IQ4XS_BOTH bool is_first(int base) const { return MORE && base < k0; }
+    IQ4XS_BOTH int place(int base) const { return is_first(base) ? base - start : base; }  // first key of the step
+    IQ4XS_BOTH int stop(int base) const { return is_first(base) ? extra : k1; }             // where its keys end
+    // whether rows that all see [lo, hi) see the whole step
+    IQ4XS_BOTH bool all_see(int base, int lo, int hi) const {
+        if (is_first(base)) return place(base) + KEYS <= (extra < hi ? extra : hi);
+        return base >= lo && base + KEYS <= hi;
+    }
+    // of a row that sees [lo, hi): what it sees of the step's kind
+    IQ4XS_BOTH int lo_in(int base, int lo) const { return is_first(base) ? 0 : lo; }
+    IQ4XS_BOTH int hi_in(int base, int hi) const { return is_first(base) && extra < hi ? extra : hi; }
+};
+
 // What a call launches.
 struct AttentionPlan {
     int tiles;      // 16-row tiles of a workgroup that streams the cache, or 0: the kernel of many rows
@@ -113,9 +267,7 @@ inline int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
 inline int64_t window_of(const iq4xs_paged_attention_args& g) { return g.window < 0x7FFFFFFF ? g.window : 0; }
 
 // Keys of a sequence that count: their places, and those of a few steps past the end, are ints in the kernels.
-inline int most_kv_of(const iq4xs_paged_attention_args& g) {
-    return (int)at_most(g.most_kv, ((int64_t)1 << 31) - 4096);
-}
+inline int most_kv_of(const iq4xs_paged_attention_args& g) { return (int)at_most(g.most_kv, KEYS_END); }
 
 inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     const int64_t group = g.q_heads / g.cache->heads, most_q = g.most_q < g.total ? g.most_q : g.total;
@@ -180,8 +332,34 @@ inline bool plan_fits(const iq4xs_paged_attention_args& g, int64_t cus, Attentio
     return p.grid <= MOST;
 }
 
-inline size_t part_bytes(const iq4xs_paged_attention_args& g, int splits) {
-    return splits > 1 ? (size_t)splits * g.total * g.q_heads * g.cache->head_dim * sizeof(float) : 0;
+// Sums of `splits` splits for every row and head.
+inline size_t parts_bytes(const iq4xs_paged_attention_args& g, int splits) {
+    return (size_t)splits * g.total * g.q_heads * g.cache->head_dim * sizeof(float);
+}
+
+// Whether first tokens are more than the window shows: a window as long as the longest sequence hides none.
+inline bool sinks_matter(const iq4xs_paged_attention_args& g, int64_t sinks) {
+    return sinks > 0 && window_of(g) > 0 && window_of(g) < g.most_kv;
+}
+
+// The launch over the prefixes of a call as one over groups: their rows all see all of it.
+inline iq4xs_paged_attention_args prefix_call(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x) {
+    iq4xs_paged_attention_args p = g;
+    p.seqs = x.groups;
+    p.most_q = x.most_rows;
+    p.most_kv = x.most_len;
+    p.causal = 0;
+    return p;
+}
+
+struct SharedPlan {
+    AttentionPlan prefix, own;
+    int splits() const { return prefix.splits + own.splits; }
+};
+
+inline bool shared_plan_fits(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x, int64_t cus,
+                             SharedPlan& p) {
+    return plan_fits(prefix_call(g, x), cus, p.prefix) && plan_fits(g, cus, p.own);
 }
 
 }  // namespace iq4xs

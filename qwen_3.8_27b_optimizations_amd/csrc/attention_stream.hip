@@ -295,8 +295,9 @@ __device__ inline u4 slots_in(int base, int j, int lo, int hi) {
     return m;
 }
 
-template <int D, typename Q, typename KV, int NT>
-__global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_attention_kernel(AttentionArgs a) {
+template <int D, typename Q, typename KV, int NT, typename Args>
+__global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_attention_kernel(Args a) {
+    constexpr bool MORE = HasMore<Args>::value;
     constexpr int OWN = D / 16, PART = D == 64 ? 64 : 128;
     using W = typename Step<D, KV>::Weight;
     constexpr uint32_t ONES = Matrix<W>::ONES;
@@ -313,7 +314,11 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     x /= a.seqs;
     const int tile = x % a.row_tiles, split = x / a.row_tiles;
     int total_fresh;
-    const Sequence s = sequence(a, seq, total_fresh);
+    Sequence s;
+    if constexpr (MORE)
+        s = sequence_more(a, seq, total_fresh);
+    else
+        s = sequence(a, seq, total_fresh);
     const int rows = s.fresh * a.group, row0 = tile * 16 * NT;
     if (row0 >= rows) return;
     const int last = (rows < row0 + 16 * NT ? rows : row0 + 16 * NT) - 1;
@@ -321,8 +326,14 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     // keys that some row of the tile sees, and those that all see
     const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
     const int all_lo = least_key(a, s, total_fresh, token1), all_hi = end_key(a, s, total_fresh, token0);
-    int k0, k1;
-    if (!split_keys(a, s, any_lo, any_hi, split, k0, k1)) return;
+    int k0, k1, extra = 0;
+    if constexpr (MORE) {
+        if (!split_keys_more(a, s, any_lo, any_hi, split, k0, k1, extra)) return;
+    } else {
+        if (!split_keys(a, s, any_lo, any_hi, split, k0, k1)) return;
+    }
+    const KeySteps<STEP_KEYS, MORE> span(k0, k1, extra);
+    const int start = span.start;
 
     // this lane's rows and their keys (lanes without a row repeat the last)
     int token[NT], lo[NT], hi[NT];
@@ -380,22 +391,22 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     // Its pages are looked up a step before they are wanted, tile t's in lane t: a load without a condition, issued ahead of
     // the step's keys, so that waiting for it is not waiting for them.
     auto look_up = [&](int base) {
-        const int key = base + 16 * (lane % 2);
-        const int32_t* p = key < k1 ? s.pages + (key >> a.c.shift) : a.starts;
+        const int key = span.place(base) + 16 * (lane % 2);
+        const int32_t* p = key < span.stop(base) ? s.pages + (key >> a.c.shift) : a.starts;
         return *p;
     };
     auto find = [&](int base, int pages, int64_t(&row)[2], bool(&there)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key = base + 16 * t, page = __builtin_amdgcn_readlane(pages, t);
-            there[t] = key < k1 && page >= 0 && page < a.c.pages;
+            const int key = span.place(base) + 16 * t, page = __builtin_amdgcn_readlane(pages, t);
+            there[t] = key < span.stop(base) && page >= 0 && page < a.c.pages;
             row[t] = page_row(a.c, there[t] ? page : 0, head, there[t] ? key & ((1 << a.c.shift) - 1) : 0);
         }
     };
 
     // the lane's slots of a step whose keys some row sees
     auto seen = [&](int base, const bool(&there)[2]) {
-        u4 some = slots_in(base, j, any_lo, any_hi);
+        u4 some = slots_in(span.place(base), j, span.lo_in(base, any_lo), span.hi_in(base, any_hi));
         if (!there[0]) some.x = some.y = 0;
         if (!there[1]) some.z = some.w = 0;
         return some;
@@ -409,7 +420,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     }
     int64_t row[2];
     bool there[2];
-    int base = k0 + STEP_KEYS * wave, pages = 0;
+    int base = start + STEP_KEYS * wave, pages = 0;
     if (base < k1) {
         const int first = look_up(base);
         pages = look_up(base + STEP_KEYS * STREAM_WAVES);
@@ -446,12 +457,13 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
 #pragma unroll
             for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(z[i][0]), "+v"(z[i][1]));
         }
-        const bool full = finite && there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi;
+        const bool full = finite && there[0] && there[1] && span.all_see(base, all_lo, all_hi);
         u4 w[NT], w_rest[EXACT ? NT : 1];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float top = -INFINITY;
-            const int from = lo[i] - base - 4 * j, to = hi[i] - base - 4 * j;
+            const int at0 = span.place(base) + 4 * j;
+            const int from = span.lo_in(base, lo[i]) - at0, to = span.hi_in(base, hi[i]) - at0;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -510,7 +522,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     if (__builtin_expect(__any(odd), 0)) {
         if constexpr (EXACT) {
             // values of large scales come with the weights as they are now, and may be infinities too: those after them
-            for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
+            for (base = start + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
                 find(base, look_up(base), row, there);
                 step.load_keys(a, row, n, j);
                 step.share_scales(lane);
@@ -520,7 +532,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 step.scores(queries, z, lane);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    u4 sees = slots_in(base, j, lo[i], hi[i]);
+                    u4 sees = slots_in(span.place(base), j, span.lo_in(base, lo[i]), span.hi_in(base, hi[i]));
                     if (!there[0]) sees.x = sees.y = 0;
                     if (!there[1]) sees.z = sees.w = 0;
 #pragma unroll
@@ -553,9 +565,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
             }
         }
         // values that are not finite reach the rows that see them as infinities (a NaN as both)
-        for (base = k0 + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
+        for (base = start + STEP_KEYS * wave; base < k1; base += STEP_KEYS * STREAM_WAVES) {
             find(base, look_up(base), row, there);
-            if (!EXACT && there[0] && there[1] && base >= all_lo && base + STEP_KEYS <= all_hi) continue;
+            if (!EXACT && there[0] && there[1] && span.all_see(base, all_lo, all_hi)) continue;
             step.load_keys(a, row, n, j);
             step.load_values(a, row, n, j);
             step.share_scales(lane);
@@ -565,7 +577,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 const u4 x = step.values(t) & seen(base, there);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const u4 sees = slots_in(base, j, lo[i], hi[i]) & ONES;
+                    const u4 sees = slots_in(span.place(base), j, span.lo_in(base, lo[i]), span.hi_in(base, hi[i])) & ONES;
                     const f4 plus = Matrix<W>::mma16(Matrix<W>::above(x), sees, f4{0, 0, 0, 0});
                     const f4 minus = Matrix<W>::mma16(Matrix<W>::below(x), sees, f4{0, 0, 0, 0});
 #pragma unroll
@@ -624,7 +636,12 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
                 }
                 const int tok = r / a.group, h = head * a.group + r % a.group;
                 const int64_t out = (int64_t)(s.first + tok) * a.q_heads + h;
-                const RowEnd end = row_end(a, s, least_key(a, s, total_fresh, tok), end_key(a, s, total_fresh, tok), split);
+                const int row_lo = least_key(a, s, total_fresh, tok), row_hi = end_key(a, s, total_fresh, tok);
+                RowEnd end;
+                if constexpr (MORE)
+                    end = row_end_more(a, s, row_lo, row_hi, split);
+                else
+                    end = row_end(a, s, row_lo, row_hi, split);
                 if (end == ROW_OUT) {
                     store4(a.out, out * D + PART * part + c, a.out_type, sum == 0.0f ? f4{0, 0, 0, 0} : v / weights);
                     if (a.lse && part == 0 && c == 0)
@@ -639,30 +656,31 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, D == 256 ? 1 : 2) void stream_at
     }
 }
 
-template <int D, int NT>
-void launch_types(const AttentionArgs& a, int type, int cache_type, dim3 grid, hipStream_t stream) {
+template <int D, int NT, typename Args>
+void launch_types(const Args& a, int type, int cache_type, dim3 grid, hipStream_t stream) {
     const dim3 block(64 * STREAM_WAVES);
     if (cache_type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, _Float16, NT>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, _Float16, NT, Args>), grid, block, 0, stream, a);
     else if (cache_type == IQ4XS_TYPE_BF16)
-        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, __bf16, NT>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, __bf16, NT, Args>), grid, block, 0, stream, a);
     else if constexpr (D == 256 && NT == 2)
         return;  // not asked for: two tiles of codes do not fit the registers
     else if (type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, int8_t, NT>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((stream_attention_kernel<D, _Float16, int8_t, NT, Args>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, int8_t, NT>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((stream_attention_kernel<D, __bf16, int8_t, NT, Args>), grid, block, 0, stream, a);
 }
 
-template <int D>
-void launch_tiles(const AttentionArgs& a, int tiles, int type, int cache_type, dim3 grid, hipStream_t stream) {
+template <int D, typename Args>
+void launch_tiles(const Args& a, int tiles, int type, int cache_type, dim3 grid, hipStream_t stream) {
     if (tiles == 1)
         launch_types<D, 1>(a, type, cache_type, grid, stream);
     else
         launch_types<D, 2>(a, type, cache_type, grid, stream);
 }
 
-void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
+template <typename Args>
+void launch_stream_attention(const Args& a, int head_dim, int tiles, int type, int cache_type, int64_t grid,
                              hipStream_t stream) {
     const dim3 blocks((unsigned)grid);
     if (head_dim == 64)
@@ -672,5 +690,10 @@ void launch_stream_attention(const AttentionArgs& a, int head_dim, int tiles, in
     else
         launch_tiles<256>(a, tiles, type, cache_type, blocks, stream);
 }
+#ifdef IQ4XS_ATTENTION_MORE
+template void launch_stream_attention(const MoreArgs&, int, int, int, int, int64_t, hipStream_t);
+#else
+template void launch_stream_attention(const AttentionArgs&, int, int, int, int, int64_t, hipStream_t);
+#endif
 
 }  // namespace iq4xs

@@ -93,8 +93,9 @@ __device__ inline u4 codes_to_f16(u2 w, _Float16 scale) {
     return x;
 }
 
-template <int D, typename Q, typename KV, bool EXACT>
-__global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attention_kernel(AttentionArgs a) {
+template <int D, typename Q, typename KV, bool EXACT, typename Args>
+__global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attention_kernel(Args a) {
+    constexpr bool MORE = HasMore<Args>::value;
     using T = Tile<D>;
     constexpr bool CODES = sizeof(KV) == 1;
     using W = typename std::conditional<CODES, _Float16, KV>::type;
@@ -113,7 +114,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // the last rows see the most keys: first
     const int tile = a.row_tiles - 1 - x % a.row_tiles, split = x / a.row_tiles;
     int total_fresh;
-    const Sequence s = sequence(a, seq, total_fresh);
+    Sequence s;
+    if constexpr (MORE)
+        s = sequence_more(a, seq, total_fresh);
+    else
+        s = sequence(a, seq, total_fresh);
     const int rows = s.fresh * a.group, row0 = tile * TILE_ROWS;
     if (row0 >= rows) return;
     const int last = (rows < row0 + TILE_ROWS ? rows : row0 + TILE_ROWS) - 1;
@@ -121,8 +126,14 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // keys that some row sees, and those that all see
     const int any_lo = least_key(a, s, total_fresh, token0), any_hi = end_key(a, s, total_fresh, token1);
     const int all_lo = least_key(a, s, total_fresh, token1), all_hi = end_key(a, s, total_fresh, token0);
-    int k0, k1;
-    if (!split_keys(a, s, any_lo, any_hi, split, k0, k1)) return;
+    int k0, k1, extra = 0;
+    if constexpr (MORE) {
+        if (!split_keys_more(a, s, any_lo, any_hi, split, k0, k1, extra)) return;
+    } else {
+        if (!split_keys(a, s, any_lo, any_hi, split, k0, k1)) return;
+    }
+    const KeySteps<T::KEYS, MORE> span(k0, k1, extra);
+    const int start = span.start;
 
     // this lane's row (lanes without one repeat the last)
     const int wave0 = row0 + 32 * wave;
@@ -168,17 +179,17 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // 16384 keys: 1116 us, and 1032 so).
     int looked_up;
     auto look_up = [&](int base) {
-        const int key = base + 16 * (lane % PARTS);
-        const int32_t* p = key < k1 ? s.pages + (key >> a.c.shift) : a.starts;
+        const int key = span.place(base) + 16 * (lane % PARTS);
+        const int32_t* p = key < span.stop(base) ? s.pages + (key >> a.c.shift) : a.starts;
         looked_up = *p;
     };
     // of the tile at `base`, which was looked up: which 16 keys are not there, and where this wave's rows begin
     auto locate = [&](int base, uint32_t& lacking) {
-        const bool held = base + 16 * (lane % PARTS) < k1 && looked_up >= 0 && looked_up < a.c.pages;
+        const bool held = span.place(base) + 16 * (lane % PARTS) < span.stop(base) && looked_up >= 0 && looked_up < a.c.pages;
         lacking = ~(uint32_t)__ballot(held) & ((1u << PARTS) - 1);
         const int page = __builtin_amdgcn_readlane(looked_up, wave);
         const bool there = !(lacking >> wave & 1);
-        return page_row(a.c, there ? page : 0, head, there ? (base + bring) & ((1 << a.c.shift) - 1) : 0);
+        return page_row(a.c, there ? page : 0, head, there ? (span.place(base) + bring) & ((1 << a.c.shift) - 1) : 0);
     };
     // rows of one side (0 keys, 1 values) on their way to a buffer; of an 8-bit cache into registers, from which `put`
     // takes them
@@ -240,10 +251,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
                 } else {
                     u4 v = codes_to_f16<true>(c, by);
                     if (__builtin_expect(large, 0)) {
-                        const int rr = bring + i * T::ROWS + in_load, key = base + rr;
+                        const int rr = bring + i * T::ROWS + in_load, key = span.place(base) + rr;
                         const u4 f = M::finite(v), x = v ^ f;
-                        odd |= key >= any_lo && key < any_hi && !(missing >> (rr / 16) & 1) &&
-                               (x.x | x.y | x.z | x.w) != 0;
+                        odd |= key >= span.lo_in(base, any_lo) && key < span.hi_in(base, any_hi) &&
+                               !(missing >> (rr / 16) & 1) && (x.x | x.y | x.z | x.w) != 0;
                         v = f;
                     }
                     *to = v;
@@ -255,9 +266,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     // the values of a tile once more, what no row sees cleared
     auto again = [&](int base, int buffer, uint32_t missing) {
         for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
-            const int rr = i / T::PIECES, p = i % T::PIECES, key = base + rr;
+            const int rr = i / T::PIECES, p = i % T::PIECES, key = span.place(base) + rr;
             u4 v{0, 0, 0, 0};
-            if (key >= any_lo && key < any_hi && !(missing >> (rr / 16) & 1)) {
+            if (key >= span.lo_in(base, any_lo) && key < span.hi_in(base, any_hi) && !(missing >> (rr / 16) & 1)) {
                 const int64_t row = page_row(a.c, s.pages[key >> a.c.shift], head, key & ((1 << a.c.shift) - 1));
                 if constexpr (CODES)
                     v = codes_to_f16<true>(*reinterpret_cast<const u2*>(static_cast<const int8_t*>(a.c.v) + row * D + 8 * p),
@@ -285,11 +296,12 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         return u4{x0.x, x0.y, x1.x, x1.y};
     };
 
-    // `z` are scores of 32 keys at `base`: hidden ones go, the running maximum moves if it must, and with it the sums and
-    // the weights `w` still to be used.
-    auto raise = [&](fx16& z, int base, uint32_t lacking, bool edge, u4(&w)[2]) {
+    // `z` are scores of 32 keys, `in_tile` into the tile at `base`: hidden ones go, the running maximum moves if it must, and
+    // with it the sums and the weights `w` still to be used.
+    auto raise = [&](fx16& z, int base, int in_tile, uint32_t lacking, bool edge, u4(&w)[2]) {
         if (__builtin_expect(edge, 0)) {
-            const int from = lo - base - 4 * half, to = hi - base - 4 * half;
+            const int at0 = span.place(base) + in_tile + 4 * half;
+            const int from = span.lo_in(base, lo) - at0, to = span.hi_in(base, hi) - at0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int in = 8 * (i / 4) + i % 4;
@@ -367,9 +379,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     auto clear = [&](int base, int buffer, uint32_t missing) {
         uint32_t some = 0;
         for (int i = threadIdx.x; i < T::KEYS * T::PIECES; i += 64 * TILE_WAVES) {
-            const int key = base + i / T::PIECES;
+            const int key = span.place(base) + i / T::PIECES;
             u4* p = reinterpret_cast<u4*>(&lds[buffer][1][16 * i]);
-            const bool seen = key >= any_lo && key < any_hi && !(missing >> (i / T::PIECES / 16) & 1);
+            const bool seen = key >= span.lo_in(base, any_lo) && key < span.hi_in(base, any_hi) &&
+                              !(missing >> (i / T::PIECES / 16) & 1);
             const u4 v = *p, f = seen ? M::finite(v) : u4{0, 0, 0, 0}, x = v ^ f;
             some |= seen ? x.x | x.y | x.z | x.w : 0u;
             *p = f;
@@ -381,19 +394,19 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         // A tile's 32 keys in turn: their scores, weights and product with the values; the next tile's codes are on their
         // way meanwhile.
         uint32_t lacking;
-        look_up(k0);
-        int64_t row = locate(k0, lacking);
+        look_up(start);
+        int64_t row = locate(start, lacking);
         fetch(0, row, 0);
         if (IN_TURN) put(0, 0);
         fetch(1, row, 0);
         if (!IN_TURN) put(0, 0);
-        put(1, 0, k0, lacking);
-        look_up(k0 + T::KEYS);
+        put(1, 0, start, lacking);
+        look_up(start + T::KEYS);
         int buffer = 0;
-        for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+        for (int base = start; base < k1; base += T::KEYS, buffer ^= 1) {
             asm volatile("" : "+v"(looked_up));
             __syncthreads();
-            const bool edge = lacking != 0 || base < all_lo || base + T::KEYS > all_hi, more = base + T::KEYS < k1;
+            const bool edge = lacking != 0 || !span.all_see(base, all_lo, all_hi), more = base + T::KEYS < k1;
             if (__builtin_expect(edge, 0)) clear(base, buffer, lacking);
             const uint32_t was_lacking = lacking;
             if (more) {
@@ -422,7 +435,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
                     for (int i = 0; i < 16; ++i) z[i] = __builtin_fmaf(part[i], (float)(i < 8 ? s0[i] : s1[i - 8]), z[i]);
                 }
                 u4 w[2] = {}, rest[2];
-                raise(z, base + 32 * s, was_lacking >> 2 * s, edge, w);
+                raise(z, base, 32 * s, was_lacking >> 2 * s, edge, w);
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], factor, -m));
@@ -458,14 +471,14 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
         // own beside the product of the weights before it: keys are wanted a tile ahead of values.  The barrier of tile T
         // comes before step 2 T + 1: keys of tile T and values of tile T - 1 are done with, those of T + 1 and T are there.
         uint32_t lacking, next_lacking = (1u << PARTS) - 1;
-        look_up(k0);
-        int64_t row = locate(k0, lacking);
+        look_up(start);
+        int64_t row = locate(start, lacking);
         fetch(0, row, 0);
         if (IN_TURN) put(0, 0);
         fetch(1, row, 0);
         if (!IN_TURN) put(0, 0);
         put(1, 0);
-        look_up(k0 + T::KEYS);
+        look_up(start + T::KEYS);
         wait_for_copies();
         __syncthreads();
         fx16 even, uneven;
@@ -477,22 +490,22 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             even = M::mma32(key_piece(key_at, c, 0), q[c], even);
             uneven = M::mma32(key_piece(key_at, c, 32 * T::ROW), q[c], uneven);
         }
-        bool edge = lacking != 0 || k0 < all_lo || k0 + T::KEYS > all_hi;
-        raise(even, k0, lacking, edge, w_even);
+        bool edge = lacking != 0 || !span.all_see(start, all_lo, all_hi);
+        raise(even, start, 0, lacking, edge, w_even);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) weigh(even, i, w_even);
-        if (k0 + T::KEYS < k1) {
-            row = locate(k0 + T::KEYS, next_lacking);
+        if (start + T::KEYS < k1) {
+            row = locate(start + T::KEYS, next_lacking);
             fetch(0, row, 1);
             put(0, 1);
-            look_up(k0 + 2 * T::KEYS);
+            look_up(start + 2 * T::KEYS);
         }
         if constexpr (D == 256) {  // with the sums, where the products read them and nothing else does
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) asm volatile("" : "+a"(q[c]));
         }
         int buffer = 0;
-        for (int base = k0; base < k1; base += T::KEYS, buffer ^= 1) {
+        for (int base = start; base < k1; base += T::KEYS, buffer ^= 1) {
             wait_for_copies();
             asm volatile("" : "+v"(looked_up));  // there now, as far as the compiler's own waits go
             __syncthreads();
@@ -510,14 +523,14 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
             const uint32_t here = buffer * 2 * T::BYTES, there = 2 * T::BYTES - here;
             u4 f[AHEAD];
             begin(key_at + there, value_at + here, f);
-            raise(uneven, base + 32, was_lacking >> 2, edge, w_even);
+            raise(uneven, base, 32, was_lacking >> 2, edge, w_even);
             step(key_at + there, value_at + here, f, even, uneven, w_even, w_odd);
             if (IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
             if (IN_TURN && base + 2 * T::KEYS < k1) fetch(0, row, buffer);
             // past the last tile these are scores of whatever lies in LDS, all masked
-            edge = lacking != 0 || base + T::KEYS < all_lo || base + 2 * T::KEYS > all_hi;
+            edge = lacking != 0 || !span.all_see(base + T::KEYS, all_lo, all_hi);
             begin(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f);
-            raise(even, base + T::KEYS, lacking, edge, w_odd);
+            raise(even, base + T::KEYS, 0, lacking, edge, w_odd);
             step(key_at + there + 32 * T::ROW, value_at + here + 32 * T::ROW, f, uneven, even, w_odd, w_even);
 
             if (!IN_TURN && base + T::KEYS < k1) put(1, buffer ^ 1);
@@ -529,11 +542,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     if (__builtin_expect(odd != 0, 0)) {
         // the values that are not finite reach the rows that see them as infinities (a NaN as both)
         wait_for_copies();
-        for (int base = k0; base < k1; base += T::KEYS) {
+        for (int base = start; base < k1; base += T::KEYS) {
             look_up(base);
             uint32_t out;
             locate(base, out);
-            if (!EXACT && out == 0 && base >= all_lo && base + T::KEYS <= all_hi) continue;
+            if (!EXACT && out == 0 && span.all_see(base, all_lo, all_hi)) continue;
             __syncthreads();
             again(base, 0, out);
             __syncthreads();
@@ -543,7 +556,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
 #pragma unroll
                 for (int i = 0; i < 16; ++i) plus[i] = minus[i] = 0.0f;
                 for (int k = 0; k < T::KEYS / 16; ++k) {
-                    const int first = lo - base - 16 * k - 4 * half, end = hi - base - 16 * k - 4 * half;
+                    const int at0 = span.place(base) + 16 * k + 4 * half, first = span.lo_in(base, lo) - at0,
+                              end = span.hi_in(base, hi) - at0;
                     u4 sees;
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
@@ -568,7 +582,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     l = sum_of_halves(l);
     rounded = EXACT ? l : sum_of_halves(rounded);
     const int64_t out = (int64_t)(s.first + token) * a.q_heads + query_head;
-    const RowEnd end = row_end(a, s, lo, hi, split);
+    RowEnd end;
+    if constexpr (MORE)
+        end = row_end_more(a, s, lo, hi, split);
+    else
+        end = row_end(a, s, lo, hi, split);
     if (end == ROW_OUT) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / rounded;
 #pragma unroll
@@ -591,24 +609,25 @@ __global__ __launch_bounds__(64 * TILE_WAVES, D == 256 ? 1 : 2) void tile_attent
     }
 }
 
-template <int D>
-void launch_types(const AttentionArgs& a, int type, int cache_type, bool exact, dim3 grid, hipStream_t stream) {
+template <int D, typename Args>
+void launch_types(const Args& a, int type, int cache_type, bool exact, dim3 grid, hipStream_t stream) {
     const dim3 block(64 * TILE_WAVES);
     if (cache_type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, _Float16, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, _Float16, false, Args>), grid, block, 0, stream, a);
     else if (cache_type == IQ4XS_TYPE_BF16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, __bf16, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, __bf16, false, Args>), grid, block, 0, stream, a);
     else if (type == IQ4XS_TYPE_F16 && exact)
-        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, true>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, true, Args>), grid, block, 0, stream, a);
     else if (type == IQ4XS_TYPE_F16)
-        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, _Float16, int8_t, false, Args>), grid, block, 0, stream, a);
     else if (exact)
-        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, true>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, true, Args>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((tile_attention_kernel<D, __bf16, int8_t, false, Args>), grid, block, 0, stream, a);
 }
 
-void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
+template <typename Args>
+void launch_tile_attention(const Args& a, int head_dim, int type, int cache_type, bool exact, int64_t grid,
                            hipStream_t stream) {
     const dim3 blocks((unsigned)grid);
     if (head_dim == 64)
@@ -618,5 +637,10 @@ void launch_tile_attention(const AttentionArgs& a, int head_dim, int type, int c
     else
         launch_types<256>(a, type, cache_type, exact, blocks, stream);
 }
+#ifdef IQ4XS_ATTENTION_MORE
+template void launch_tile_attention(const MoreArgs&, int, int, int, bool, int64_t, hipStream_t);
+#else
+template void launch_tile_attention(const AttentionArgs&, int, int, int, bool, int64_t, hipStream_t);
+#endif
 
 }  // namespace iq4xs
