@@ -466,6 +466,49 @@ size_t iq4xs_shared_attention_workspace_bytes(const struct iq4xs_paged_attention
 int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const struct iq4xs_shared_prefix* prefix,
                            void* ws, size_t ws_bytes, void* stream);
 
+/* ================= layers that keep a state in place of a cache =================
+ * Linear attention with a decay for each head.  The same conventions as above. */
+
+struct iq4xs_linear_attention_args {
+    const void* q;      /* [total][qk_heads][dk], in_type */
+    const void* k;      /* as q */
+    const void* v;      /* [total][heads][dv], in_type */
+    const float* decay; /* natural logarithms: [heads] (decay_stride 0) or [total][heads] */
+    const int32_t* starts;     /* [seqs + 1] first row of each sequence, never falling, the last at most total */
+    float* states;             /* [slots][heads][dk][dv], or NULL */
+    const int64_t* from_slots; /* [seqs] states that sequences go on from, or NULL: all begin at zeros */
+    const int64_t* to_slots;   /* [seqs] where their states are left, or NULL: nowhere */
+    void* out;                 /* [total][heads][dv], out_type; not the memory of an input */
+    int64_t q_stride, k_stride, v_stride, decay_stride; /* of a token, in elements */
+    int64_t slots, seqs, total;
+    int64_t most_q; /* at least the tokens of any sequence */
+    int32_t heads;  /* a multiple of qk_heads: head h reads q and k of head h / (heads / qk_heads) */
+    int32_t qk_heads;
+    int32_t dk, dv; /* 64, 128 or 256 each (NOT_SUPPORTED otherwise) */
+    int32_t in_type, out_type;
+    float scale;
+};
+
+/* Bytes of workspace iq4xs_linear_attention needs; 0 also for arguments it refuses
+ * (IQ4XS_ERROR_INVALID_CONFIG: launches of more than 2^31 - 1 workgroups). */
+size_t iq4xs_linear_attention_workspace_bytes(const struct iq4xs_linear_attention_args* args);
+
+/* Token by token, for each head, from S_0 = the state at from_slots (zeros where the
+ * slot is negative or past the states):
+ *   S_t = exp(decay_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t,
+ * and the last S_t goes to to_slots (nowhere where that slot is negative or past the
+ * states).  A sequence of no tokens leaves its states as they are.  States and sums are
+ * fp32; products of many tokens go through matrix units as sums of 16-bit parts that
+ * keep 24 bits of states, updates and fp32 inputs (16 of what makes 16-bit outputs).
+ * Two sequences must not have one to_slot, nor one's to_slot be another's from_slot;
+ * a sequence's own two may be one, and several may begin at one state.
+ * A sequence of more than most_q tokens is cut to its first most_q; rows past them and
+ * those of no sequence are not written.  What is not finite in a token reaches the
+ * outputs and states of its head from that token on (of v, its channel's), as infinities
+ * or NaN, and nothing else.  Decays are taken as -200 at least, exp of which is nothing
+ * beside any fp32 number.  The same call gives the same bits. */
+int iq4xs_linear_attention(const struct iq4xs_linear_attention_args* args, void* ws, size_t ws_bytes, void* stream);
+
 /* ================================ debug exports ================================
  * No counterpart in the reference; they exist so the Q8_1 blocks and the
  * per-32-element int32 sums can be checked bit for bit. */

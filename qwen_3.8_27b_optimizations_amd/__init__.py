@@ -91,6 +91,8 @@ SIGNATURES = {
     "iq4xs_paged_attention_sinks": (_INT, [_P, _I64, _P, ctypes.c_size_t, _P]),
     "iq4xs_shared_attention_workspace_bytes": (ctypes.c_size_t, [_P, _P]),
     "iq4xs_shared_attention": (_INT, [_P, _P, _P, ctypes.c_size_t, _P]),
+    "iq4xs_linear_attention_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "iq4xs_linear_attention": (_INT, [_P, _P, ctypes.c_size_t, _P]),
     "iq4xs_q8_1_to_blocks": (_INT, [_P, _P, _I64, _I64, _P]),
     "iq4xs_subblock_sums": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _INT, _P]),
     "iq4xs_probe_mfma_i8": (_INT, [_P, _P, _P, _P]),
@@ -335,6 +337,7 @@ _CACHE = struct.Struct("@PPPPqiiii")
 _QK = struct.Struct("@PPPqqqPPPPPPPqiiiiiiif")
 _ATTENTION = struct.Struct("@PPPPPPPqqqqqqqiiiif")
 _SHARED = struct.Struct("@PPqqq")
+_LINEAR = struct.Struct("@PPPPPPPPPqqqqqqqqiiiiiif")
 
 
 _TYPES = {}  # torch dtype -> TYPE_*, filled once a GPU has been seen
@@ -565,6 +568,53 @@ def shared_attention(q, cache, table, starts, kv_len, shared_len, most_q: int, m
     L.check("iq4xs_shared_attention", args, prefix, ws.data_ptr() if nbytes else 0, nbytes,
             torch._C._cuda_getCurrentRawStream(here))
     return (out, sums) if lse else out
+
+
+def linear_attention(q, k, v, decay, starts, most_q: int, states=None, from_slots=None, to_slots=None, scale: float = 1.0,
+                     out_type=None):
+    """Linear attention with a decay for each head, token by token of each sequence: S = exp(decay) S + k v^T, out = scale
+    q^T S, for q and k [total, qk_heads, dk] and v [total, heads, dv] (heads a multiple of qk_heads, dk and dv 64, 128 or
+    256, one type: float32, float16 or bfloat16).
+
+    decay (float32, natural logarithms): [heads], or [total, heads] for decays of each token.  starts [seqs + 1] (int32):
+    first row of each sequence; most_q: at least the tokens of any.  states [slots, heads, dk, dv] (float32) are read at
+    from_slots [seqs] (int64; None, negative or past the states: zeros) and written, in place, at to_slots (None, negative
+    or past the states: not kept); two sequences must not write one slot, nor one what another reads.  Returns out [total,
+    heads, dv] in out_type (default: v's); rows of no sequence are left as they were allocated."""
+    torch = _torch()
+    here = _here(torch, q)
+    types = _types(torch)
+    kind = q.dtype
+    out_type = kind if out_type is None else out_type
+    if kind not in types or out_type not in types or k.dtype != kind or v.dtype != kind:
+        raise ValueError("q, k and v must have one type and out_type be one: float32, float16 or bfloat16")
+    total, hk, dk, q_stride = _rows(q, "q")
+    kt, kh, kd, k_stride = _rows(k, "k")
+    vt, heads, dv, v_stride = _rows(v, "v")
+    if (kt, kh, kd) != (total, hk, dk) or vt != total or k.get_device() != here or v.get_device() != here:
+        raise ValueError("q, k and v must hold the same tokens, q and k the same heads, on the current GPU")
+    if hk == 0 or heads % hk:
+        raise ValueError("v's heads must be a multiple of q's")
+    each = decay.dim() == 2
+    dp = _whole(decay, "decay", torch.float32, (total, heads) if each else (heads,), here)
+    seqs = starts.numel() - 1
+    sp = _whole(starts, "starts", torch.int32, (seqs + 1,), here)
+    slots = 0 if states is None else states.size(0)
+    xp = 0 if states is None else _whole(states, "states", torch.float32, (slots, heads, dk, dv), here)
+    if states is None and (from_slots is not None or to_slots is not None):
+        raise ValueError("slots need states")
+    fp = 0 if from_slots is None else _whole(from_slots, "from_slots", torch.int64, (seqs,), here)
+    tp = 0 if to_slots is None else _whole(to_slots, "to_slots", torch.int64, (seqs,), here)
+    out = q.new_empty((total, heads, dv), dtype=out_type)
+    args = _LINEAR.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dp, sp, xp, fp, tp, out.data_ptr(), q_stride, k_stride,
+                        v_stride, heads if each else 0, slots, seqs, total, most_q, heads, hk, dk, dv, types[kind],
+                        types[out_type], scale)
+    L = lib()
+    nbytes = L.iq4xs_linear_attention_workspace_bytes(args)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    L.check("iq4xs_linear_attention", args, ws.data_ptr() if nbytes else 0, nbytes,
+            torch._C._cuda_getCurrentRawStream(here))
+    return out
 
 
 def synthetic_weights(K: int, N: int, seed: int, first_block: int = 0, device=None):

@@ -5,6 +5,7 @@
 #include "attention_internal.h"
 #include "iq4xs_internal.h"
 #include "iq4xs_mi355x.h"
+#include "linear_internal.h"
 
 using namespace iq4xs;
 
@@ -74,6 +75,27 @@ int check_shared(const iq4xs_paged_attention_args* a, const iq4xs_shared_prefix*
     if (a->window != 0) return hipErrorNotSupported;
     if (a->total == 0 || a->seqs == 0) return hipSuccess;
     return x->len && count(x->most_len) && count(x->most_rows) ? hipSuccess : hipErrorInvalidValue;
+}
+
+int check_linear(const iq4xs_linear_attention_args* a) {
+    if (!a || a->heads <= 0 || a->qk_heads <= 0 || a->heads % a->qk_heads != 0 || a->dk <= 0 || a->dv <= 0)
+        return hipErrorInvalidValue;
+    if (!plain_type(a->in_type) || !plain_type(a->out_type) || !(a->scale == a->scale)) return hipErrorInvalidValue;
+    if (!served_head(a->dk) || !served_head(a->dv)) return hipErrorNotSupported;
+    if (a->total < 0 || a->total >= MAX_COUNT || a->seqs < 0 || a->seqs >= MAX_COUNT - 64) return hipErrorInvalidValue;
+    if (a->total == 0 || a->seqs == 0) return hipSuccess;
+    if (!given(a->q) || !given(a->k) || !given(a->v) || !given(a->out) || !a->decay || !a->starts)
+        return hipErrorInvalidValue;
+    if (!count(a->most_q) || (a->decay_stride != 0 && (a->decay_stride < a->heads || a->decay_stride >= MAX_COUNT)))
+        return hipErrorInvalidValue;
+    if (!stride_of(a->q_stride, a->qk_heads, a->dk) || !stride_of(a->k_stride, a->qk_heads, a->dk) ||
+        !stride_of(a->v_stride, a->heads, a->dv))
+        return hipErrorInvalidValue;
+    if (a->from_slots || a->to_slots) {
+        // a slot's place is counted in 64 bits
+        if (!given(a->states) || a->slots < 0 || a->slots >= MAX_COUNT) return hipErrorInvalidValue;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -147,6 +169,18 @@ int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const 
     const int err = check_shared(args, prefix);
     if (err != hipSuccess || args->total == 0 || args->seqs == 0) return err;
     return launch_shared_attention(*args, *prefix, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+size_t iq4xs_linear_attention_workspace_bytes(const struct iq4xs_linear_attention_args* args) {
+    if (check_linear(args) != hipSuccess || args->total == 0 || args->seqs == 0) return 0;
+    size_t bytes = 0;
+    return linear_attention_workspace(*args, &bytes) == hipSuccess ? bytes : 0;
+}
+
+int iq4xs_linear_attention(const struct iq4xs_linear_attention_args* args, void* ws, size_t ws_bytes, void* stream) {
+    const int err = check_linear(args);
+    if (err != hipSuccess || args->total == 0 || args->seqs == 0) return err;
+    return launch_linear_attention(*args, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
