@@ -505,7 +505,7 @@ size_t iq4xs_linear_attention_workspace_bytes(const struct iq4xs_linear_attentio
  * A sequence of more than most_q tokens is cut to its first most_q; rows past them and
  * those of no sequence are not written.  What is not finite in a token reaches the
  * outputs and states of its head from that token on (of v, its channel's), as infinities
- * or NaN, and nothing else.  Decays are taken as -200 at least, exp of which is nothing
+ * or NaN; others keep their bits.  Decays are taken as -200 at least, exp of which is nothing
  * beside any fp32 number.  The same call gives the same bits. */
 int iq4xs_linear_attention(const struct iq4xs_linear_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 

@@ -31,14 +31,11 @@
 #include "attention_core.h"
 #include "attention_internal.h"
 #include "iq4xs_internal.h"
+#include "lds_device.h"
 
 namespace iq4xs {
 
 constexpr int TILE_WAVES = 4, TILE_ROWS = 32 * TILE_WAVES;
-
-__device__ inline uint32_t lds_address(const void* p) {
-    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(const_cast<void*>(p));
-}
 
 // 16 bytes for each lane, from global base + offset to LDS at lds + 16 * lane, asynchronously (lds the same in all
 // lanes).  As asm: the compiler would let every later LDS read wait for it.  The kernel waits before the barrier that
@@ -48,16 +45,6 @@ __device__ inline void copy_to_lds(const void* base, uint32_t offset, uint32_t l
                  : "memory", "m0");
 }
 __device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-__device__ inline u4 read_row(uint32_t lds) {
-    return *reinterpret_cast<__attribute__((address_space(3))) const u4*>((uintptr_t)lds);
-}
-// Four keys of the lane's channel: 16 lanes read 4 rows of 16 channels and each gets a column.
-__device__ inline u2 read_column(uint32_t lds) {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(
-        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4*>((uintptr_t)lds)));
-}
 
 // Geometry of a tile in LDS: KEYS rows of 2 * D bytes, 16-byte pieces exchanged within a row.
 template <int D>

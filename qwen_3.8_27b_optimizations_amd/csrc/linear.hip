@@ -13,18 +13,26 @@ static LinearArgs args_of(const iq4xs_linear_attention_args& g) {
 }
 
 hipError_t linear_attention_workspace(const iq4xs_linear_attention_args& g, size_t* bytes) {
-    if (g.seqs > 0x7FFFFFFF / g.heads / 8) return hipErrorInvalidConfiguration;
-    *bytes = 0;
+    LinearPlan p;
+    if (!linear_plan(g, device_cu_count(), p)) return hipErrorInvalidConfiguration;
+    *bytes = p.state_bytes + p.decay_bytes;
     return hipSuccess;
 }
 
 hipError_t launch_linear_attention(const iq4xs_linear_attention_args& g, void* ws, size_t ws_bytes, hipStream_t stream) {
-    size_t need;
-    const hipError_t err = linear_attention_workspace(g, &need);
-    if (err != hipSuccess) return err;
+    LinearPlan p;
+    if (!linear_plan(g, device_cu_count(), p)) return hipErrorInvalidConfiguration;
+    const size_t need = p.state_bytes + p.decay_bytes;
     if (ws_bytes < need || (need && (!ws || reinterpret_cast<uintptr_t>(ws) % 256 != 0))) return hipErrorInvalidValue;
     clear_launch_error();
-    launch_linear_step(args_of(g), g.dk, g.dv, g.in_type, linear_step_grid(g), stream);
+    const LinearArgs a = args_of(g);
+    if (p.steps) {
+        launch_linear_steps(a, g.dk, g.dv, g.in_type, p.grid, stream);
+    } else {
+        float* states = static_cast<float*>(ws);
+        const LinearSegments segments{states, states + p.state_bytes / sizeof(float), p.segments, p.length};
+        launch_linear_chunks(a, segments, g.dk, g.dv, g.in_type, stream);
+    }
     return hipGetLastError();
 }
 

@@ -3,12 +3,21 @@
 
 #include <hip/hip_runtime.h>
 
-#include "iq4xs_mi355x.h"
+#include "linear_plan.h"
 
 namespace iq4xs {
 
 struct LinearArgs;
-int64_t linear_step_grid(const iq4xs_linear_attention_args& args);
-void launch_linear_step(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream);
+
+// Segments of `length` tokens that sequences are cut into; with one there are no states.
+struct LinearSegments {
+    float* states;  // [seqs][count][heads][dk][dv] that each begins with
+    float* decays;  // [seqs][count][heads] what each keeps of it
+    int count, length;
+};
+
+void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream);
+void launch_linear_chunks(const LinearArgs& a, const LinearSegments& segments, int dk, int dv, int type,
+                          hipStream_t stream);
 
 }  // namespace iq4xs

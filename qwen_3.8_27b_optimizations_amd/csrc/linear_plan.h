@@ -1,0 +1,49 @@
+// linear_plan.h -- which kernel takes a call of linear attention, and the segments of its sequences.  Plain arithmetic in a
+// header of its own, so that the host tests compile the same rules.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "iq4xs_mi355x.h"
+
+namespace iq4xs {
+
+// Columns of a state that a workgroup of the kernel of chunks takes: 128 while their accumulators fit the registers.
+inline int linear_chunk_columns(int dk, int dv) { return dk == 256 || dv == 64 ? 64 : 128; }
+
+struct LinearPlan {
+    bool steps;           // token by token
+    int segments;         // of the longest sequence
+    int length;           // tokens of a segment, a multiple of 64
+    int64_t grid;         // workgroups of the largest launch
+    size_t state_bytes;   // states that segments begin with
+    size_t decay_bytes;   // and what segments keep of them
+};
+
+// False: its launches would be too large.
+inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, LinearPlan& p) {
+    constexpr int64_t MOST = 0x7FFFFFFF;
+    const int64_t most = g.most_q < g.total ? g.most_q : g.total;
+    p = {true, 1, (int)((most + 63) / 64 * 64), 0, 0, 0};
+    if (g.seqs > MOST / g.heads / 8) return false;  // 32 columns of 256 at a time
+    p.grid = (g.seqs * g.heads * (g.dv / 32) + 3) / 4;
+    if (most <= 16) return true;
+    p.steps = false;
+    const int64_t units = g.seqs * g.heads * (g.dv / linear_chunk_columns(g.dk, g.dv));
+    int64_t segments = 2 * cus / units;
+    if (segments > most / 256) segments = most / 256;
+    if (segments > 1) {
+        p.length = (int)(((most + segments - 1) / segments + 63) / 64 * 64);
+        p.segments = (int)((most + p.length - 1) / p.length);
+    }
+    if (p.segments > 1) {
+        const int64_t places = g.seqs * p.segments * g.heads;
+        p.state_bytes = (size_t)places * g.dk * g.dv * sizeof(float);
+        p.decay_bytes = ((size_t)places * sizeof(float) + 255) / 256 * 256;
+    }
+    p.grid = units * p.segments;
+    return true;
+}
+
+}  // namespace iq4xs

@@ -90,11 +90,7 @@ static void launch_types(const LinearArgs& a, int dv, int type, dim3 grid, hipSt
         hipLaunchKernelGGL((linear_step_kernel<DK, __bf16>), grid, block, 0, stream, a, dv);
 }
 
-int64_t linear_step_grid(const iq4xs_linear_attention_args& g) {
-    return (g.seqs * g.heads * (g.dv / STEP_COLUMNS) + STEP_WAVES - 1) / STEP_WAVES;
-}
-
-void launch_linear_step(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream) {
+void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream) {
     const dim3 blocks((unsigned)grid);
     if (dk == 64)
         launch_types<64>(a, dv, type, blocks, stream);
