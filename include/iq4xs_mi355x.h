@@ -479,7 +479,7 @@ struct iq4xs_linear_attention_args {
     const int64_t* from_slots; /* [seqs] states that sequences go on from, or NULL: all begin at zeros */
     const int64_t* to_slots;   /* [seqs] where their states are left, or NULL: nowhere */
     void* out;                 /* [total][heads][dv], out_type; not the memory of an input */
-    int64_t q_stride, k_stride, v_stride, decay_stride; /* of a token, in elements */
+    int64_t q_stride, k_stride, v_stride, decay_stride; /* of a token, in elements: below 2^23 */
     int64_t slots, seqs, total;
     int64_t most_q; /* at least the tokens of any sequence */
     int32_t heads;  /* a multiple of qk_heads: head h reads q and k of head h / (heads / qk_heads) */

@@ -86,7 +86,11 @@ int check_linear(const iq4xs_linear_attention_args* a) {
     if (a->total == 0 || a->seqs == 0) return hipSuccess;
     if (!given(a->q) || !given(a->k) || !given(a->v) || !given(a->out) || !a->decay || !a->starts)
         return hipErrorInvalidValue;
-    if (!count(a->most_q) || (a->decay_stride != 0 && (a->decay_stride < a->heads || a->decay_stride >= MAX_COUNT)))
+    // places within a chunk of tokens are counted in 32 bits
+    constexpr int64_t MOST_STRIDE = (int64_t)1 << 23;
+    if (!count(a->most_q) || (a->decay_stride != 0 && a->decay_stride < a->heads)) return hipErrorInvalidValue;
+    if (a->q_stride >= MOST_STRIDE || a->k_stride >= MOST_STRIDE || a->v_stride >= MOST_STRIDE ||
+        a->decay_stride >= MOST_STRIDE)
         return hipErrorInvalidValue;
     if (!stride_of(a->q_stride, a->qk_heads, a->dk) || !stride_of(a->k_stride, a->qk_heads, a->dk) ||
         !stride_of(a->v_stride, a->heads, a->dv))

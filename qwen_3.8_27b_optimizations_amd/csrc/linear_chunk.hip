@@ -11,7 +11,7 @@
 
 namespace iq4xs {
 
-constexpr int CHUNK_WAVES = 4, CHUNK_THREADS = 64 * CHUNK_WAVES;
+constexpr int CHUNK = 32;  // tokens
 
 // Numbers as sums of bf16 parts: as many as hold the input types exactly.
 template <typename T>
@@ -57,10 +57,19 @@ struct Piece {
     }
     __device__ bool finite(int i) const { return fabsf(at(i)) <= FLT_MAX; }
     __device__ bool finite() const {
-        bool ok = true;
+        if constexpr (sizeof(T) == 4) {
+            uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ok = ok && finite(i);
-        return ok;
+            for (int i = 0; i < 8; ++i) top = max(top, w[i / 4][i % 4] & 0x7FFFFFFFu);
+            return top < 0x7F800000u;
+        } else {
+            typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+            s2 top{0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(s2, w[0][i] & 0x7FFF7FFFu));
+            return max(top.x, top.y) < (__is_same(T, _Float16) ? 0x7C00 : 0x7F80);
+        }
     }
     __device__ void clear_at(int i) {
         if constexpr (sizeof(T) == 4)
@@ -92,43 +101,91 @@ struct Piece {
 };
 
 // A tile in LDS: ROWS rows of CHANNELS bf16 numbers, 16-byte pieces exchanged within a row so that 16 rows' pieces of one
-// place lie in 16 places.
+// place lie in 16 places (reads of rows), and those of 4 rows in 4 groups of places (reads of columns).
 template <int ROWS, int CHANNELS>
 struct ChunkTile {
     static constexpr int ROW = 2 * CHANNELS, BYTES = ROWS * ROW, PIECES = CHANNELS / 8;
-    static constexpr int LOADS = ROWS * PIECES / CHUNK_THREADS;  // pieces of a thread
     static __device__ int place(int row, int piece) {
-        return piece ^ (PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : 0);
+        return piece ^ (PIECES >= 16 ? (row & 3) << 2 | (row >> 2 & 3) : PIECES == 8 ? (row & 2) << 1 | (row >> 2 & 3) : 0);
     }
     static __device__ uint32_t at(int row, int piece) { return row * ROW + 16 * place(row, piece); }
 };
 
-// 8 tokens of the lane's channel, as the left or right operand of a product over tokens: rows row0 to row0 + 7 of the lane's
-// group of 16, which reads channels 4 (lane % 4) of `piece`'s half `half`.
+// Sums over this lane and those before it.
+template <int CTRL, int ROWS>
+__device__ inline double plus_moved(double x) {
+    const u2 w = __builtin_bit_cast(u2, x);
+    const u2 y{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, ROWS, 0xF, false),
+               (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, ROWS, 0xF, false)};
+    return x + __builtin_bit_cast(double, y);
+}
+__device__ inline double running_sum(double x) {
+    x = plus_moved<0x111, 0xF>(x);  // 1, 2, 4 and 8 lanes on within 16
+    x = plus_moved<0x112, 0xF>(x);
+    x = plus_moved<0x114, 0xF>(x);
+    x = plus_moved<0x118, 0xF>(x);
+    x = plus_moved<0x142, 0xA>(x);     // the last of 16 to the next 16
+    return plus_moved<0x143, 0xC>(x);  // and the last of 32 to the next 32
+}
+
+// 2^x where x is large: its whole part apart, so that the rest keeps its bits.
+__device__ inline float exp2_of(double x) {
+    const double whole = rint(x);
+    return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)whole);
+}
+
+// Four tokens of the lane's channel and the four after them, as the left or right operand of a product over tokens.
 template <typename Tile>
-__device__ inline u4 eight_tokens(uint32_t tile, int row0, int piece, int half, int lane) {
-    const int row = row0 + lane % 16 / 4;
-    const u2 x = read_column(tile + Tile::at(row, piece) + 8 * half), y = read_column(tile + Tile::at(row + 4, piece) + 8 * half);
+__device__ inline u4 eight_tokens(uint32_t at) {
+    const u2 x = read_column(at), y = read_column((at ^ 16) + 4 * Tile::ROW);
     return u4{x.x, x.y, y.x, y.y};
 }
 
-// DK by DVT of a head's state belong to a workgroup, DVT / 4 columns to a wave, in accumulators.  OUT: parts that outputs
-// are made of.
-template <int DK, int DVT, int C, typename T, int OUT, bool STATE_ONLY>
-__global__ __launch_bounds__(CHUNK_THREADS, 2) void linear_chunk_kernel(LinearArgs a, LinearSegments seg, int dv) {
-    constexpr int IN = parts_of<T>, NT = DVT / 64, KS = DK / 32, TS = C / 32, IT = C / 16;
+// Eight fp32 values rounded to `type`.
+__device__ inline void store8(void* p, int type, f4 x, f4 y) {
+    if (type == IQ4XS_TYPE_F32) {
+        static_cast<f4*>(p)[0] = x;
+        static_cast<f4*>(p)[1] = y;
+        return;
+    }
+    typedef float f8 __attribute__((ext_vector_type(8)));
+    const f8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    if (type == IQ4XS_TYPE_F16)
+        *static_cast<h8*>(p) = __builtin_convertvector(v, h8);
+    else
+        *static_cast<b8*>(p) = __builtin_convertvector(v, b8);
+}
+
+// What a chunk's decays come to.
+template <int C>
+struct ChunkScales {
+    double sum[C];         // of decays up to a token, times log2(e)
+    float from_start[C];   // of the state in an output: 2^sum, the output's scale, and 2^held as the chunk begins
+    float to_end[C];       // of a token in the state: 2^(whole - sum), and 2^-held as it ends
+    float again;           // what the accumulators are multiplied by before the chunk's tokens come to them
+};
+
+// DK by 16 NT WAVES of a head's state belong to a workgroup, 16 NT columns to a wave, in accumulators.  OUT: parts of the
+// state and of weights that outputs are made of.  AHEAD: whether the next chunk's keys and values have room in LDS beside
+// this one's.
+template <int DK, int NT, int WAVES, typename T, int OUT, bool STATE_ONLY, bool AHEAD>
+__global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs a, LinearSegments seg, int dv) {
+    constexpr int C = CHUNK, IN = parts_of<T>, KS = DK / 32, IT = C / 16, DVT = 16 * NT * WAVES, THREADS = 64 * WAVES;
+    // products of parts p and o count while p + o is below OUT
+    constexpr int BUFFERS = AHEAD ? 2 : 1;
     using KTile = ChunkTile<C, DK>;
     using VTile = ChunkTile<C, DVT>;
     using PTile = ChunkTile<C, C>;
-    static_assert(KTile::LOADS * CHUNK_THREADS == C * KTile::PIECES && VTile::LOADS * CHUNK_THREADS == C * VTile::PIECES,
-                  "pieces are dealt out evenly");
-    __shared__ __attribute__((aligned(1024))) uint8_t qs[STATE_ONLY ? 1 : IN][STATE_ONLY ? 16 : KTile::BYTES];
-    __shared__ __attribute__((aligned(1024))) uint8_t ks[IN][KTile::BYTES];
-    __shared__ __attribute__((aligned(1024))) uint8_t vs[IN][VTile::BYTES];
-    __shared__ __attribute__((aligned(1024))) uint8_t ps[STATE_ONLY ? 1 : OUT][STATE_ONLY ? 16 : PTile::BYTES];
-    __shared__ double sum[C];             // of decays up to a token, times log2(e)
-    __shared__ float from_start[C], to_end[C];
-    __shared__ int odd, odd_from[DVT];    // whether values are not finite, and a channel's first token of such
+    constexpr int K_LOADS = C * KTile::PIECES / THREADS, V_LOADS = C * VTile::PIECES / THREADS;  // pieces of a thread
+    static_assert(K_LOADS * THREADS == C * KTile::PIECES && V_LOADS * THREADS == C * VTile::PIECES, "dealt out evenly");
+    constexpr int K_BYTES = IN * KTile::BYTES, V_BYTES = IN * VTile::BYTES;  // of a buffer
+    __shared__ __attribute__((aligned(1024))) uint8_t qs[STATE_ONLY ? 1024 : K_BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t ks[BUFFERS * K_BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t vs[BUFFERS * V_BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t ps[STATE_ONLY ? 1024 : OUT * PTile::BYTES];
+    __shared__ ChunkScales<C> scales[WAVES];  // of as many chunks at a time
+    __shared__ double wholes[WAVES];
+    __shared__ int odd[2], odd_from[2][DVT];  // whether values are not finite, and a channel's first token of such
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int n = lane % 16, j = lane / 16;
 
@@ -147,18 +204,31 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void linear_chunk_kernel(LinearAr
     if (STATE_ONLY && last) return;
     const int end = last ? all.count : begin + seg.length;
 
-    const uint32_t q_at = lds_address(qs), k_at = lds_address(ks), v_at = lds_address(vs), p_at = lds_address(ps);
+    // Where this lane reads: rows n, piece j; columns by groups of 16 lanes that read 4 rows of 4 pieces' halves.  Other
+    // pieces are exclusive ors away, other rows sums; 4 rows on are a piece's neighbour.
+    const int r4 = lane % 16 / 4, base = 16 * NT * wave;  // base: of the wave's columns
+    uint32_t q_row = lds_address(qs) + KTile::at(n, j), k_row = lds_address(ks) + KTile::at(n, j);
+    uint32_t p_row = lds_address(ps) + PTile::at(n, j), k_column = lds_address(ks) + KTile::at(8 * j + r4, lane % 4);
+    uint32_t v_column = lds_address(vs) + (NT == 2 ? VTile::at(8 * j + r4, base / 8 + lane % 4)
+                                                   : VTile::at(8 * j + r4, base / 8 + lane % 4 / 2) + 8 * (lane % 2));
     const T* q = static_cast<const T*>(a.q) + (head / a.group) * DK;
     const T* k = static_cast<const T*>(a.k) + (head / a.group) * DK;
     const T* v = static_cast<const T*>(a.v) + head * dv + tile * DVT;
 
     // state: column n of the wave's tile u, rows 32 s + 8 j + 4 t + r
-    const int base = DVT / 4 * wave;  // of the wave's columns
     auto column = [&](int u, int m) { return NT == 2 ? base + 8 * (m / 4) + 4 * u + m % 4 : base + m; };
+    auto state_place = [&](auto* state, int s, int t, int u, int r) {
+        const uint32_t lane_off = (8 * j * dv + tile * DVT + column(u, n)) * (uint32_t)sizeof(float);
+        using P = decltype(state);
+        return reinterpret_cast<P>((char*)(state + (32 * s + 4 * t + r) * dv) + lane_off);
+    };
     f4 S[KS][2][NT];
-    const float* from = STATE_ONLY ? nullptr
-                        : part == 0 && last ? state_at(a, a.from_slots, seq, head, DK * dv)
-                                            : seg.states + ((int64_t)(seq * seg.count + part) * a.heads + head) * DK * dv;
+    auto segment_state = [&](int i) { return seg.states + ((int64_t)(seq * seg.count + i) * a.heads + head) * DK * dv; };
+    // The first segment goes on from the sequence's state, in both passes: the pass over states leaves a copy of it, since
+    // the last segment may write it while others begin.
+    const float* from = part == 0 && (STATE_ONLY || last) ? state_at(a, a.from_slots, seq, head, DK * dv)
+                        : STATE_ONLY                      ? nullptr
+                                                          : segment_state(part);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -167,99 +237,177 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void linear_chunk_kernel(LinearAr
             for (int u = 0; u < NT; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    S[s][t][u][r] = from ? from[(32 * s + 8 * j + 4 * t + r) * dv + tile * DVT + column(u, n)] : 0.0f;
-    if constexpr (!STATE_ONLY) {
-        for (int i = threadIdx.x; i < OUT * PTile::BYTES / 16; i += CHUNK_THREADS)
-            *reinterpret_cast<u4*>(&ps[0][16 * i]) = u4{0, 0, 0, 0};  // above the diagonal
+                    S[s][t][u][r] = from ? *state_place(from, s, t, u, r) : 0.0f;
+
+    if constexpr (STATE_ONLY) {
+        if (part == 0) {
+            float* copy = segment_state(0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) *state_place(copy, s, t, u, r) = S[s][t][u][r];
+        }
     }
 
-    Piece<T> qn[STATE_ONLY ? 1 : KTile::LOADS], kn[KTile::LOADS], vn[VTile::LOADS];
-    float gn;
-    // rows past the end read the last one, and are cleared on their way into LDS
-    auto fetch = [&](int chunk) {
-        auto row = [&](int i) { return (int64_t)(all.first + (chunk + i < end ? chunk + i : end - 1)); };
+    Piece<T> qn[STATE_ONLY ? 1 : K_LOADS], kn[K_LOADS], vn[V_LOADS];
+    // places of this thread's pieces in a chunk, in bytes; rows past the end read the last one, and are cleared on their way
+    // into LDS
+    uint32_t q_off[K_LOADS], k_off[K_LOADS], v_off[V_LOADS];
+    auto places = [&](int count) {
+        auto row = [&](int i) { return (uint32_t)(i < count ? i : count - 1); };
 #pragma unroll
-        for (int l = 0; l < KTile::LOADS; ++l) {
-            const int i = threadIdx.x + l * CHUNK_THREADS;
-            if constexpr (!STATE_ONLY) qn[l].load(q + row(i / KTile::PIECES) * a.q_stride + 8 * (i % KTile::PIECES));
-            kn[l].load(k + row(i / KTile::PIECES) * a.k_stride + 8 * (i % KTile::PIECES));
+        for (int l = 0; l < K_LOADS; ++l) {
+            const int i = threadIdx.x + l * THREADS, channel = 8 * (i % KTile::PIECES);
+            q_off[l] = (row(i / KTile::PIECES) * (uint32_t)a.q_stride + channel) * sizeof(T);
+            k_off[l] = (row(i / KTile::PIECES) * (uint32_t)a.k_stride + channel) * sizeof(T);
         }
 #pragma unroll
-        for (int l = 0; l < VTile::LOADS; ++l) {
-            const int i = threadIdx.x + l * CHUNK_THREADS;
-            vn[l].load(v + row(i / VTile::PIECES) * a.v_stride + 8 * (i % VTile::PIECES));
+        for (int l = 0; l < V_LOADS; ++l) {
+            const int i = threadIdx.x + l * THREADS;
+            v_off[l] = (row(i / VTile::PIECES) * (uint32_t)a.v_stride + 8 * (i % VTile::PIECES)) * sizeof(T);
         }
-        gn = decay_at(a, row(lane % C), head);
     };
-    // The first `count` rows of the chunk that was fetched, zeros behind them.  A value that is not finite would reach the
-    // rows before it (a weight of zero times an infinity): it becomes zero, and its channel NaN from its row on.
-    auto put = [&](int count) {
+    auto fetch = [&](int chunk) {
+        if (end - chunk < C) places(end - chunk);
+        const int64_t row = all.first + chunk;
+        auto at = [&](const T* p, int64_t stride, uint32_t off) {
+            return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p + row * stride) + off);
+        };
+#pragma unroll
+        for (int l = 0; l < K_LOADS; ++l) {
+            if constexpr (!STATE_ONLY) qn[l].load(at(q, a.q_stride, q_off[l]));
+            kn[l].load(at(k, a.k_stride, k_off[l]));
+        }
+#pragma unroll
+        for (int l = 0; l < V_LOADS; ++l) vn[l].load(at(v, a.v_stride, v_off[l]));
+    };
+    // The first `count` rows of the chunk that was fetched, zeros behind them, into a buffer.  A value that is not finite
+    // would reach the rows before it (a weight of zero times an infinity): it becomes zero, and its channel NaN from its row
+    // on.
+    auto put = [&](int count, int parity) {
+        const int buffer = AHEAD ? parity : 0;
         auto store = [&](uint8_t* to, int bytes, uint32_t at, const u4* p) {
 #pragma unroll
             for (int i = 0; i < IN; ++i) *reinterpret_cast<u4*>(to + i * bytes + at) = p[i];
         };
         u4 p[IN];
 #pragma unroll
-        for (int l = 0; l < KTile::LOADS; ++l) {
-            const int i = threadIdx.x + l * CHUNK_THREADS, row = i / KTile::PIECES;
+        for (int l = 0; l < K_LOADS; ++l) {
+            const int i = threadIdx.x + l * THREADS, row = i / KTile::PIECES;
             const uint32_t at = KTile::at(row, i % KTile::PIECES);
             if constexpr (!STATE_ONLY) {
                 qn[l].parts(p);
-                store(qs[0], KTile::BYTES, at, p);
+                store(qs, KTile::BYTES, at, p);
             }
-            Piece<T> y = kn[l];
-            y.clear(row >= count);
-            y.parts(p);
-            store(ks[0], KTile::BYTES, at, p);
+            kn[l].clear(row >= count);
+            kn[l].parts(p);
+            store(ks + buffer * K_BYTES, KTile::BYTES, at, p);
         }
 #pragma unroll
-        for (int l = 0; l < VTile::LOADS; ++l) {
-            const int i = threadIdx.x + l * CHUNK_THREADS, row = i / VTile::PIECES;
-            Piece<T> y = vn[l];
-            y.clear(row >= count);
-            if (__builtin_expect(!y.finite(), 0)) {
+        for (int l = 0; l < V_LOADS; ++l) {
+            const int i = threadIdx.x + l * THREADS, row = i / VTile::PIECES;
+            vn[l].clear(row >= count);
+            if (__builtin_expect(!vn[l].finite(), 0)) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (y.finite(e)) continue;
-                    y.clear_at(e);
-                    atomicMin(&odd_from[8 * (i % VTile::PIECES) + e], row);
+                    if (vn[l].finite(e)) continue;
+                    vn[l].clear_at(e);
+                    atomicMin(&odd_from[parity][8 * (i % VTile::PIECES) + e], row);
                 }
-                odd = 1;
+                odd[parity] = 1;
             }
-            y.parts(p);
-            store(vs[0], VTile::BYTES, VTile::at(row, i % VTile::PIECES), p);
-        }
-        if (wave == 0 && lane < C) {
-            double g = lane < count ? (double)gn * 1.4426950408889634 : 0.0;
-#pragma unroll
-            for (int d = 1; d < C; d *= 2) {
-                const double before = __shfl_up(g, d);
-                if (lane >= d) g += before;
-            }
-            const double whole = __shfl(g, C - 1);
-            sum[lane] = g;
-            from_start[lane] = __builtin_amdgcn_exp2f((float)g);
-            to_end[lane] = __builtin_amdgcn_exp2f((float)(whole - g));
+            vn[l].parts(p);
+            store(vs + buffer * V_BYTES, VTile::BYTES, VTile::at(row, i % VTile::PIECES), p);
         }
     };
 
-    double decayed = 0.0;  // of the segment so far, times log2(e)
-    auto compute = [&](int chunk, int count, bool some_odd) {
+    // What the accumulators hold is the state times 2^-held: decays of many chunks go into the scales of what is added and
+    // read, and into the accumulators only when they pass 2^40.  The scales of the next chunks, one to a wave (scanning the
+    // decays of one chunk after another would keep the other waves waiting for the one that does).
+    double held = 0.0, decayed = 0.0;  // and of the segment so far, times log2(e)
+    float gn;
+    auto decays = [&](int chunk) {  // of the wave's chunk of those from `chunk` on, ahead of their use
+        const int i = chunk + C * wave + lane % C;
+        const int64_t row = all.first + (i < end ? i : end - 1);
+        gn = a.decay[row * a.decay_stride + head];
+    };
+    auto scale = [&](int chunk) {
+        const int mine = chunk + C * wave;
+        // decays below -200 are zeros beside any fp32 number, and sums of them keep their bits; a NaN stays
+        const double g = running_sum(mine + lane < end ? (double)(gn < -200.0f ? -200.0f : gn) * 1.4426950408889634 : 0.0);
+        if (lane == C - 1) wholes[wave] = g;
+        __syncthreads();
+        double before = 0.0, after = 0.0, whole = 0.0;  // held around the wave's chunk
+        float by = 1.0f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            const double x = wholes[i];
+            if (i == wave) before = held, whole = x;
+            held += x;
+            decayed += x;
+            const bool over = !(fabs(held) < 40.0);
+            if (i == wave && over) by = exp2_of(held);
+            if (over) held = 0.0;
+            if (i == wave) after = held;
+        }
+        ChunkScales<C>& to = scales[wave];
+        if (lane < C) {
+            to.sum[lane] = g;
+            to.from_start[lane] = __builtin_amdgcn_exp2f((float)g) * (a.scale * exp2_of(before));
+            to.to_end[lane] = __builtin_amdgcn_exp2f((float)(whole - g)) * exp2_of(-after);
+        }
+        if (lane == 0) to.again = by;
+        decays(chunk + C * WAVES);
+    };
+
+    const uint32_t out_bytes = a.out_type == IQ4XS_TYPE_F32 ? 4 : 2;
+    for (int i = threadIdx.x; i < 2 * DVT; i += THREADS) odd_from[i / DVT][i % DVT] = C;
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+    if constexpr (!STATE_ONLY) {
+        for (int i = threadIdx.x; i < OUT * PTile::BYTES / 16; i += THREADS)
+            *reinterpret_cast<u4*>(&ps[16 * i]) = u4{0, 0, 0, 0};  // above the diagonal
+    }
+    __syncthreads();
+    decays(begin);
+    places(C);
+    fetch(begin);
+    put(end - begin, 0);
+    if (begin + C < end) fetch(begin + C);
+    __syncthreads();
+    bool was_odd = false;
+    for (int chunk = begin, which = 0; chunk < end; chunk += C, ++which) {
+        const int parity = which % 2;
+        const bool more = chunk + C < end;
+        const int count = end - chunk;
+        if (which % WAVES == 0) {
+            scale(chunk);
+            __syncthreads();
+        }
+        const ChunkScales<C>& sc = scales[which % WAVES];
+        // the places along a row are cheaper computed than kept
+        asm volatile("" : "+v"(q_row), "+v"(k_row), "+v"(p_row), "+v"(k_column), "+v"(v_column));
+        const uint32_t k_buffer = AHEAD ? parity * K_BYTES : 0, v_buffer = AHEAD ? parity * V_BYTES : 0;
+        if (__builtin_expect(was_odd, 0)) {
+            for (int i = threadIdx.x; i < DVT; i += THREADS) odd_from[parity ^ 1][i] = C;
+            if (threadIdx.x == 0) odd[parity ^ 1] = 0;
+        }
+        f4 O[IT][NT];
         if constexpr (!STATE_ONLY) {
             // weighted scores of tiles on and below the diagonal: keys 16 kt + 4 j + r of query 16 it + n
-#pragma unroll
-            for (int i = 0; i < (IT * (IT + 1) / 2 + CHUNK_WAVES - 1) / CHUNK_WAVES; ++i) {
-                const int which = i * CHUNK_WAVES + wave;
-                if (which >= IT * (IT + 1) / 2) break;
-                const int it = which >= 6 ? 3 : which >= 3 ? 2 : which >= 1 ? 1 : 0, kt = which - it * (it + 1) / 2;
+            if (wave < 3) {
+                const int it = wave > 0, kt = wave > 1;
                 f4 z{0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     u4 x[IN], y[IN];
 #pragma unroll
                     for (int p = 0; p < IN; ++p) {
-                        x[p] = read_row(k_at + p * KTile::BYTES + KTile::at(16 * kt + n, 4 * s + j));
-                        y[p] = read_row(q_at + p * KTile::BYTES + KTile::at(16 * it + n, 4 * s + j));
+                        x[p] = read_row((k_row ^ 64 * s) + k_buffer + p * KTile::BYTES + 16 * kt * KTile::ROW);
+                        y[p] = read_row((q_row ^ 64 * s) + p * KTile::BYTES + 16 * it * KTile::ROW);
                     }
 #pragma unroll
                     for (int p = IN - 1; p >= 0; --p)
@@ -268,232 +416,255 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void linear_chunk_kernel(LinearAr
                             if (p + o < OUT) z = Matrix<__bf16>::mma16(x[p], y[o], z);
                 }
                 const int query = 16 * it + n, key = 16 * kt + 4 * j;
-                const double g = sum[query];
+                const double g = sc.sum[query];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float w = __builtin_amdgcn_exp2f((float)(g - sum[key + r])) * a.scale;
+                    const float w = __builtin_amdgcn_exp2f((float)(g - sc.sum[key + r])) * a.scale;
                     z[r] = key + r <= query ? z[r] * w : 0.0f;
                 }
-                uint32_t lo2[OUT], hi2[OUT];
-                split<OUT>(z[0], z[1], lo2);
-                split<OUT>(z[2], z[3], hi2);
+                uint32_t lo[OUT], hi[OUT];
+                split<OUT>(z[0], z[1], lo);
+                split<OUT>(z[2], z[3], hi);
 #pragma unroll
                 for (int p = 0; p < OUT; ++p)
-                    *reinterpret_cast<u2*>(&ps[p][PTile::at(query, key / 8) + 2 * (key % 8)]) = u2{lo2[p], hi2[p]};
+                    *reinterpret_cast<u2*>(&ps[p * PTile::BYTES + PTile::at(query, key / 8) + 2 * (key % 8)]) = u2{lo[p], hi[p]};
             }
-        }
-        // the wave's values: channels of tile u by tokens 32 t + 8 j + e
-        u4 V[TS][NT][IN];
-#pragma unroll
-        for (int t = 0; t < TS; ++t)
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int p = 0; p < IN; ++p) {
-                    const uint32_t at = v_at + p * VTile::BYTES;
-                    V[t][u][p] = NT == 2 ? eight_tokens<VTile>(at, 32 * t + 8 * j, base / 8 + lane % 4, u, lane)
-                                         : eight_tokens<VTile>(at, 32 * t + 8 * j, base / 8 + lane % 4 / 2, lane % 2, lane);
-                }
-        if constexpr (!STATE_ONLY) {
-            f4 O[IT][NT];
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
                 for (int u = 0; u < NT; ++u) O[i][u] = f4{0, 0, 0, 0};
+            // a step's queries are read while the step before it is multiplied
+            u4 y[2][IT][IN];
+            auto queries = [&](int s) {
+#pragma unroll
+                for (int i = 0; i < IT; ++i)
+#pragma unroll
+                    for (int p = 0; p < IN; ++p)
+                        y[s % 2][i][p] = read_row((q_row ^ 64 * s) + p * KTile::BYTES + 16 * i * KTile::ROW);
+            };
+            queries(0);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
+                if (s + 1 < KS) queries(s + 1);
+                __builtin_amdgcn_sched_barrier(0);
                 u4 x[NT][OUT];
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        uint32_t y[OUT];
-                        split<OUT>(S[s][e / 2][u][2 * (e % 2)], S[s][e / 2][u][2 * (e % 2) + 1], y);
+                        uint32_t z[OUT];
+                        split<OUT>(S[s][e / 2][u][2 * (e % 2)], S[s][e / 2][u][2 * (e % 2) + 1], z);
 #pragma unroll
-                        for (int p = 0; p < OUT; ++p) x[u][p][e] = y[p];
+                        for (int p = 0; p < OUT; ++p) x[u][p][e] = z[p];
                     }
 #pragma unroll
-                for (int i = 0; i < IT; ++i) {
-                    u4 y[IN];
+                for (int p = OUT - 1; p >= 0; --p)
 #pragma unroll
-                    for (int p = 0; p < IN; ++p)
-                        y[p] = read_row(q_at + p * KTile::BYTES + KTile::at(16 * i + n, 4 * s + j));
+                    for (int o = IN - 1; o >= 0; --o)
 #pragma unroll
-                    for (int u = 0; u < NT; ++u)
+                        for (int i = 0; i < IT; ++i)
 #pragma unroll
-                        for (int p = OUT - 1; p >= 0; --p)
-#pragma unroll
-                            for (int o = IN - 1; o >= 0; --o)
-                                if (p + o < OUT) O[i][u] = Matrix<__bf16>::mma16(x[u][p], y[o], O[i][u]);
-                }
+                            for (int u = 0; u < NT; ++u)
+                                if (p + o < OUT) O[i][u] = Matrix<__bf16>::mma16(x[u][p], y[s % 2][i][o], O[i][u]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __syncthreads();  // weighted scores are there
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
-                const float w = from_start[16 * i + n] * a.scale;
+                const float w = sc.from_start[16 * i + n];
 #pragma unroll
                 for (int u = 0; u < NT; ++u) O[i][u] *= w;
+            }
+            __syncthreads();  // weighted scores are there, queries done with
+        }
+        if (AHEAD && more) {
+            put(end - chunk - C, parity ^ 1);
+            if (chunk + 2 * C < end) fetch(chunk + 2 * C);
+        }
+        // keys of a step of the state's update, read while the step before it is multiplied
+        u4 kx[2][2][IN];
+        auto keys = [&](int s) {
 #pragma unroll
-                for (int t = 0; t <= i / 2; ++t) {
-                    u4 y[OUT];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int p = 0; p < OUT; ++p) y[p] = read_row(p_at + p * PTile::BYTES + PTile::at(16 * i + n, 4 * t + j));
+                for (int p = 0; p < IN; ++p)
+                    kx[s % 2][h][p] = eight_tokens<KTile>((k_column ^ 64 * s) + 8 * h + k_buffer + p * KTile::BYTES);
+        };
+        // the wave's values: channels of tile u by tokens 8 j + e
+        u4 V[NT][IN];
 #pragma unroll
-                    for (int u = 0; u < NT; ++u)
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-                        for (int p = OUT - 1; p >= 0; --p)
+            for (int p = 0; p < IN; ++p) V[u][p] = eight_tokens<VTile>(v_column + v_buffer + 8 * u + p * VTile::BYTES);
+        const bool some_odd = odd[parity] != 0;
+        float w[8];
+        const float again = sc.again;
 #pragma unroll
-                            for (int o = IN - 1; o >= 0; --o)
-                                if (p + o < OUT) O[i][u] = Matrix<__bf16>::mma16(V[t][u][o], y[p], O[i][u]);
+        for (int e = 0; e < 8; ++e) w[e] = sc.to_end[8 * j + e];
+        u4 y[IT][OUT];
+        if constexpr (!STATE_ONLY) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int p = 0; p < OUT; ++p) y[i][p] = read_row(p_row + p * PTile::BYTES + 16 * i * PTile::ROW);
+        }
+        keys(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!STATE_ONLY) {
+#pragma unroll
+            for (int p = OUT - 1; p >= 0; --p)
+#pragma unroll
+                for (int o = IN - 1; o >= 0; --o)
+#pragma unroll
+                    for (int i = 0; i < IT; ++i)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+                            if (p + o < OUT) O[i][u] = Matrix<__bf16>::mma16(V[u][o], y[i][p], O[i][u]);
+        }
+        if (__builtin_expect(again != 1.0f, 0)) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) S[s][h][u] *= again;
+        }
+        // values times what is left of them at the chunk's end, and the state's update
+        u4 W[NT][3];
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x0 = __uint_as_float(V[u][IN - 1][e] << 16), x1 = high_part(__uint_as_float(V[u][IN - 1][e]));
+#pragma unroll
+                for (int p = IN - 2; p >= 0; --p) {
+                    x0 += __uint_as_float(V[u][p][e] << 16);
+                    x1 += high_part(__uint_as_float(V[u][p][e]));
                 }
+                uint32_t z[3];
+                split<3>(x0 * w[2 * e], x1 * w[2 * e + 1], z);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) W[u][p][e] = z[p];
+            }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) keys(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int o = 2; o >= 0; --o)
+#pragma unroll
+                for (int p = IN - 1; p >= 0; --p)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+                            if (p + o < 3) S[s][h][u] = Matrix<__bf16>::mma16(kx[s % 2][h][p], W[u][o], S[s][h][u]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!STATE_ONLY) {
+            char* out = static_cast<char*>(a.out) + (int64_t)(all.first + chunk) * a.heads * dv * out_bytes;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
                 const int row = 16 * i + n;
                 if (__builtin_expect(some_odd, 0)) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (row >= odd_from[column(u, 4 * j + r)]) O[i][u][r] = NAN;
+                            if (row >= odd_from[parity][column(u, 4 * j + r)]) O[i][u][r] = NAN;
                 }
                 if (row < count) {
-                    const int64_t at = ((int64_t)(all.first + chunk + row) * a.heads + head) * dv + tile * DVT;
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) store4(a.out, at + column(u, 4 * j), a.out_type, O[i][u]);
+                    // two tiles' columns of a lane lie one after another
+                    const uint32_t at = ((uint32_t)row * a.heads + head) * dv + tile * DVT + column(0, 4 * j);
+                    char* to = out + at * out_bytes;
+                    if constexpr (NT == 2)
+                        store8(to, a.out_type, O[i][0], O[i][NT - 1]);
+                    else
+                        store4(to, 0, a.out_type, O[i][0]);
                 }
             }
         }
-        // values times what is left of them at the chunk's end, and the state's update
-        const float keep = from_start[C - 1];
-        u4 W[TS][NT][3];
-#pragma unroll
-        for (int t = 0; t < TS; ++t) {
-            const float* w = &to_end[32 * t + 8 * j];
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x0 = 0.0f, x1 = 0.0f;
-#pragma unroll
-                    for (int p = IN - 1; p >= 0; --p) {
-                        x0 += __uint_as_float(V[t][u][p][e] << 16);
-                        x1 += high_part(__uint_as_float(V[t][u][p][e]));
-                    }
-                    uint32_t y[3];
-                    split<3>(x0 * w[2 * e], x1 * w[2 * e + 1], y);
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) W[t][u][p][e] = y[p];
-                }
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int u = 0; u < NT; ++u) S[s][h][u] *= keep;
-#pragma unroll
-                for (int t = 0; t < TS; ++t) {
-                    u4 x[IN];
-#pragma unroll
-                    for (int p = 0; p < IN; ++p)
-                        x[p] = eight_tokens<KTile>(k_at + p * KTile::BYTES, 32 * t + 8 * j, 4 * s + lane % 4, h, lane);
-#pragma unroll
-                    for (int u = 0; u < NT; ++u)
-#pragma unroll
-                        for (int o = 2; o >= 0; --o)
-#pragma unroll
-                            for (int p = IN - 1; p >= 0; --p)
-                                if (p + o < 3) S[s][h][u] = Matrix<__bf16>::mma16(x[p], W[t][u][o], S[s][h][u]);
-                }
-            }
         if (__builtin_expect(some_odd, 0)) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
-                const float x = odd_from[column(u, n)] < C ? NAN : 0.0f;
+                const float x = odd_from[parity][column(u, n)] < C ? NAN : 0.0f;
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) S[s][h][u] += x;
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < DVT; i += CHUNK_THREADS) odd_from[i] = C;
-            if (threadIdx.x == 0) odd = 0;
         }
-        if constexpr (STATE_ONLY) decayed += sum[C - 1];
-    };
-
-    for (int i = threadIdx.x; i < DVT; i += CHUNK_THREADS) odd_from[i] = C;
-    if (threadIdx.x == 0) odd = 0;
-    fetch(begin);
-    for (int chunk = begin; chunk < end; chunk += C) {
-        const int count = end - chunk < C ? end - chunk : C;
-        __syncthreads();  // the chunk before is done with
-        put(count);
-        __syncthreads();
-        const bool some_odd = odd != 0;
-        if (chunk + C < end) fetch(chunk + C);
-        compute(chunk, count, some_odd);
+        was_odd = some_odd;
+        __syncthreads();  // keys and values are done with, and the next there
+        if (!AHEAD && more) {
+            put(end - chunk - C, parity ^ 1);
+            if (chunk + 2 * C < end) fetch(chunk + 2 * C);
+            __syncthreads();
+        }
     }
 
+    if (STATE_ONLY && tile == 0 && threadIdx.x == 0)
+        seg.decays[(seq * seg.count + part) * (int64_t)a.heads + head] = exp2_of(decayed);
     float* to = STATE_ONLY ? seg.states + ((int64_t)(seq * seg.count + part + 1) * a.heads + head) * DK * dv
                 : last     ? state_at(a, a.to_slots, seq, head, DK * dv)
                            : nullptr;
-    if (to) {
+    if (!to) return;
+    // the scales of chunks past the last one are those of no decay
+    const float by = exp2_of(held);
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int u = 0; u < NT; ++u)
+            for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        to[(32 * s + 8 * j + 4 * t + r) * dv + tile * DVT + column(u, n)] = S[s][t][u][r];
-    }
-    if constexpr (STATE_ONLY) {
-        if (threadIdx.x == 0 && tile == 0)
-            seg.decays[(seq * seg.count + part) * (int64_t)a.heads + head] = __builtin_amdgcn_exp2f((float)decayed);
-    }
+                for (int r = 0; r < 4; ++r)
+                    *state_place(to, s, t, u, r) = S[s][t][u][r] * by;
 }
 
-// The states that segments begin with, from the sequence's own and what each segment adds: in place, the first included.
+// The states that segments begin with, in the place of what each adds, from the third on.
 __global__ __launch_bounds__(256) void join_segments_kernel(LinearArgs a, LinearSegments seg, int size) {
     const int pieces = size / 4;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int piece = (int)(at % pieces), head = (int)(at / pieces % a.heads), seq = (int)(at / pieces / a.heads);
     if (seq >= a.seqs) return;
     const Rows all = rows_of(a, seq);
-    if (all.count <= seg.length) return;
-    const float* from = state_at(a, a.from_slots, seq, head, size);
-    f4 s = from ? load4(from + 4 * piece) : f4{0, 0, 0, 0};
     const int count = (all.count + seg.length - 1) / seg.length;
-    for (int i = 0; i < count; ++i) {
-        const int64_t place = (int64_t)(seq * seg.count + i) * a.heads + head;
-        f4* p = reinterpret_cast<f4*>(seg.states + place * size + 4 * piece);
-        if (i > 0) s = s * seg.decays[place - a.heads] + *p;
-        *p = s;
+    if (count < 3) return;
+    const int64_t first = (int64_t)seq * seg.count * a.heads + head;
+    f4* p = reinterpret_cast<f4*>(seg.states + first * size + 4 * piece);
+    const int64_t step = (int64_t)a.heads * pieces;
+    f4 s = p[step];
+#pragma unroll 8
+    for (int i = 2; i < count; ++i) {
+        s = s * seg.decays[first + (i - 1) * (int64_t)a.heads] + p[i * step];
+        p[i * step] = s;
     }
 }
 
-template <int DK, int DVT, int C, typename T, int OUT>
+template <int DK, int NT, int WAVES, typename T, int OUT>
 static void launch(const LinearArgs& a, const LinearSegments& seg, int dv, hipStream_t stream) {
-    const dim3 block(CHUNK_THREADS), grid((unsigned)((int64_t)a.seqs * seg.count * a.heads * (dv / DVT)));
+    // 160 KiB of LDS: queries of all parts once, keys and values twice
+    constexpr int ROWS = 2 * CHUNK * parts_of<T>, COLUMNS = 16 * NT * WAVES;
+    constexpr bool AHEAD = ROWS * (3 * DK + 2 * COLUMNS) + 12 * 1024 <= 160 * 1024;
+    const dim3 block(64 * WAVES), grid((unsigned)((int64_t)a.seqs * seg.count * a.heads * (dv / COLUMNS)));
     if (seg.count > 1) {
-        hipLaunchKernelGGL((linear_chunk_kernel<DK, DVT, C, T, OUT, true>), grid, block, 0, stream, a, seg, dv);
+        hipLaunchKernelGGL((linear_chunk_kernel<DK, NT, WAVES, T, 2, true, AHEAD>), grid, block, 0, stream, a, seg, dv);
         const int64_t pieces = (int64_t)a.seqs * a.heads * DK * dv / 4;
         hipLaunchKernelGGL(join_segments_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, a, seg, DK * dv);
     }
-    hipLaunchKernelGGL((linear_chunk_kernel<DK, DVT, C, T, OUT, false>), grid, block, 0, stream, a, seg, dv);
+    hipLaunchKernelGGL((linear_chunk_kernel<DK, NT, WAVES, T, OUT, false, AHEAD>), grid, block, 0, stream, a, seg, dv);
 }
 
 template <int DK, typename T, int OUT>
 static void launch_columns(const LinearArgs& a, const LinearSegments& seg, int dv, hipStream_t stream) {
-    constexpr int C = parts_of<T> == 1 && DK < 256 ? 64 : 32;
-    if constexpr (DK == 256) {
-        launch<DK, 64, C, T, OUT>(a, seg, dv, stream);
-    } else {
-        if (linear_chunk_columns(DK, dv) == 64)
-            launch<DK, 64, C, T, OUT>(a, seg, dv, stream);
-        else
-            launch<DK, 128, C, T, OUT>(a, seg, dv, stream);
-    }
+    if (linear_chunk_columns(DK, dv) == 64)
+        launch<DK, 1, 4, T, OUT>(a, seg, dv, stream);
+    else if constexpr (DK == 64)
+        launch<DK, 2, 4, T, OUT>(a, seg, dv, stream);
+    else if constexpr (DK == 128 && parts_of<T> == 1)
+        launch<DK, 2, 4, T, OUT>(a, seg, dv, stream);
+    else if constexpr (DK == 128)
+        launch<DK, 1, 8, T, OUT>(a, seg, dv, stream);
 }
 
 template <int DK>

@@ -11,8 +11,8 @@ struct LinearArgs;
 
 // Segments of `length` tokens that sequences are cut into; with one there are no states.
 struct LinearSegments {
-    float* states;  // [seqs][count][heads][dk][dv] that each begins with
-    float* decays;  // [seqs][count][heads] what each keeps of it
+    float* states;  // [seqs][count][heads][dk][dv]: a sequence's own, and what each segment leaves (the first) or adds
+    float* decays;  // [seqs][count][heads] what each keeps of the state that it begins with
     int count, length;
 };
 

@@ -30,10 +30,15 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
     p.grid = (g.seqs * g.heads * (g.dv / 32) + 3) / 4;
     if (most <= 16) return true;
     p.steps = false;
-    const int64_t units = g.seqs * g.heads * (g.dv / linear_chunk_columns(g.dk, g.dv));
-    int64_t segments = 2 * cus / units;
-    if (segments > most / 256) segments = most / 256;
-    if (segments > 1) {
+    // Segments: as long as makes work for the workgroups that the CUs hold at once, two each of bf16 inputs and one of others,
+    // whose parts fill LDS, and none less than 256 tokens.  Their states cost half of the work again, so only where the
+    // longest sequence would take half as long again as that.
+    const int64_t units = g.heads * (g.dv / linear_chunk_columns(g.dk, g.dv));
+    const int64_t slots = (g.in_type == IQ4XS_TYPE_BF16 ? 2 : 1) * cus;
+    int64_t length = (g.total * units + slots - 1) / slots;
+    if (length < 256) length = 256;
+    if (2 * most > 3 * length) {
+        const int64_t segments = (most + length - 1) / length;
         p.length = (int)(((most + segments - 1) / segments + 63) / 64 * 64);
         p.segments = (int)((most + p.length - 1) / p.length);
     }
@@ -42,7 +47,7 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
         p.state_bytes = (size_t)places * g.dk * g.dv * sizeof(float);
         p.decay_bytes = ((size_t)places * sizeof(float) + 255) / 256 * 256;
     }
-    p.grid = units * p.segments;
+    p.grid = g.seqs * units * p.segments;
     return true;
 }
 
