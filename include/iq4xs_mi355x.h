@@ -439,6 +439,12 @@ int iq4xs_paged_attention(const struct iq4xs_paged_attention_args* args, void* w
 int iq4xs_paged_attention_sinks(const struct iq4xs_paged_attention_args* args, int64_t sinks, void* ws, size_t ws_bytes,
                                 void* stream);
 
+/* Whether shared tokens are gone through once for a group or again for each sequence: AUTO
+ * takes what is faster (once for few rows of each sequence over much that is shared). */
+#define IQ4XS_SHARED_AUTO 0
+#define IQ4XS_SHARED_ONCE 1
+#define IQ4XS_SHARED_EACH 2
+
 /* Sequences that begin with the same tokens, on the same pages. */
 struct iq4xs_shared_prefix {
     const int32_t* first; /* [groups + 1] first sequence of each group, never falling; NULL: one group of all */
@@ -446,23 +452,24 @@ struct iq4xs_shared_prefix {
     int64_t groups;
     int64_t most_len;  /* at least the shared tokens of any group */
     int64_t most_rows; /* at least the new tokens of a group's sequences together */
+    int32_t path;      /* IQ4XS_SHARED_* */
 };
 
 /* Bytes of workspace iq4xs_shared_attention needs; 0 also for arguments it refuses. */
 size_t iq4xs_shared_attention_workspace_bytes(const struct iq4xs_paged_attention_args* args,
                                               const struct iq4xs_shared_prefix* prefix);
 
-/* iq4xs_paged_attention of a batch whose sequences begin with the same tokens, each
- * group's read and multiplied once for the rows of all its sequences.  Tables and
- * kv_len are as there (the shared tokens among them); the shared tokens are read on
- * the pages of a group's first sequence, any number of them, with or without the end
- * of a page; a sequence of no group shares none.  args->most_kv is at least the cached
- * tokens of any sequence after its shared ones; args->window is 0 (NOT_SUPPORTED
- * otherwise: a window's calls read little of a prefix).  New tokens come after the
- * shared ones (kv_len - new >= len); what a row before their end sees of them is not
- * specified.  Where len is above most_len, the first of the shared keys count, and the
- * sequence's own keys go on after those; rows of a group past most_rows are not
- * written.  An 8-bit cache's keys of the prefix are rounded as there, by most_rows. */
+/* iq4xs_paged_attention of a batch whose sequences begin with the same tokens, those
+ * read and multiplied once for the rows of all of a group's sequences.  Tables and
+ * kv_len are as there, the shared tokens among them: any number of them, with or without
+ * the end of a page, of which every table of a group holds the same keys and values (as
+ * the same pages do); they are read through one table or another.  A sequence of no group
+ * shares none.  args->most_kv is at least the cached tokens of any sequence after its
+ * shared ones; args->window is 0 (NOT_SUPPORTED otherwise: a window's calls read little
+ * of a prefix).  New tokens come after the shared ones (kv_len - new >= len); what a row
+ * before their end sees of them is not specified.  Where len is above most_len, the rest
+ * of the shared keys are a sequence's own; rows of a group past most_rows may be left
+ * unwritten.  An 8-bit cache's keys of the prefix are rounded as there, by most_rows. */
 int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const struct iq4xs_shared_prefix* prefix,
                            void* ws, size_t ws_bytes, void* stream);
 

@@ -44,6 +44,9 @@ TYPE_BF16 = 2
 TYPE_Q8 = 3
 ROPE_HALF = 0
 ROPE_INTERLEAVED = 1
+SHARED_AUTO = 0
+SHARED_ONCE = 1
+SHARED_EACH = 2
 
 # (restype, argtypes) of every exported symbol, in header order
 _P = ctypes.c_void_p
@@ -336,7 +339,7 @@ def dequant(W, n_blocks: int, out=None):
 _CACHE = struct.Struct("@PPPPqiiii")
 _QK = struct.Struct("@PPPqqqPPPPPPPqiiiiiiif")
 _ATTENTION = struct.Struct("@PPPPPPPqqqqqqqiiiif")
-_SHARED = struct.Struct("@PPqqq")
+_SHARED = struct.Struct("@PPqqqi")
 _LINEAR = struct.Struct("@PPPPPPPPPqqqqqqqqiiiiiif")
 
 
@@ -546,22 +549,22 @@ def paged_attention(q, cache, table, starts, kv_len, most_q: int, most_kv: int, 
 
 def shared_attention(q, cache, table, starts, kv_len, shared_len, most_q: int, most_own: int, most_shared: int,
                      groups=None, most_group: int | None = None, causal: bool = True, lse: bool = False,
-                     scale: float | None = None, out_type=None):
+                     scale: float | None = None, out_type=None, path: int = SHARED_AUTO):
     """paged_attention of a batch whose sequences begin with the same tokens, on the same pages: those are read and
-    multiplied once for all of them.
+    multiplied once for all of them (path: SHARED_ONCE; again for each: SHARED_EACH; what is faster: SHARED_AUTO).
 
     groups [n + 1] (int32): first sequence of each group of sequences that share; None: one group of all.  shared_len [n]
     (int32): the tokens that a group's sequences share, which new tokens come after.  Tables and kv_len are as in
     paged_attention, the shared tokens among them.  most_own and most_shared: at least the cached tokens of any sequence
     after its shared ones, and the shared ones of any group; most_group: at least the new tokens of a group's sequences
-    together (default: all rows).  Rows of a group past most_group are left as they were allocated."""
+    together (default: all rows).  Rows of a group past most_group may be left as they were allocated."""
     torch = _torch()
     args, out, sums, here = _attention(torch, q, cache, table, starts, kv_len, most_q, most_own, causal, 0, lse, scale,
                                        out_type)
     n = 1 if groups is None else groups.numel() - 1
     gp = 0 if groups is None else _whole(groups, "groups", torch.int32, (n + 1,), here)
     prefix = _SHARED.pack(gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared,
-                          max(1, q.size(0)) if most_group is None else most_group)
+                          max(1, q.size(0)) if most_group is None else most_group, path)
     L = lib()
     nbytes = L.iq4xs_shared_attention_workspace_bytes(args, prefix)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None

@@ -233,7 +233,7 @@ hipError_t launch_sinks_attention(const iq4xs_paged_attention_args& g, int64_t s
 hipError_t shared_attention_workspace(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x, size_t* bytes) {
     SharedPlan p;
     if (!shared_plan_fits(g, x, device_cu_count(), p)) return hipErrorInvalidConfiguration;
-    *bytes = workspace_of(g, p.splits());
+    *bytes = workspace_of(g, p.parts());
     return hipSuccess;
 }
 
@@ -241,14 +241,15 @@ hipError_t launch_shared_attention(const iq4xs_paged_attention_args& g, const iq
                                    size_t ws_bytes, hipStream_t stream) {
     SharedPlan p;
     if (!shared_plan_fits(g, x, device_cu_count(), p)) return hipErrorInvalidConfiguration;
-    if (!enough(ws, ws_bytes, workspace_of(g, p.splits()))) return hipErrorInvalidValue;
+    if (!p.once) return launch_paged_attention(each_call(g, x), ws, ws_bytes, stream);
+    if (!enough(ws, ws_bytes, workspace_of(g, p.parts()))) return hipErrorInvalidValue;
     clear_launch_error();
     const iq4xs_paged_attention_args prefix = prefix_call(g, x);
-    const MoreArgs first{args_of(prefix, p.prefix, ws, p.splits()), PASS_PREFIX, 0, x.first, x.len, (int)x.groups,
+    const MoreArgs first{args_of(prefix, p.prefix, ws, p.parts()), PASS_PREFIX, 0, x.first, x.len, (int)x.groups,
                          (int)at_most(x.most_len, KEYS_END), (int)g.seqs, p.prefix.splits, p.prefix.chunk,
                          (int)x.most_rows};
     launch_rows(first, prefix, p.prefix, stream);
-    MoreArgs own{args_of(g, p.own, ws, p.splits()), PASS_OWN, 0, x.first, x.len, (int)x.groups, first.most_shared,
+    MoreArgs own{args_of(g, p.own, ws, p.parts()), PASS_OWN, 0, x.first, x.len, (int)x.groups, first.most_shared,
                  (int)g.seqs, p.prefix.splits, p.prefix.chunk, (int)x.most_rows};
     own.part += p.prefix.splits * g.total * g.q_heads * g.cache->head_dim;
     own.part_ml += p.prefix.splits * g.total * g.q_heads * 4;

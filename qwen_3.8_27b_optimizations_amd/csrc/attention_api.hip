@@ -72,6 +72,8 @@ int check_shared(const iq4xs_paged_attention_args* a, const iq4xs_shared_prefix*
     if (err != hipSuccess) return err;
     if (!x || x->groups <= 0 || x->groups >= MAX_COUNT - 64) return hipErrorInvalidValue;
     if (!x->first && x->groups != 1) return hipErrorInvalidValue;
+    if (x->path != IQ4XS_SHARED_AUTO && x->path != IQ4XS_SHARED_ONCE && x->path != IQ4XS_SHARED_EACH)
+        return hipErrorInvalidValue;
     if (a->window != 0) return hipErrorNotSupported;
     if (a->total == 0 || a->seqs == 0) return hipSuccess;
     return x->len && count(x->most_len) && count(x->most_rows) ? hipSuccess : hipErrorInvalidValue;

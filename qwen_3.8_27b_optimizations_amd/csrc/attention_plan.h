@@ -352,14 +352,50 @@ inline iq4xs_paged_attention_args prefix_call(const iq4xs_paged_attention_args& 
     return p;
 }
 
+// Each sequence by itself: a call without shared prefixes.
+inline iq4xs_paged_attention_args each_call(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x) {
+    iq4xs_paged_attention_args p = g;
+    p.most_kv = at_most(x.most_len, KEYS_END) + at_most(g.most_kv, KEYS_END);
+    return p;
+}
+
 struct SharedPlan {
-    AttentionPlan prefix, own;
-    int splits() const { return prefix.splits + own.splits; }
+    bool once;
+    AttentionPlan prefix, own;  // with `once`; the latter else each sequence's whole
+    int parts() const { return once ? prefix.splits + own.splits : own.splits > 1 ? own.splits : 0; }
 };
+
+// Once costs two more launches, each sequence by itself reads shared keys again, though from caches that hold them: 8 heads of
+// 128, one token each, fp16, 4096 shared tokens, 8, 16 and 32 sequences 29, 32, 37 us once and 21, 34, 56 each; 16384, 2, 4
+// and 64 sequences 26, 28, 74 and 22, 34, 317; 8 bits 4 heads of 256, 4 tokens each, 4096, 16 and 32 sequences 77, 81 and 66,
+// 117: from 2^26 elements of keys read again on.  Full tiles of rows are bound by their products, of which there are no
+// fewer (64 tokens of 64 heads, 16384, 8 and 16 sequences 246, 456 and 238, 444).
+inline bool shared_once(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x) {
+    if (x.path != IQ4XS_SHARED_AUTO) return x.path == IQ4XS_SHARED_ONCE;
+    const int64_t most_q = g.most_q < g.total ? g.most_q : g.total;
+    if (most_q * (g.q_heads / g.cache->heads) >= 128) return false;
+    const int64_t again = g.seqs > x.groups ? g.seqs - x.groups : 0, each = (int64_t)g.cache->heads * g.cache->head_dim;
+    return again > 0 && x.most_len > ((int64_t)1 << 26) / each / again;
+}
 
 inline bool shared_plan_fits(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x, int64_t cus,
                              SharedPlan& p) {
-    return plan_fits(prefix_call(g, x), cus, p.prefix) && plan_fits(g, cus, p.own);
+    p.once = shared_once(g, x);
+    if (!p.once) return plan_fits(each_call(g, x), cus, p.own);
+    if (!plan_fits(prefix_call(g, x), cus, p.prefix) || !plan_fits(g, cus, p.own)) return false;
+    if (p.prefix.tiles == 0 && p.prefix.splits > 1) {
+        // groups' prefixes are mostly alike: no workgroup more than the CUs hold at once, or it takes as long again (two
+        // groups of 350 rows over 8187 tokens of heads of 256, 8 bits: 264 workgroups 135 us, 240 77)
+        const int64_t rows = p.prefix.grid / p.prefix.splits, held = g.cache->head_dim == 256 ? 1 : 2;
+        int64_t splits = held * cus / rows;
+        if (splits < 1) splits = 1;
+        if (splits < p.prefix.splits) {
+            p.prefix.chunk = (int)(((x.most_len + splits - 1) / splits + 127) / 128 * 128);
+            p.prefix.splits = (int)((x.most_len + p.prefix.chunk - 1) / p.prefix.chunk);
+            p.prefix.grid = rows * p.prefix.splits;
+        }
+    }
+    return true;
 }
 
 }  // namespace iq4xs

@@ -119,7 +119,7 @@ int64_t wrong_of_shared(const Args& first, const Args& own, const iq4xs::SharedP
             iq4xs::RowParts parts = iq4xs::row_parts(own, s, lo, hi);
             parts.before = iq4xs::prefix_parts(own, iq4xs::shared_keys(own, g));
             Taken all;
-            std::vector<int> written(p.splits(), 0);
+            std::vector<int> written(p.parts(), 0);
             for (int split = 0; split < p.own.splits; ++split) {
                 Taken mine;
                 iq4xs::RowEnd end = iq4xs::ROW_NONE;
@@ -150,8 +150,8 @@ int64_t wrong_of_shared(const Args& first, const Args& own, const iq4xs::SharedP
             }
             for (int i = 0; i < parts.count(); ++i) {
                 const int part = parts.at(i);
-                ok = ok && part >= 0 && part < p.splits() && written[part] != 0;
-                if (part >= 0 && part < p.splits()) written[part] = 0;
+                ok = ok && part >= 0 && part < p.parts() && written[part] != 0;
+                if (part >= 0 && part < p.parts()) written[part] = 0;
             }
             for (int x : written) ok = ok && x != 2;  // every part with keys is joined
             const int64_t place = (int64_t)s.keys - fresh + token;
@@ -199,6 +199,7 @@ int main() {
         g.out_type = IQ4XS_TYPE_BF16;
         g.causal = (int32_t)causal;
         g.lse = lse ? &some : nullptr;
+        x.path = IQ4XS_SHARED_ONCE;
         x.first = given ? firsts.data() : nullptr;
         x.len = lens.data();
         static const int32_t table[1] = {0};

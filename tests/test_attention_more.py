@@ -34,9 +34,9 @@ def test_first_tokens_are_keys_before_the_window():
 
 
 def shared_of(pkg, **over):
-    f = dict(first=0, len=FAKE, groups=1, most_len=16, most_rows=3)
+    f = dict(first=0, len=FAKE, groups=1, most_len=16, most_rows=3, path=pkg.SHARED_ONCE)
     f.update(over)
-    return pkg._SHARED.pack(*f.values())
+    return pkg._SHARED.pack(*f.values()) + bytes(4)
 
 
 def test_the_struct_matches_the_header(pkg, tmp_path):
@@ -44,14 +44,15 @@ def test_the_struct_matches_the_header(pkg, tmp_path):
         pytest.skip("needs a host C++ compiler")
     src = tmp_path / "s.cpp"
     src.write_text('#include "iq4xs_mi355x.h"\n#include <cstdio>\nint main() { std::printf("%zu %zu", '
-                   'sizeof(iq4xs_shared_prefix), offsetof(iq4xs_shared_prefix, most_rows)); }')
+                   'sizeof(iq4xs_shared_prefix), offsetof(iq4xs_shared_prefix, path)); }')
     subprocess.run(["g++", "-I" + os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
     size, last = map(int, subprocess.run([str(tmp_path / "s")], capture_output=True, text=True).stdout.split())
-    assert (size, last + 8) == (pkg._SHARED.size,) * 2
+    assert last + 4 == pkg._SHARED.size and size >= pkg._SHARED.size
 
 
 BAD_SHARED = [dict(len=0), dict(groups=0), dict(groups=-1), dict(groups=2), dict(groups=1 << 31, first=FAKE),
-              dict(most_len=0), dict(most_len=1 << 31), dict(most_rows=0), dict(most_rows=-1)]
+              dict(most_len=0), dict(most_len=1 << 31), dict(most_rows=0), dict(most_rows=-1), dict(path=3),
+              dict(path=-1)]
 
 
 def test_refusals_before_launch(pkg):
@@ -104,6 +105,21 @@ def test_nothing_to_do_launches_nothing(pkg):
         assert L.iq4xs_paged_attention_sinks(args, 4, None, 0, None) == 0
         assert L.iq4xs_shared_attention_workspace_bytes(args, shared_of(pkg, len=0, most_len=0)) == 0
         assert L.iq4xs_shared_attention(args, shared_of(pkg, len=0), None, 0, None) == 0
+
+
+def test_each_sequence_by_itself_is_the_plain_call(pkg):
+    """And taken for little that is shared, for one sequence of a group, and for full tiles of rows."""
+    L, good = pkg.lib(), cache_of(pkg, heads=8)
+    ask = lambda f, *a: L.iq4xs_shared_attention_workspace_bytes(f, *a)  # noqa: E731
+    for seqs, new, most_len, once in ((64, 1, 16384, True), (2, 1, 100, False), (1, 1, 1 << 20, False), (3, 1, 1 << 20, True),
+                                      (64, 40, 16384, False)):
+        f = dict(hq=64, qs=64 * 128, total=seqs * new, most_q=new, seqs=seqs)
+        args = attention_args(pkg, good, most_kv=1000, **f)
+        sizes = [ask(args, shared_of(pkg, most_len=most_len, most_rows=seqs * new, path=p))
+                 for p in (pkg.SHARED_AUTO, pkg.SHARED_ONCE, pkg.SHARED_EACH)]
+        assert sizes[0] == sizes[1 if once else 2] and sizes[1] > 0, (seqs, new, most_len)
+        whole = attention_args(pkg, good, most_kv=1000 + most_len, **f)
+        assert sizes[2] == L.iq4xs_paged_attention_workspace_bytes(whole)
 
 
 def test_workspaces_hold_both_launches(pkg):

@@ -32,7 +32,7 @@ def sinks_check(pkg, dev, p, window, sinks, causal=True):
     return out, lse
 
 
-def shared_run(pkg, dev, p, firsts, lens, causal=True, most_own=None, most_shared=None, most_group=None, **kw):
+def shared_run(pkg, dev, p, firsts, lens, causal=True, most_own=None, most_shared=None, most_group=None, path=1, **kw):
     q, c, table, starts, kv_len = p.on(pkg, dev)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
     groups = firsts if firsts is not None else [0, len(p.kv)]
@@ -43,7 +43,7 @@ def shared_run(pkg, dev, p, firsts, lens, causal=True, most_own=None, most_share
     return pkg.shared_attention(q, c, table, starts, kv_len, i32(lens), max(p.new), max(own + [1]) if most_own is None else
                                 most_own, max(list(lens) + [1]) if most_shared is None else most_shared,
                                 groups=None if firsts is None else i32(firsts), most_group=most_group, causal=causal,
-                                lse=True, scale=p.scale, **kw)
+                                lse=True, scale=p.scale, path=path, **kw)
 
 
 def shared_check(pkg, dev, p, firsts, lens, causal=True, **kw):
@@ -210,7 +210,7 @@ def test_lengths_that_differ_from_what_the_call_was_told(pkg, dev):
         args = pkg._ATTENTION.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr(), c._address, table.data_ptr(),
                                    starts.data_ptr(), kv_len.data_ptr(), 8 * 128, table.shape[1], 3, 7, most_q, 60, 0, 8,
                                    pkg.TYPE_F16, pkg.TYPE_F16, 1, p.scale)
-        prefix = pkg._SHARED.pack(0, one.data_ptr(), 1, 250, most_rows)
+        prefix = pkg._SHARED.pack(0, one.data_ptr(), 1, 250, most_rows, pkg.SHARED_ONCE) + bytes(4)
         ws = torch.empty(pkg.lib().iq4xs_shared_attention_workspace_bytes(args, prefix), dtype=torch.uint8, device=dev)
         pkg.lib().check("iq4xs_shared_attention", args, prefix, ws.data_ptr(), ws.numel(),
                         torch.cuda.current_stream().cuda_stream)
@@ -224,23 +224,34 @@ def test_lengths_that_differ_from_what_the_call_was_told(pkg, dev):
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("cache,q_type", CACHES)
 def test_what_shared_calls_do_not_see_does_not_matter(pkg, dev, new, cache, q_type):
-    """Past every sequence's end, in pages of nobody, and in what the other sequences' tables hold of the prefix."""
+    """Past every sequence's end and in pages of nobody."""
     p = more.share(Problem([new + 60, new + 75, new + 51], [new] * 3, 2, 4, 128, 16, cache, q_type), [0, 3], [50])
-    clean, lse = shared_run(pkg, dev, p, None, [50])
-    more.compare(p, clean.cpu(), lse.cpu(), more.window_and_sinks(True, 0, 0))
-    mine = {(int(p.table[s, j // 16]), j % 16) for s, n in enumerate(p.kv) for j in range(n) if s == 0 or j >= 50}
-    for page in range(p.k.shape[0]):
-        for off in range(16):
-            if (page, off) in mine:
-                continue
-            for x, s in ((p.k, p.ks), (p.v, p.vs)):
-                if s is None:
-                    x[page, :, off] = math.nan if off % 2 else math.inf
-                else:
-                    x[page, :, off], s[page, :, off] = 127, math.nan if off % 2 else math.inf
-    p.table[1:, :3] = -1
-    again, lse2 = shared_run(pkg, dev, p, None, [50])
-    assert torch.equal(clean, again) and torch.equal(lse, lse2)
+    for path in (pkg.SHARED_ONCE, pkg.SHARED_EACH):
+        clean, lse = shared_run(pkg, dev, p, None, [50], path=path)
+        more.compare(p, clean.cpu(), lse.cpu(), more.window_and_sinks(True, 0, 0))
+        kept = [None if t is None else t.clone() for t in (p.k, p.v, p.ks, p.vs)]
+        mine = {(int(p.table[s, j // 16]), j % 16) for s, n in enumerate(p.kv) for j in range(n)}
+        for page in range(p.k.shape[0]):
+            for off in range(16):
+                if (page, off) in mine:
+                    continue
+                for x, s in ((p.k, p.ks), (p.v, p.vs)):
+                    if s is None:
+                        x[page, :, off] = math.nan if off % 2 else math.inf
+                    else:
+                        x[page, :, off], s[page, :, off] = 127, math.nan if off % 2 else math.inf
+        again, lse2 = shared_run(pkg, dev, p, None, [50], path=path)
+        assert torch.equal(clean, again) and torch.equal(lse, lse2)
+        p.k, p.v, p.ks, p.vs = kept
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_each_sequence_by_itself_is_the_plain_call(pkg, dev, new):
+    p = more.share(Problem([new + 400, new + 275, new + 351], [new] * 3, 2, 4, 128, 16, "f16"), [0, 3], [250])
+    want = p.run(pkg, dev)
+    for path in (pkg.SHARED_AUTO, pkg.SHARED_EACH):
+        got = shared_run(pkg, dev, p, None, [250], path=path, most_own=max(p.kv) - 250, most_shared=250)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 @pytest.mark.parametrize("new", [1, 50])
@@ -264,7 +275,7 @@ def test_graphs_streams_and_repeats(pkg, dev):
 
     def step():
         a = pkg.paged_attention(q, cache, table, starts, kv_len, 1, 500, window=100, sinks=4, lse=True)
-        b = pkg.shared_attention(q, cache, table, starts, kv_len, shared, 1, 220, 280, lse=True)
+        b = pkg.shared_attention(q, cache, table, starts, kv_len, shared, 1, 220, 280, lse=True, path=pkg.SHARED_ONCE)
         return [*a, *b]
 
     first = step()
@@ -303,6 +314,6 @@ def test_refused_tensors(pkg, dev):
                 dict(groups=torch.tensor([0, 2])), dict(groups=torch.tensor([0, 2], device=dev))):
         with pytest.raises(ValueError):
             run(**bad)
-    for bad in (dict(most_group=0), dict(scale=math.nan)):
+    for bad in (dict(most_group=0), dict(scale=math.nan), dict(path=7)):
         with pytest.raises(pkg.Iq4xsError):
             run(**bad)
