@@ -385,7 +385,7 @@ inline bool shared_plan_fits(const iq4xs_paged_attention_args& g, const iq4xs_sh
     if (!plan_fits(prefix_call(g, x), cus, p.prefix) || !plan_fits(g, cus, p.own)) return false;
     if (p.prefix.tiles == 0 && p.prefix.splits > 1) {
         // groups' prefixes are mostly alike: no workgroup more than the CUs hold at once, or it takes as long again (two
-        // groups of 350 rows over 8187 tokens of heads of 256, 8 bits: 264 workgroups 135 us, 240 77)
+        // groups of 350 rows over 8187 tokens of heads of 256, 8 bits: 264 workgroups 135 us, 240 97)
         const int64_t rows = p.prefix.grid / p.prefix.splits, held = g.cache->head_dim == 256 ? 1 : 2;
         int64_t splits = held * cus / rows;
         if (splits < 1) splits = 1;

@@ -27,7 +27,7 @@ hipError_t launch_linear_attention(const iq4xs_linear_attention_args& g, void* w
     clear_launch_error();
     const LinearArgs a = args_of(g);
     if (p.steps) {
-        launch_linear_steps(a, g.dk, g.dv, g.in_type, p.grid, stream);
+        launch_linear_steps(a, g.dk, g.dv, g.in_type, p.units, stream);
     } else {
         float* states = static_cast<float*>(ws);
         const LinearSegments segments{states, states + p.state_bytes / sizeof(float), p.segments, p.length};

@@ -234,11 +234,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
+            for (int u = 0; u < NT; ++u) S[s][t][u] = f4{0, 0, 0, 0};
+    if (from) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    S[s][t][u][r] = from ? *state_place(from, s, t, u, r) : 0.0f;
-
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[s][t][u][r] = *state_place(from, s, t, u, r);
+    }
     if constexpr (STATE_ONLY) {
         if (part == 0) {
             float* copy = segment_state(0);
@@ -303,14 +309,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
                 qn[l].parts(p);
                 store(qs, KTile::BYTES, at, p);
             }
-            kn[l].clear(row >= count);
+            if (count < C) kn[l].clear(row >= count);
             kn[l].parts(p);
             store(ks + buffer * K_BYTES, KTile::BYTES, at, p);
         }
 #pragma unroll
         for (int l = 0; l < V_LOADS; ++l) {
             const int i = threadIdx.x + l * THREADS, row = i / VTile::PIECES;
-            vn[l].clear(row >= count);
+            if (count < C) vn[l].clear(row >= count);
             if (__builtin_expect(!vn[l].finite(), 0)) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {

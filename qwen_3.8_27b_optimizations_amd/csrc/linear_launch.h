@@ -16,7 +16,8 @@ struct LinearSegments {
     int count, length;
 };
 
-void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream);
+// units: of 32 columns of a head's state.
+void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t units, hipStream_t stream);
 void launch_linear_chunks(const LinearArgs& a, const LinearSegments& segments, int dk, int dv, int type,
                           hipStream_t stream);
 

@@ -16,7 +16,7 @@ struct LinearPlan {
     bool steps;           // token by token
     int segments;         // of the longest sequence
     int length;           // tokens of a segment, a multiple of 64
-    int64_t grid;         // workgroups of the largest launch
+    int64_t units;        // of 32 columns of a head's state, token by token
     size_t state_bytes;   // states that segments begin with
     size_t decay_bytes;   // and what segments keep of them
 };
@@ -27,7 +27,7 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
     const int64_t most = g.most_q < g.total ? g.most_q : g.total;
     p = {true, 1, (int)((most + 63) / 64 * 64), 0, 0, 0};
     if (g.seqs > MOST / g.heads / 8) return false;  // 32 columns of 256 at a time
-    p.grid = (g.seqs * g.heads * (g.dv / 32) + 3) / 4;
+    p.units = g.seqs * g.heads * (g.dv / 32);
     if (most <= 16) return true;
     p.steps = false;
     // Segments: as long as makes work for the workgroups that the CUs hold at once, two each of bf16 inputs and one of others,
@@ -47,8 +47,7 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
         p.state_bytes = (size_t)places * g.dk * g.dv * sizeof(float);
         p.decay_bytes = ((size_t)places * sizeof(float) + 255) / 256 * 256;
     }
-    p.grid = g.seqs * units * p.segments;
-    return true;
+    return g.seqs * units <= MOST / p.segments;
 }
 
 }  // namespace iq4xs

@@ -12,7 +12,7 @@
 
 namespace iq4xs {
 
-constexpr int STEP_COLUMNS = 32, STEP_WAVES = 4;
+constexpr int STEP_COLUMNS = 32, STEP_WAVES = 4;  // of a workgroup at most
 
 // N consecutive elements as fp32.
 template <int N, typename T>
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void linear_step_kernel(LinearArgs
     constexpr int N = DK / 8;  // rows of a lane
     const int lane = threadIdx.x % 64, column = 4 * (lane % 8), row0 = N * (lane / 8);
     const int tiles = dv / STEP_COLUMNS;
-    const int64_t unit = (int64_t)blockIdx.x * STEP_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t unit = (int64_t)blockIdx.x * (blockDim.x / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if (unit >= (int64_t)a.seqs * a.heads * tiles) return;
     const int tile = (int)(unit % tiles), head = (int)(unit / tiles % a.heads), seq = (int)(unit / tiles / a.heads);
     const Rows rows = rows_of(a, seq);
@@ -80,8 +80,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void linear_step_kernel(LinearArgs
 }
 
 template <int DK>
-static void launch_types(const LinearArgs& a, int dv, int type, dim3 grid, hipStream_t stream) {
-    const dim3 block(64 * STEP_WAVES);
+static void launch_types(const LinearArgs& a, int dv, int type, dim3 grid, dim3 block, hipStream_t stream) {
     if (type == IQ4XS_TYPE_F32)
         hipLaunchKernelGGL((linear_step_kernel<DK, float>), grid, block, 0, stream, a, dv);
     else if (type == IQ4XS_TYPE_F16)
@@ -90,14 +89,16 @@ static void launch_types(const LinearArgs& a, int dv, int type, dim3 grid, hipSt
         hipLaunchKernelGGL((linear_step_kernel<DK, __bf16>), grid, block, 0, stream, a, dv);
 }
 
-void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t grid, hipStream_t stream) {
-    const dim3 blocks((unsigned)grid);
+void launch_linear_steps(const LinearArgs& a, int dk, int dv, int type, int64_t units, hipStream_t stream) {
+    // a wave by itself while that makes no more workgroups than a few to a CU, so that all CUs load
+    const int waves = units <= 1024 ? 1 : STEP_WAVES;
+    const dim3 blocks((unsigned)((units + waves - 1) / waves)), block(64 * waves);
     if (dk == 64)
-        launch_types<64>(a, dv, type, blocks, stream);
+        launch_types<64>(a, dv, type, blocks, block, stream);
     else if (dk == 128)
-        launch_types<128>(a, dv, type, blocks, stream);
+        launch_types<128>(a, dv, type, blocks, block, stream);
     else
-        launch_types<256>(a, dv, type, blocks, stream);
+        launch_types<256>(a, dv, type, blocks, block, stream);
 }
 
 }  // namespace iq4xs
