@@ -400,6 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         if (__builtin_expect(was_odd, 0)) {
             for (int i = threadIdx.x; i < DVT; i += THREADS) odd_from[parity ^ 1][i] = C;
             if (threadIdx.x == 0) odd[parity ^ 1] = 0;
+            if (STATE_ONLY) __syncthreads();  // before the next chunk says which of its values are; else below
         }
         f4 O[IT][NT];
         if constexpr (!STATE_ONLY) {

@@ -28,11 +28,15 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
     p = {true, 1, (int)((most + 63) / 64 * 64), 0, 0, 0};
     if (g.seqs > MOST / g.heads / 8) return false;  // 32 columns of 256 at a time
     p.units = g.seqs * g.heads * (g.dv / 32);
-    if (most <= 16) return true;
+    // Token by token while that is no slower: a chunk's work hardly grows with its tokens, a step's does (64 sequences of 64
+    // heads of 128 x 128, of 4, 8 and 16 tokens: bf16 115, 153 and 239 us in steps and 111, 113 and 117 in a chunk, fp16 111,
+    // 153, 237 and 158, 161, 163, fp32 124, 169, 268 and 179, 183, 195; one sequence 10, 11, 18 and 11 to 14).
+    if (most <= (g.in_type == IQ4XS_TYPE_BF16 ? 4 : 8)) return true;
     p.steps = false;
     // Segments: as long as makes work for the workgroups that the CUs hold at once, two each of bf16 inputs and one of others,
-    // whose parts fill LDS, and none less than 256 tokens.  Their states cost half of the work again, so only where the
-    // longest sequence would take half as long again as that.
+    // whose parts fill LDS, and none less than 256 tokens (4096 tokens of 64 heads, bf16: 8 segments 117 us, 4 160, 11 153).
+    // Their states cost half of the work again, so only where the longest sequence would take half as long again as that
+    // (5 prompts of 987 to 4001 tokens, fp16: 474 us whole, 660 in up to 3 segments).
     const int64_t units = g.heads * (g.dv / linear_chunk_columns(g.dk, g.dv));
     const int64_t slots = (g.in_type == IQ4XS_TYPE_BF16 ? 2 : 1) * cus;
     int64_t length = (g.total * units + slots - 1) / slots;
@@ -44,6 +48,7 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
     }
     if (p.segments > 1) {
         const int64_t places = g.seqs * p.segments * g.heads;
+        if (g.seqs * g.heads > MOST / 64) return false;  // the launch that joins them: 1024 elements of 256 x 256 each
         p.state_bytes = (size_t)places * g.dk * g.dv * sizeof(float);
         p.decay_bytes = ((size_t)places * sizeof(float) + 255) / 256 * 256;
     }

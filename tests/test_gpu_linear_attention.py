@@ -176,6 +176,22 @@ def test_what_is_not_finite_stays_where_it_belongs(pkg, dev, kind, value, n, at)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [160, 1400])
+def test_values_that_are_not_finite_in_chunk_after_chunk(pkg, dev, kind, n):
+    """Each in a channel of its own, several in one chunk, in every segment: every channel from its token on."""
+    p = Problem(dev, [n], 2, 1, 128, 128, kind, each=False)
+    clean, states = p.run(pkg)
+    allowed, rest = torch.zeros_like(clean, dtype=torch.bool), torch.zeros_like(states, dtype=torch.bool)
+    for c, t in enumerate([3, 31, 32, 33, 63, 64, 70, 95, 97, 128, 130, n // 2, n // 2 + 1, n - 40, n - 2, n - 1]):
+        p.v[t, 1, 8 * c + c % 8] = math.nan if c % 2 else math.inf
+        allowed[t:, 1, 8 * c + c % 8] = True
+        rest[p.dst[0], 1, :, 8 * c + c % 8] = True
+    out, s = p.run(pkg)
+    assert torch.equal(out[~allowed], clean[~allowed]) and not bool(torch.isfinite(out[allowed]).any())
+    assert torch.equal(s[~rest], states[~rest]) and not bool(torch.isfinite(s[rest]).any())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("lens", [[1, 1], [70, 5], [800, 130]])
 def test_rows_of_no_sequence(pkg, dev, kind, lens):
     """NaN before the first and behind the last: not a bit changes, and those outputs are not written."""
