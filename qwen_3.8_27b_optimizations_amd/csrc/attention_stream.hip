@@ -26,6 +26,10 @@
 // that this rounding is left, and that of weights below 2^-21 of the largest, whose second part is below fp16's normal
 // range (2^-32 of the largest each).  bf16 queries for it become fp16 with a power of
 // two taken out of each row, exact down to 2^-14 of the row's largest element.
+//
+// First tokens beside a window are further steps before those of the window, of the first split, with masks of their own: 64
+// sequences of up to 32768 tokens, window 4096, 4 first tokens, 64 heads on 8 of 128, bf16: 155 us, 5.2 TB/s; 8 x 5 tokens
+// over a window of 2048 and 64 first tokens, 8-bit heads of 256: 37 us.
 #include "attention_core.h"
 #include "attention_internal.h"
 #include "iq4xs_internal.h"

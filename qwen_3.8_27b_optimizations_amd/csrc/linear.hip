@@ -1,4 +1,4 @@
-// linear.hip -- linear attention with a decay for each head: which kernel takes a call.
+// linear.hip -- linear attention with a decay for each head: a call's launches (by linear_plan.h).
 #include "iq4xs_internal.h"
 #include "linear_device.h"
 #include "linear_internal.h"

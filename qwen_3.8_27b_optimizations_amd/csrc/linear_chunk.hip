@@ -3,6 +3,29 @@
 // With G the sum of decays from a chunk's beginning and S the state there,
 //   o_i = scale (exp(G_i) q_i^T S + sum_{j <= i} exp(G_i - G_j) (q_i k_j) v_j)
 //   S  <- exp(G_C) S + sum_j exp(G_C - G_j) k_j v_j^T
+//
+// Four products of 16 x 16 x 32 on matrix units for each chunk of 32 tokens.  States and sums are fp32 and inputs 16 bits, so
+// what is fp32 (the state, values times their weights, weighted scores, fp32 inputs) goes as a sum of bf16 parts, which
+// have fp32's range: three for the state's update and fp32 outputs, two for what makes 16-bit outputs.  Exponents of
+// weights are differences of 64-bit sums, since a large decay would take the bits of the small ones behind it.
+// - A workgroup has DK x 64 or DK x 128 of a head's state in accumulators through all chunks of its segment; a wave has whole
+//   columns, so that only weighted scores pass between waves.  The state's accumulators hold, in each lane, 8 rows of a
+//   column: the left operand of S^T Q^T as they stand, and values read as columns serve V^T P^T and the update alike.
+// - LDS holds queries once, keys and values twice: the next chunk goes in beside this one's products (where three parts
+//   have no room for that, after them).  Two waits of the workgroup for each chunk.
+// - Decays do not touch the accumulators until they come to 2^-40: they are in the scales of what is read and added.  These
+//   scales are made for as many chunks as there are waves at a time, a chunk to a wave.
+// - A long sequence is cut into segments side by side: a first pass leaves what each adds to the state, a launch joins them,
+//   and the second pass begins with the states.
+// Bound by vector instructions (parts of the state and of the weighted values: about as many issue cycles as the products
+// take) and by the chain read, multiply, exchange, multiply, wait of each chunk, with two waves to a SIMD to hide it.
+// Measured: 4096 tokens, 64 heads of 128 x 128 on 16 of q and k, bf16: 117 us (39 for the states, 10 to join them, 79), of
+// which memory takes 34; a chunk 2.1 us of a CU.  5 prompts of 987 to 4001 tokens, 32 heads of 128 x 256, fp16 to fp32: 474
+// us, 1.8 TB/s.  Slower or no faster: chunks of 64 tokens (an earlier second pass 82 us for 70: registers), one tile of
+// columns on eight waves for bf16 (77 and 79), three workgroups to a CU (87), single buffers (490 and 474 us of the prompts),
+// scales by one wave a chunk ahead (as fast alone, but the pass over states waits for it), fp16 inputs as they are with
+// the state in fp16's range (500 us: keeping the range costs what the parts do), sums of earlier segments in each
+// workgroup instead of a launch that joins (96 against 64 + 12 us).
 #include "attention_core.h"
 #include "iq4xs_internal.h"
 #include "lds_device.h"
@@ -628,7 +651,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
                     *state_place(to, s, t, u, r) = S[s][t][u][r] * by;
 }
 
-// The states that segments begin with, in the place of what each adds, from the third on.
+// The states that segments begin with, in the place of what each adds, from the third on.  Bound by memory: 16 bytes read and
+// 16 written of a piece, all segments' reads on their way at once (7 segments of 4 MiB: 10 us, 5.6 TB/s).
 __global__ __launch_bounds__(256) void join_segments_kernel(LinearArgs a, LinearSegments seg, int size) {
     const int pieces = size / 4;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -6,6 +6,8 @@
 // of a head's state into registers, 4 in each of 8 lanes by dk / 8 rows, so that a row's 32 columns are a whole line of
 // 128 bytes; columns do not meet, so waves need no LDS and no barrier.  q and k of the lane's rows and v of its columns are
 // fetched a token ahead; what the 8 lanes of a column have of q^T S is added in three exchanges.
+// Measured: 64 sequences of 64 heads of 128 x 128, fp32, one token: 99 us, 5.5 TB/s (a large copy 5.1); one sequence 5.0 us
+// (5.6 with four waves to a workgroup, 64 of 256 CUs), a chain of dependent loads.
 #include "iq4xs_internal.h"
 #include "linear_device.h"
 #include "linear_launch.h"
