@@ -469,7 +469,8 @@ size_t iq4xs_shared_attention_workspace_bytes(const struct iq4xs_paged_attention
  * of a prefix).  New tokens come after the shared ones (kv_len - new >= len); what a row
  * before their end sees of them is not specified.  Where len is above most_len, the rest
  * of the shared keys are a sequence's own; rows of a group past most_rows may be left
- * unwritten.  An 8-bit cache's keys of the prefix are rounded as there, by most_rows. */
+ * unwritten.  Once, an 8-bit cache's keys of the prefix are rounded as there, by
+ * most_rows. */
 int iq4xs_shared_attention(const struct iq4xs_paged_attention_args* args, const struct iq4xs_shared_prefix* prefix,
                            void* ws, size_t ws_bytes, void* stream);
 

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     const Rows all = rows_of(a, seq);
     const int begin = part * seg.length;
     if (begin >= all.count) return;
-    const bool last = begin + seg.length >= all.count;
+    const bool last = all.count - begin <= seg.length;
     if (STATE_ONLY && last) return;
     const int end = last ? all.count : begin + seg.length;
 
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(256) void join_segments_kernel(LinearArgs a, Linear
     const int piece = (int)(at % pieces), head = (int)(at / pieces % a.heads), seq = (int)(at / pieces / a.heads);
     if (seq >= a.seqs) return;
     const Rows all = rows_of(a, seq);
-    const int count = (all.count + seg.length - 1) / seg.length;
+    const int count = (int)((all.count + (int64_t)seg.length - 1) / seg.length);
     if (count < 3) return;
     const int64_t first = (int64_t)seq * seg.count * a.heads + head;
     f4* p = reinterpret_cast<f4*>(seg.states + first * size + 4 * piece);

@@ -25,7 +25,7 @@ struct LinearPlan {
 inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, LinearPlan& p) {
     constexpr int64_t MOST = 0x7FFFFFFF;
     const int64_t most = g.most_q < g.total ? g.most_q : g.total;
-    p = {true, 1, (int)((most + 63) / 64 * 64), 0, 0, 0};
+    p = {true, 1, (int)(most < MOST - 63 ? (most + 63) / 64 * 64 : MOST), 0, 0, 0};  // one segment: as long as any sequence
     if (g.seqs > MOST / g.heads / 8) return false;  // 32 columns of 256 at a time
     p.units = g.seqs * g.heads * (g.dv / 32);
     // Token by token while that is no slower: a chunk's work hardly grows with its tokens, a step's does (64 sequences of 64

@@ -88,3 +88,37 @@ def test_the_struct_matches_the_header(pkg, tmp_path):
     subprocess.run(["g++", "-I" + os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
     size, scale = map(int, subprocess.run([str(tmp_path / "s")], capture_output=True, text=True).stdout.split())
     assert scale + 4 == pkg._LINEAR.size and size >= pkg._LINEAR.size
+
+
+PLAN = """
+#include "linear_plan.h"
+#include <initializer_list>
+#include <cstdio>
+int main() {
+    const long long most = 0x7FFFFFFF, lengths[] = {5, 9, 17, 300, 4096, 1 << 30, most - 64, most - 63, most - 1, most};
+    for (long long heads : {1LL, 64LL, 1LL << 15}) for (long long seqs : {1LL, 5LL, 1000LL}) for (long long total : lengths)
+        for (long long most_q : lengths) for (int type = 0; type < 3; ++type) {
+            iq4xs_linear_attention_args g = {};
+            g.seqs = seqs, g.total = total, g.most_q = most_q, g.heads = heads, g.dk = g.dv = 128, g.in_type = type;
+            iq4xs::LinearPlan p;
+            if (!iq4xs::linear_plan(g, 256, p) || p.steps) continue;
+            const long long longest = most_q < total ? most_q : total;
+            if (p.length < 1 || p.segments < 1 || p.segments > 514 || (long long)p.length * p.segments < longest ||
+                (long long)p.length * (p.segments - 1) >= longest || (p.segments > 1 && p.length % 64 != 0))
+                std::printf("%lld %lld %lld %lld %d\\n", heads, seqs, total, most_q, type);
+        }
+}
+"""
+
+
+def test_segments_hold_the_longest_sequence(pkg, tmp_path):
+    """Up to the longest that a call may name: none empty, no more than the chip holds at once and what they round up to."""
+    if shutil.which("g++") is None:
+        pytest.skip("needs a host C++ compiler")
+    src = tmp_path / "s.cpp"
+    src.write_text(PLAN)
+    subprocess.run(["g++", "-std=c++17", "-I" + os.path.join(ROOT, "include"),
+                    "-I" + os.path.join(ROOT, "qwen_3.8_27b_optimizations_amd", "csrc"), str(src), "-o", str(tmp_path / "s")],
+                   check=True)
+    r = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True)
+    assert r.stdout == ""
