@@ -292,8 +292,9 @@ inline AttentionPlan plan_of(const iq4xs_paged_attention_args& g, int64_t cus) {
     else
         p.tiles = rows <= 16 || (codes && (wide || (rows > 32 && rows <= 48))) ? 1 : 2;
     const int64_t tile = p.tiles ? 16 * p.tiles : 128, row_tiles = (most_q * group + tile - 1) / tile;
-    // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32
-    int64_t span = g.most_kv;
+    // the keys of a sequence that some row sees; a window's first key lies anywhere in a step of 32.  No more than count: a
+    // call may name lengths whose splits, rounded up to 128 keys, are no ints.
+    int64_t span = most_kv_of(g);
     const int64_t window = window_of(g);
     if (window > 0 && window + most_q + 32 < span) span = window + most_q + 32;
     const int64_t pairs = g.seqs * g.cache->heads * row_tiles;
@@ -353,7 +354,7 @@ inline iq4xs_paged_attention_args prefix_call(const iq4xs_paged_attention_args& 
     iq4xs_paged_attention_args p = g;
     p.seqs = x.groups;
     p.most_q = x.most_rows;
-    p.most_kv = x.most_len;
+    p.most_kv = at_most(x.most_len, KEYS_END);
     p.causal = 0;
     return p;
 }
@@ -396,8 +397,9 @@ inline bool shared_plan_fits(const iq4xs_paged_attention_args& g, const iq4xs_sh
         int64_t splits = held * cus / rows;
         if (splits < 1) splits = 1;
         if (splits < p.prefix.splits) {
-            p.prefix.chunk = (int)(((x.most_len + splits - 1) / splits + 127) / 128 * 128);
-            p.prefix.splits = (int)((x.most_len + p.prefix.chunk - 1) / p.prefix.chunk);
+            const int64_t keys = at_most(x.most_len, KEYS_END);
+            p.prefix.chunk = (int)(((keys + splits - 1) / splits + 127) / 128 * 128);
+            p.prefix.splits = (int)((keys + p.prefix.chunk - 1) / p.prefix.chunk);
             p.prefix.grid = rows * p.prefix.splits;
         }
     }
