@@ -343,6 +343,11 @@ _SHARED = struct.Struct("@PPqqqi")
 _LINEAR = struct.Struct("@PPPPPPPPPqqqqqqqqiiiiiif")
 
 
+def _block(layout, *fields) -> bytes:
+    """A C struct with what pads it behind its last field: the library may copy all of it."""
+    return layout.pack(*fields) + bytes(-layout.size % 8)
+
+
 _TYPES = {}  # torch dtype -> TYPE_*, filled once a GPU has been seen
 
 
@@ -516,9 +521,9 @@ def _attention(torch, q, cache, table, starts, kv_len, most_q, most_kv, causal, 
     lp = _whole(kv_len, "kv_len", torch.int32, (seqs,), here)
     out = q.new_empty((total, hq, d), dtype=out_type)
     sums = q.new_empty((total, hq), dtype=torch.float32) if lse else None
-    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), sums.data_ptr() if lse else 0, cache._address, tp, sp, lp,
-                           q_stride, width, seqs, total, most_q, most_kv, window, hq, kind, types[out_type],
-                           bool(causal), d ** -0.5 if scale is None else scale)
+    args = _block(_ATTENTION, q.data_ptr(), out.data_ptr(), sums.data_ptr() if lse else 0, cache._address, tp, sp, lp,
+                  q_stride, width, seqs, total, most_q, most_kv, window, hq, kind, types[out_type], bool(causal),
+                  d ** -0.5 if scale is None else scale)
     return args, out, sums, here
 
 
@@ -563,8 +568,8 @@ def shared_attention(q, cache, table, starts, kv_len, shared_len, most_q: int, m
                                        out_type)
     n = 1 if groups is None else groups.numel() - 1
     gp = 0 if groups is None else _whole(groups, "groups", torch.int32, (n + 1,), here)
-    prefix = _SHARED.pack(gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared,
-                          max(1, q.size(0)) if most_group is None else most_group, path)
+    prefix = _block(_SHARED, gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared,
+                    max(1, q.size(0)) if most_group is None else most_group, path)
     L = lib()
     nbytes = L.iq4xs_shared_attention_workspace_bytes(args, prefix)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
@@ -609,9 +614,9 @@ def linear_attention(q, k, v, decay, starts, most_q: int, states=None, from_slot
     fp = 0 if from_slots is None else _whole(from_slots, "from_slots", torch.int64, (seqs,), here)
     tp = 0 if to_slots is None else _whole(to_slots, "to_slots", torch.int64, (seqs,), here)
     out = q.new_empty((total, heads, dv), dtype=out_type)
-    args = _LINEAR.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dp, sp, xp, fp, tp, out.data_ptr(), q_stride, k_stride,
-                        v_stride, heads if each else 0, slots, seqs, total, most_q, heads, hk, dk, dv, types[kind],
-                        types[out_type], scale)
+    args = _block(_LINEAR, q.data_ptr(), k.data_ptr(), v.data_ptr(), dp, sp, xp, fp, tp, out.data_ptr(), q_stride, k_stride,
+                  v_stride, heads if each else 0, slots, seqs, total, most_q, heads, hk, dk, dv, types[kind],
+                  types[out_type], scale)
     L = lib()
     nbytes = L.iq4xs_linear_attention_workspace_bytes(args)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None

@@ -63,3 +63,14 @@ def compiled(tmp_path_factory):
 def test_plans_of_the_longest_lengths(compiled):
     """`At least` so many tokens, up to the largest number: splits hold every key that counts, and none is empty."""
     assert compiled(PLAN) == ""
+
+
+def test_blocks_are_whole_structs(pkg, compiled):
+    """What the Python side passes is as long as the struct, padding and all: the library copies it."""
+    sizes = compiled('#include "iq4xs_mi355x.h"\n#include <cstdio>\nint main() { std::printf("%zu %zu %zu", '
+                     "sizeof(iq4xs_paged_attention_args), sizeof(iq4xs_shared_prefix), sizeof(iq4xs_linear_attention_args)); }")
+    layouts = (pkg._ATTENTION, pkg._SHARED, pkg._LINEAR)
+    blocks = [pkg._block(x, *x.unpack(bytes(x.size))) for x in layouts]
+    assert [len(b) for b in blocks] == [int(n) for n in sizes.split()]
+    source = open(pkg.__file__).read()
+    assert all(f"_{name}.pack(" not in source for name in ("ATTENTION", "SHARED", "LINEAR"))
