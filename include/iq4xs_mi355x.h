@@ -450,7 +450,7 @@ struct iq4xs_shared_prefix {
     const int32_t* first; /* [groups + 1] first sequence of each group, never falling; NULL: one group of all */
     const int32_t* len;   /* [groups] tokens that the sequences of a group share */
     int64_t groups;
-    int64_t most_len;  /* at least the shared tokens of any group */
+    int64_t most_len;  /* at least the shared tokens of any group, and 1 */
     int64_t most_rows; /* at least the new tokens of a group's sequences together */
     int32_t path;      /* IQ4XS_SHARED_* */
 };

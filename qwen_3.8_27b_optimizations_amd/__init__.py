@@ -561,14 +561,14 @@ def shared_attention(q, cache, table, starts, kv_len, shared_len, most_q: int, m
     groups [n + 1] (int32): first sequence of each group of sequences that share; None: one group of all.  shared_len [n]
     (int32): the tokens that a group's sequences share, which new tokens come after.  Tables and kv_len are as in
     paged_attention, the shared tokens among them.  most_own and most_shared: at least the cached tokens of any sequence
-    after its shared ones, and the shared ones of any group; most_group: at least the new tokens of a group's sequences
+    after its shared ones, and the shared ones of any group (0 if no group shares any); most_group: at least the new tokens of a group's sequences
     together (default: all rows).  Rows of a group past most_group may be left as they were allocated."""
     torch = _torch()
     args, out, sums, here = _attention(torch, q, cache, table, starts, kv_len, most_q, most_own, causal, 0, lse, scale,
                                        out_type)
     n = 1 if groups is None else groups.numel() - 1
     gp = 0 if groups is None else _whole(groups, "groups", torch.int32, (n + 1,), here)
-    prefix = _block(_SHARED, gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared,
+    prefix = _block(_SHARED, gp, _whole(shared_len, "shared_len", torch.int32, (n,), here), n, most_shared or 1,
                     max(1, q.size(0)) if most_group is None else most_group, path)
     L = lib()
     nbytes = L.iq4xs_shared_attention_workspace_bytes(args, prefix)
