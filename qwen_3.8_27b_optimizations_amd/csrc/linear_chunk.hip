@@ -13,8 +13,10 @@
 //   column: the left operand of S^T Q^T as they stand, and values read as columns serve V^T P^T and the update alike.
 // - LDS holds queries once, keys and values twice: the next chunk goes in beside this one's products (where three parts
 //   have no room for that, after them).  Two waits of the workgroup for each chunk.
-// - Decays do not touch the accumulators until they come to 2^-40: they are in the scales of what is read and added.  These
-//   scales are made for as many chunks as there are waves at a time, a chunk to a wave.
+// - The accumulators hold the state itself, multiplied by its decay beside the products of each chunk's update, so that what
+//   fits fp32 fits here.  (Decays kept in the scales of what is read and added, up to 2^40, save no time: 114 us either way
+//   for the 4096 tokens below; large values overflowed.)  Scales are made for as many chunks as there are waves at a time,
+//   a chunk to a wave.
 // - A long sequence is cut into segments side by side: a first pass leaves what each adds to the state, a launch joins them,
 //   and the second pass begins with the states.
 // Bound by vector instructions (parts of the state and of the weighted values: about as many issue cycles as the products
@@ -182,10 +184,10 @@ __device__ inline void store8(void* p, int type, f4 x, f4 y) {
 // What a chunk's decays come to.
 template <int C>
 struct ChunkScales {
-    double sum[C];         // of decays up to a token, times log2(e)
-    float from_start[C];   // of the state in an output: 2^sum, the output's scale, and 2^held as the chunk begins
-    float to_end[C];       // of a token in the state: 2^(whole - sum), and 2^-held as it ends
-    float again;           // what the accumulators are multiplied by before the chunk's tokens come to them
+    double sum[C];        // of decays up to a token, times log2(e)
+    float from_start[C];  // of the state in an output: 2^sum and the output's scale
+    float to_end[C];      // of a token in the state: 2^(whole - sum)
+    float whole;          // of the state before the chunk's tokens come to it: 2^whole
 };
 
 // DK by 16 NT WAVES of a head's state belong to a workgroup, 16 NT columns to a wave, in accumulators.  OUT: parts of the
@@ -207,7 +209,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     __shared__ __attribute__((aligned(1024))) uint8_t vs[BUFFERS * V_BYTES];
     __shared__ __attribute__((aligned(1024))) uint8_t ps[STATE_ONLY ? 1024 : OUT * PTile::BYTES];
     __shared__ ChunkScales<C> scales[WAVES];  // of as many chunks at a time
-    __shared__ double wholes[WAVES];
     __shared__ int odd[2], odd_from[2][DVT];  // whether values are not finite, and a channel's first token of such
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int n = lane % 16, j = lane / 16;
@@ -354,10 +355,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         }
     };
 
-    // What the accumulators hold is the state times 2^-held: decays of many chunks go into the scales of what is added and
-    // read, and into the accumulators only when they pass 2^40.  The scales of the next chunks, one to a wave (scanning the
-    // decays of one chunk after another would keep the other waves waiting for the one that does).
-    double held = 0.0, decayed = 0.0;  // and of the segment so far, times log2(e)
+    // The scales of the next chunks, one to a wave (scanning the decays of one chunk after another would keep the other
+    // waves waiting for the one that does).
     float gn;
     auto decays = [&](int chunk) {  // of the wave's chunk of those from `chunk` on, ahead of their use
         const int i = chunk + C * wave + lane % C;
@@ -368,30 +367,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         const int mine = chunk + C * wave;
         // decays below -200 are zeros beside any fp32 number, and sums of them keep their bits; a NaN stays
         const double g = running_sum(mine + lane < end ? (double)(gn < -200.0f ? -200.0f : gn) * 1.4426950408889634 : 0.0);
-        if (lane == C - 1) wholes[wave] = g;
-        __syncthreads();
-        double before = 0.0, after = 0.0, whole = 0.0;  // held around the wave's chunk
-        float by = 1.0f;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            const double x = wholes[i];
-            if (i == wave) before = held, whole = x;
-            held += x;
-            decayed += x;
-            const bool over = !(fabs(held) < 40.0);
-            if (i == wave && over) by = exp2_of(held);
-            if (over) held = 0.0;
-            if (i == wave) after = held;
-        }
+        const u2 w = __builtin_bit_cast(u2, g);
+        const double whole = __builtin_bit_cast(double, u2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, C - 1),
+                                                           (uint32_t)__builtin_amdgcn_readlane((int)w.y, C - 1)});
         ChunkScales<C>& to = scales[wave];
         if (lane < C) {
             to.sum[lane] = g;
-            to.from_start[lane] = __builtin_amdgcn_exp2f((float)g) * (a.scale * exp2_of(before));
-            to.to_end[lane] = __builtin_amdgcn_exp2f((float)(whole - g)) * exp2_of(-after);
+            to.from_start[lane] = exp2_of(g) * a.scale;
+            to.to_end[lane] = exp2_of(whole - g);
         }
-        if (lane == 0) to.again = by;
+        if (lane == 0) to.whole = exp2_of(whole);
         decays(chunk + C * WAVES);
     };
+    double decayed = 0.0;  // sum of the segment's decays so far, times log2(e)
 
     const uint32_t out_bytes = a.out_type == IQ4XS_TYPE_F32 ? 4 : 2;
     for (int i = threadIdx.x; i < 2 * DVT; i += THREADS) odd_from[i / DVT][i % DVT] = C;
@@ -527,7 +515,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
             for (int p = 0; p < IN; ++p) V[u][p] = eight_tokens<VTile>(v_column + v_buffer + 8 * u + p * VTile::BYTES);
         const bool some_odd = odd[parity] != 0;
         float w[8];
-        const float again = sc.again;
+        const float whole = sc.whole;
+        if constexpr (STATE_ONLY) decayed += sc.sum[C - 1];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = sc.to_end[8 * j + e];
         u4 y[IT][OUT];
@@ -550,14 +539,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
                         for (int u = 0; u < NT; ++u)
                             if (p + o < OUT) O[i][u] = Matrix<__bf16>::mma16(V[u][o], y[i][p], O[i][u]);
         }
-        if (__builtin_expect(again != 1.0f, 0)) {
+        auto decay = [&](int s) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) S[s][h][u] *= again;
-        }
+                for (int u = 0; u < NT; ++u) S[s][h][u] *= whole;
+        };
         // values times what is left of them at the chunk's end, and the state's update
         u4 W[NT][3];
 #pragma unroll
@@ -579,6 +566,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         for (int s = 0; s < KS; ++s) {
             if (s + 1 < KS) keys(s + 1);
             __builtin_amdgcn_sched_barrier(0);
+            if (s == 0) decay(0);
+            if (s + 1 < KS) decay(s + 1);
 #pragma unroll
             for (int o = 2; o >= 0; --o)
 #pragma unroll
@@ -638,8 +627,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
                 : last     ? state_at(a, a.to_slots, seq, head, DK * dv)
                            : nullptr;
     if (!to) return;
-    // the scales of chunks past the last one are those of no decay
-    const float by = exp2_of(held);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -648,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
             for (int u = 0; u < NT; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    *state_place(to, s, t, u, r) = S[s][t][u][r] * by;
+                    *state_place(to, s, t, u, r) = S[s][t][u][r];
 }
 
 // The states that segments begin with, in the place of what each adds, from the third on.  Bound by memory: 16 bytes read and
