@@ -510,6 +510,7 @@ size_t iq4xs_linear_attention_workspace_bytes(const struct iq4xs_linear_attentio
  * keep 24 bits of states, updates and fp32 inputs (16 of what makes 16-bit outputs).
  * Sums of products with a query are taken before the decays of up to 31 tokens: with
  * the state that far back and with those tokens' keys they have to fit fp32 as well.
+ * Decays above 0 let states grow: within 32 tokens, by less than 2^127.
  * Two sequences must not have one to_slot, nor one's to_slot be another's from_slot;
  * a sequence's own two may be one, and several may begin at one state.
  * A sequence of more than most_q tokens is cut to its first most_q; rows past them and

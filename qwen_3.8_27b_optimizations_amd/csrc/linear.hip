@@ -30,7 +30,9 @@ hipError_t launch_linear_attention(const iq4xs_linear_attention_args& g, void* w
         launch_linear_steps(a, g.dk, g.dv, g.in_type, p.units, stream);
     } else {
         float* states = static_cast<float*>(ws);
-        const LinearSegments segments{states, states + p.state_bytes / sizeof(float), p.segments, p.length};
+        static_assert(sizeof(SegmentDecay) == SEGMENT_DECAY_BYTES, "as the workspace counts them");
+        const LinearSegments segments{states, reinterpret_cast<SegmentDecay*>(states + p.state_bytes / sizeof(float)),
+                                      p.segments, p.length};
         launch_linear_chunks(a, segments, g.dk, g.dv, g.in_type, stream);
     }
     return hipGetLastError();

@@ -153,10 +153,14 @@ __device__ inline double running_sum(double x) {
     return plus_moved<0x143, 0xC>(x);  // and the last of 32 to the next 32
 }
 
-// 2^x where x is large: its whole part apart, so that the rest keeps its bits.
+// 2^x where x is large: its whole part apart, so that the rest keeps its bits, and `part` in (1/2, 1].
+__device__ inline SegmentDecay exp2_parts(double x) {
+    const double whole = ceil(x);
+    return {__builtin_amdgcn_exp2f((float)(x - whole)), (int)fmin(fmax(whole, -10000.0), 10000.0)};
+}
 __device__ inline float exp2_of(double x) {
-    const double whole = rint(x);
-    return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)whole);
+    const SegmentDecay d = exp2_parts(x);
+    return ldexpf(d.part, d.exponent);
 }
 
 // Four tokens of the lane's channel and the four after them, as the left or right operand of a product over tokens.
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     }
 
     if (STATE_ONLY && tile == 0 && threadIdx.x == 0)
-        seg.decays[(seq * seg.count + part) * (int64_t)a.heads + head] = exp2_of(decayed);
+        seg.decays[(seq * seg.count + part) * (int64_t)a.heads + head] = exp2_parts(decayed);
     float* to = STATE_ONLY ? seg.states + ((int64_t)(seq * seg.count + part + 1) * a.heads + head) * DK * dv
                 : last     ? state_at(a, a.to_slots, seq, head, DK * dv)
                            : nullptr;
@@ -654,7 +658,11 @@ __global__ __launch_bounds__(256) void join_segments_kernel(LinearArgs a, Linear
     f4 s = p[step];
 #pragma unroll 8
     for (int i = 2; i < count; ++i) {
-        s = s * seg.decays[first + (i - 1) * (int64_t)a.heads] + p[i * step];
+        // of a state that grows, 2^decays alone may pass what fp32 holds
+        const SegmentDecay d = seg.decays[first + (i - 1) * (int64_t)a.heads];
+        const f4 x = p[i * step];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = ldexpf(s[e] * d.part, d.exponent) + x[e];
         p[i * step] = s;
     }
 }

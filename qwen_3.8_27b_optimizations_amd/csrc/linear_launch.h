@@ -9,10 +9,16 @@ namespace iq4xs {
 
 struct LinearArgs;
 
+// 2^decays of a segment, times log2(e): part * 2^exponent.
+struct SegmentDecay {
+    float part;
+    int exponent;
+};
+
 // Segments of `length` tokens that sequences are cut into; with one there are no states.
 struct LinearSegments {
     float* states;  // [seqs][count][heads][dk][dv]: a sequence's own, and what each segment leaves (the first) or adds
-    float* decays;  // [seqs][count][heads] what each keeps of the state that it begins with
+    SegmentDecay* decays;  // [seqs][count][heads] what each keeps of the state that it begins with
     int count, length;
 };
 

@@ -12,6 +12,8 @@ namespace iq4xs {
 // Columns of a state that a workgroup of the kernel of chunks takes: 128 while their accumulators fit the registers.
 inline int linear_chunk_columns(int dk, int dv) { return dk == 256 || dv == 64 ? 64 : 128; }
 
+constexpr size_t SEGMENT_DECAY_BYTES = 8;
+
 struct LinearPlan {
     bool steps;           // token by token
     int segments;         // of the longest sequence
@@ -50,7 +52,7 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
         const int64_t places = g.seqs * p.segments * g.heads;
         if (g.seqs * g.heads > MOST / 64) return false;  // the launch that joins them: 1024 elements of 256 x 256 each
         p.state_bytes = (size_t)places * g.dk * g.dv * sizeof(float);
-        p.decay_bytes = ((size_t)places * sizeof(float) + 255) / 256 * 256;
+        p.decay_bytes = ((size_t)places * SEGMENT_DECAY_BYTES + 255) / 256 * 256;
     }
     return g.seqs * units <= MOST / p.segments;
 }

@@ -1,5 +1,5 @@
-"""Linear attention over the range of fp32: large keys, values, queries and states beside decays that take most of them away.
-Tolerances: linear_reference."""
+"""Linear attention over the range of fp32: large keys, values, queries and states beside decays that take most of them away,
+and states that grow.  Tolerances: linear_reference."""
 import math
 
 import pytest
@@ -56,3 +56,20 @@ def test_states_of_any_size(pkg, dev, kind, state, n):  # noqa: F811
     if n >= 100:
         p.q[n // 2:n] *= 1e4
     p.check(pkg, torch.float32)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_states_that_grow(pkg, dev, kind):  # noqa: F811
+    """By more than fp32 holds, while there is nothing or next to nothing that grows."""
+    n = 1100
+    p = Problem(dev, [n], 2, 1, 64, 64, kind, decay=torch.full((n, 2), 0.5))
+    p.states.zero_()
+    p.v[:-20] = 0
+    p.check(pkg)
+    n = 768
+    p = Problem(dev, [n], 2, 1, 64, 64, kind, decay=torch.full((n, 2), 0.4))
+    p.states.zero_()
+    p.v[:-9] = 0
+    p.v[240:256] = (1e-30 * torch.randn(16, 2, 64, device=dev)).to(p.v.dtype)
+    p.decay[512:] = 0.05
+    p.check(pkg)
