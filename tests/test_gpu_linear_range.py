@@ -1,5 +1,5 @@
 """Linear attention over the range of fp32: large keys, values, queries and states beside decays that take most of them away,
-and states that grow.  Tolerances: linear_reference."""
+states that grow, and decays that are not finite.  Tolerances: linear_reference."""
 import math
 
 import pytest
@@ -73,3 +73,20 @@ def test_states_that_grow(pkg, dev, kind):  # noqa: F811
     p.v[240:256] = (1e-30 * torch.randn(16, 2, 64, device=dev)).to(p.v.dtype)
     p.decay[512:] = 0.05
     p.check(pkg)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("n,at", [(3, 1), (31, 9), (150, 70), (150, 127), (300, 0), (900, 500), (900, 899)])
+def test_decays_that_are_not_finite(pkg, dev, kind, value, n, at):  # noqa: F811
+    """The head, from that token on; other heads, earlier tokens and other sequences keep their bits."""
+    p = Problem(dev, [n, n], 4, 2, 64, 64, kind)
+    clean, states = p.run(pkg)
+    p.decay[at, 1] = value
+    out, s = p.run(pkg)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[at:n, 1] = True
+    assert torch.equal(out[~hit], clean[~hit]) and not bool(torch.isfinite(out[hit]).any())
+    rest = torch.zeros_like(states, dtype=torch.bool)
+    rest[p.dst[0], 1] = True
+    assert torch.equal(s[~rest], states[~rest]) and not bool(torch.isfinite(s[rest]).any())
