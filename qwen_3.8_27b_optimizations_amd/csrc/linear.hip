@@ -32,7 +32,7 @@ hipError_t launch_linear_attention(const iq4xs_linear_attention_args& g, void* w
         float* states = static_cast<float*>(ws);
         static_assert(sizeof(SegmentDecay) == SEGMENT_DECAY_BYTES, "as the workspace counts them");
         const LinearSegments segments{states, reinterpret_cast<SegmentDecay*>(states + p.state_bytes / sizeof(float)),
-                                      p.segments, p.length};
+                                      p.segments, p.length, p.runs, p.kept, p.join_rows, p.grid};
         launch_linear_chunks(a, segments, g.dk, g.dv, g.in_type, stream);
     }
     return hipGetLastError();

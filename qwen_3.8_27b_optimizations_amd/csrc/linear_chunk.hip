@@ -14,9 +14,9 @@
 // - LDS holds queries once, keys and values twice: the next chunk goes in beside this one's products (where three parts
 //   have no room for that, after them).  Two waits of the workgroup for each chunk.
 // - The accumulators hold the state itself, multiplied by its decay beside the products of each chunk's update, so that what
-//   fits fp32 fits here.  (Decays kept in the scales of what is read and added, up to 2^40, save no time: 114 us either way
-//   for the 4096 tokens below; large values overflowed.)  Scales are made for as many chunks as there are waves at a time,
-//   a chunk to a wave.
+//   fits fp32 fits here.  (Decays kept in the scales of what is read and added, up to 2^40, save 2 of 116 us of the 4096
+//   tokens below, and large values overflow.)  Scales are made for as many chunks as there are waves at a time, a chunk to a
+//   wave.
 // - A long sequence is cut into segments side by side: a first pass leaves what each adds to the state, a launch joins them,
 //   and the second pass begins with the states.
 // Bound by vector instructions (parts of the state and of the weighted values: about as many issue cycles as the products
@@ -153,14 +153,15 @@ __device__ inline double running_sum(double x) {
     return plus_moved<0x143, 0xC>(x);  // and the last of 32 to the next 32
 }
 
-// 2^x where x is large: its whole part apart, so that the rest keeps its bits, and `part` in (1/2, 1].
+// 2^x where x is large: its whole part apart, so that the rest keeps its bits.
+__device__ inline float exp2_of(double x) {
+    const double whole = rint(x);
+    return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)whole);
+}
+// The same apart, `part` in (1/2, 1].
 __device__ inline SegmentDecay exp2_parts(double x) {
     const double whole = ceil(x);
     return {__builtin_amdgcn_exp2f((float)(x - whole)), (int)fmin(fmax(whole, -10000.0), 10000.0)};
-}
-__device__ inline float exp2_of(double x) {
-    const SegmentDecay d = exp2_parts(x);
-    return ldexpf(d.part, d.exponent);
 }
 
 // Four tokens of the lane's channel and the four after them, as the left or right operand of a product over tokens.
@@ -183,6 +184,22 @@ __device__ inline void store8(void* p, int type, f4 x, f4 y) {
         *static_cast<h8*>(p) = __builtin_convertvector(v, h8);
     else
         *static_cast<b8*>(p) = __builtin_convertvector(v, b8);
+}
+
+// The last sequence that begins at a place or before it, -1 if none does: a 64th of the sequences left at a time.
+// before(first row, index): whether it does, which later ones never do again.
+template <typename Before>
+__device__ inline int last_sequence(const LinearArgs& a, int lane, Before before) {
+    int seq = -1, from = 0, left = a.seqs;
+    while (left > 0) {
+        const int step = (left + 63) / 64, i = lane * step;
+        const int n = __popcll(__ballot(i < left && before(a.starts[i < left ? from + i : from], from + i)));
+        if (n == 0) break;
+        seq = from + (n - 1) * step;
+        left = min(step, from + left - seq) - 1;
+        from = seq + 1;
+    }
+    return seq;
 }
 
 // What a chunk's decays come to.
@@ -224,10 +241,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     x /= a.heads;
     const int tile = x % (dv / DVT);
     x /= dv / DVT;
-    const int part = x % seg.count, seq = x / seg.count;
-    const Rows all = rows_of(a, seq);
-    const int begin = part * seg.length;
-    if (begin >= all.count) return;
+    int seq;
+    int64_t part64;
+    Rows all;
+    if (seg.runs.rows == 0) {
+        seq = x / seg.runs.each;
+        part64 = x % seg.runs.each;
+        all = rows_of(a, seq);
+    } else {
+        seq = last_sequence(a, lane, [&](int row, int i) { return seg.runs.of(max(row, 0), i) <= x; });
+        if (seq < 0) return;
+        all = rows_of(a, seq);
+        if (all.count == 0) return;
+        part64 = x - seg.runs.of(all.first, seq);
+    }
+    if (part64 < 0 || part64 * seg.length >= all.count) return;
+    const int part = (int)part64, begin = part * seg.length;
     const bool last = all.count - begin <= seg.length;
     if (STATE_ONLY && last) return;
     const int end = last ? all.count : begin + seg.length;
@@ -251,7 +280,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         return reinterpret_cast<P>((char*)(state + (32 * s + 4 * t + r) * dv) + lane_off);
     };
     f4 S[KS][2][NT];
-    auto segment_state = [&](int i) { return seg.states + ((int64_t)(seq * seg.count + i) * a.heads + head) * DK * dv; };
+    // place of the sequence's first segment among those that are kept
+    const int64_t kept = seg.count > 1 ? seg.kept.of(all.first, seq) * a.heads + head : 0;
+    auto segment_state = [&](int i) { return seg.states + (kept + (int64_t)i * a.heads) * DK * dv; };
     // The first segment goes on from the sequence's state, in both passes: the pass over states leaves a copy of it, since
     // the last segment may write it while others begin.
     const float* from = part == 0 && (STATE_ONLY || last) ? state_at(a, a.from_slots, seq, head, DK * dv)
@@ -369,8 +400,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     };
     auto scale = [&](int chunk) {
         const int mine = chunk + C * wave;
-        // decays below -200 are zeros beside any fp32 number, and sums of them keep their bits; a NaN stays
-        const double g = running_sum(mine + lane < end ? (double)(gn < -200.0f ? -200.0f : gn) * 1.4426950408889634 : 0.0);
+        // decays below -200 are zeros beside any fp32 number, those above 200 infinities, and sums of them keep their bits; a
+        // NaN stays
+        gn = gn < -200.0f ? -200.0f : gn > 200.0f ? 200.0f : gn;
+        const double g = running_sum(mine + lane < end ? (double)gn * 1.4426950408889634 : 0.0);
         const u2 w = __builtin_bit_cast(u2, g);
         const double whole = __builtin_bit_cast(double, u2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, C - 1),
                                                            (uint32_t)__builtin_amdgcn_readlane((int)w.y, C - 1)});
@@ -626,8 +659,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     }
 
     if (STATE_ONLY && tile == 0 && threadIdx.x == 0)
-        seg.decays[(seq * seg.count + part) * (int64_t)a.heads + head] = exp2_parts(decayed);
-    float* to = STATE_ONLY ? seg.states + ((int64_t)(seq * seg.count + part + 1) * a.heads + head) * DK * dv
+        seg.decays[kept + (int64_t)part * a.heads] = exp2_parts(decayed);
+    float* to = STATE_ONLY ? segment_state(part + 1)
                 : last     ? state_at(a, a.to_slots, seq, head, DK * dv)
                            : nullptr;
     if (!to) return;
@@ -647,12 +680,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
 __global__ __launch_bounds__(256) void join_segments_kernel(LinearArgs a, LinearSegments seg, int size) {
     const int pieces = size / 4;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int piece = (int)(at % pieces), head = (int)(at / pieces % a.heads), seq = (int)(at / pieces / a.heads);
-    if (seq >= a.seqs) return;
+    const int piece = (int)(at % pieces), head = (int)(at / pieces % a.heads);
+    const int64_t which = at / pieces / a.heads, row = which * 2 * seg.length;
+    const int seq = seg.join_rows ? last_sequence(a, threadIdx.x % 64, [&](int start, int) { return start <= row; }) : (int)which;
+    if (seq < 0 || seq >= a.seqs) return;
     const Rows all = rows_of(a, seq);
     const int count = (int)((all.count + (int64_t)seg.length - 1) / seg.length);
-    if (count < 3) return;
-    const int64_t first = (int64_t)seq * seg.count * a.heads + head;
+    if (count < 3 || (seg.join_rows && row - all.first >= 2 * (int64_t)seg.length)) return;
+    const int64_t first = seg.kept.of(all.first, seq) * a.heads + head;
     f4* p = reinterpret_cast<f4*>(seg.states + first * size + 4 * piece);
     const int64_t step = (int64_t)a.heads * pieces;
     f4 s = p[step];
@@ -672,10 +707,11 @@ static void launch(const LinearArgs& a, const LinearSegments& seg, int dv, hipSt
     // 160 KiB of LDS: queries of all parts once, keys and values twice
     constexpr int ROWS = 2 * CHUNK * parts_of<T>, COLUMNS = 16 * NT * WAVES;
     constexpr bool AHEAD = ROWS * (3 * DK + 2 * COLUMNS) + 12 * 1024 <= 160 * 1024;
-    const dim3 block(64 * WAVES), grid((unsigned)((int64_t)a.seqs * seg.count * a.heads * (dv / COLUMNS)));
+    const dim3 block(64 * WAVES), grid((unsigned)seg.grid);
     if (seg.count > 1) {
         hipLaunchKernelGGL((linear_chunk_kernel<DK, NT, WAVES, T, 2, true, AHEAD>), grid, block, 0, stream, a, seg, dv);
-        const int64_t pieces = (int64_t)a.seqs * a.heads * DK * dv / 4;
+        const int64_t joins = seg.join_rows ? joining_rows(a.total, seg.length) : a.seqs;
+        const int64_t pieces = joins * a.heads * DK * dv / 4;
         hipLaunchKernelGGL(join_segments_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, a, seg, DK * dv);
     }
     hipLaunchKernelGGL((linear_chunk_kernel<DK, NT, WAVES, T, OUT, false, AHEAD>), grid, block, 0, stream, a, seg, dv);

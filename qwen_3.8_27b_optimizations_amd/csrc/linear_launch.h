@@ -17,9 +17,12 @@ struct SegmentDecay {
 
 // Segments of `length` tokens that sequences are cut into; with one there are no states.
 struct LinearSegments {
-    float* states;  // [seqs][count][heads][dk][dv]: a sequence's own, and what each segment leaves (the first) or adds
-    SegmentDecay* decays;  // [seqs][count][heads] what each keeps of the state that it begins with
+    float* states;  // [places of `kept`][heads][dk][dv]: a sequence's own, and what each segment leaves (the first) or adds
+    SegmentDecay* decays;  // [places of `kept`][heads] what each keeps of the state that it begins with
     int count, length;
+    SegmentPlaces runs, kept;
+    bool join_rows;
+    int64_t grid;
 };
 
 // units: of 32 columns of a head's state.
