@@ -13,18 +13,22 @@
 //   column: the left operand of S^T Q^T as they stand, and values read as columns serve V^T P^T and the update alike.
 // - LDS holds queries once, keys and values twice: the next chunk goes in beside this one's products (where three parts
 //   have no room for that, after them).  Two waits of the workgroup for each chunk.
-// - The accumulators hold the state itself, multiplied by its decay beside the products of each chunk's update, so that what
-//   fits fp32 fits here.  (Decays kept in the scales of what is read and added, up to 2^40, save 2 of 116 us of the 4096
-//   tokens below, and large values overflow.)  Scales are made for as many chunks as there are waves at a time, a chunk to a
-//   wave.
+// - Decays go into the accumulators as whole powers of two, which rounds nothing, with each chunk that comes to one; the rest
+//   is in the scales of what is read and added, which are 1 or less (of decays, no growth), so that what fits fp32 fits here.
+//   (Up to 2^40 in the scales saves 2 of 116 us of the 4096 tokens below, and large values overflow.  Fractions in the
+//   accumulators, without a rest: 116 us, and 7.0e-7 for 4.8e-7 of error in the states of the prompts below.)  Scales are
+//   made for as many chunks as there are waves at a time, a chunk to a wave.
 // - A long sequence is cut into segments side by side: a first pass leaves what each adds to the state, a launch joins them,
 //   and the second pass begins with the states.
 // Bound by vector instructions (parts of the state and of the weighted values: about as many issue cycles as the products
 // take) and by the chain read, multiply, exchange, multiply, wait of each chunk, with two waves to a SIMD to hide it.
-// Measured: 4096 tokens, 64 heads of 128 x 128 on 16 of q and k, bf16: 117 us (39 for the states, 10 to join them, 79), of
-// which memory takes 34; a chunk 2.1 us of a CU.  5 prompts of 987 to 4001 tokens, 32 heads of 128 x 256, fp16 to fp32: 474
-// us, 1.8 TB/s.  Slower or no faster: chunks of 64 tokens (an earlier second pass 82 us for 70: registers), one tile of
-// columns on eight waves for bf16 (77 and 79), three workgroups to a CU (87), single buffers (490 and 474 us of the prompts),
+// Measured: 4096 tokens, 64 heads of 128 x 128 on 16 of q and k, bf16: 116 us (40 for the states, 10 to join them, 80 with the
+// clock of a trace), of which memory takes 34; a chunk 2.1 us of a CU.  5 prompts of 987 to 4001 tokens, 32 heads of 128 x
+// 256, fp16 to fp32: 471 us, 1.85 TB/s.  One prompt of 4096 tokens beside 63 single ones, bf16: 216 us for 138 of memory.
+// Of fp16, 64 columns on four waves, two workgroups to a CU: 469 for 481 us of the prompts before, but 131 for 116 of 4 x 1024
+// tokens.
+// Slower or no faster: chunks of 64 tokens (an earlier second pass 82 us for 70: registers), one tile of columns on eight
+// waves for bf16 (77 and 79), three workgroups to a CU (87), single buffers (490 and 474 us of the prompts, earlier),
 // scales by one wave a chunk ahead (as fast alone, but the pass over states waits for it), fp16 inputs as they are with
 // the state in fp16's range (500 us: keeping the range costs what the parts do), sums of earlier segments in each
 // workgroup instead of a launch that joins (96 against 64 + 12 us).
@@ -206,9 +210,9 @@ __device__ inline int last_sequence(const LinearArgs& a, int lane, Before before
 template <int C>
 struct ChunkScales {
     double sum[C];        // of decays up to a token, times log2(e)
-    float from_start[C];  // of the state in an output: 2^sum and the output's scale
-    float to_end[C];      // of a token in the state: 2^(whole - sum)
-    float whole;          // of the state before the chunk's tokens come to it: 2^whole
+    float from_start[C];  // of the accumulators in an output: 2^sum, the output's scale, and 2^held as the chunk begins
+    float to_end[C];      // of a token in the accumulators: 2^(whole - sum), and 2^-held as the chunk ends
+    float by;             // power of two that the accumulators go down by before the chunk's tokens come to them
 };
 
 // DK by 16 NT WAVES of a head's state belong to a workgroup, 16 NT columns to a wave, in accumulators.  OUT: parts of the
@@ -219,6 +223,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     constexpr int C = CHUNK, IN = parts_of<T>, KS = DK / 32, IT = C / 16, DVT = 16 * NT * WAVES, THREADS = 64 * WAVES;
     // products of parts p and o count while p + o is below OUT
     constexpr int BUFFERS = AHEAD ? 2 : 1;
+    // whether the accumulators are multiplied beside the products of their update, every time, or before them, where there is
+    // something to do: 2048 tokens of 32 heads of 256 x 256, fp16 258 and 263 us, fp32 333 and 341; 5 prompts of 128 x 256,
+    // fp16 479 and 471, 4096 tokens of 128 x 128, bf16 118 and 117
+    constexpr bool DECAY_BESIDE = KS * IN >= 16;
     using KTile = ChunkTile<C, DK>;
     using VTile = ChunkTile<C, DVT>;
     using PTile = ChunkTile<C, C>;
@@ -230,6 +238,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     __shared__ __attribute__((aligned(1024))) uint8_t vs[BUFFERS * V_BYTES];
     __shared__ __attribute__((aligned(1024))) uint8_t ps[STATE_ONLY ? 1024 : OUT * PTile::BYTES];
     __shared__ ChunkScales<C> scales[WAVES];  // of as many chunks at a time
+    __shared__ double wholes[WAVES];
     __shared__ int odd[2], odd_from[2][DVT];  // whether values are not finite, and a channel's first token of such
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int n = lane % 16, j = lane / 16;
@@ -390,8 +399,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         }
     };
 
-    // The scales of the next chunks, one to a wave (scanning the decays of one chunk after another would keep the other
-    // waves waiting for the one that does).
+    // What the accumulators hold is the state times 2^-rest, the rest of the segment's decays over whole powers of two: these go
+    // into the accumulators, which rounds nothing, and the rest, in [0, 1), into the scales of what is read and added.  The
+    // scales of the next chunks, one to a wave (scanning the decays of one chunk after another would keep the other waves
+    // waiting for the one that does).
+    double decayed = 0.0;  // the segment's decays up to the next scales, times log2(e)
     float gn;
     auto decays = [&](int chunk) {  // of the wave's chunk of those from `chunk` on, ahead of their use
         const int i = chunk + C * wave + lane % C;
@@ -400,23 +412,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
     };
     auto scale = [&](int chunk) {
         const int mine = chunk + C * wave;
-        // decays below -200 are zeros beside any fp32 number, those above 200 infinities, and sums of them keep their bits; a
-        // NaN stays
-        gn = gn < -200.0f ? -200.0f : gn > 200.0f ? 200.0f : gn;
+        // decays below -200 are zeros beside any fp32 number, those above 200 infinities, and sums of them keep their bits;
+        // what is not finite stays
+        gn = gn < -200.0f ? -200.0f : gn > 200.0f && gn <= FLT_MAX ? 200.0f : gn;
         const double g = running_sum(mine + lane < end ? (double)gn * 1.4426950408889634 : 0.0);
-        const u2 w = __builtin_bit_cast(u2, g);
-        const double whole = __builtin_bit_cast(double, u2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, C - 1),
-                                                           (uint32_t)__builtin_amdgcn_readlane((int)w.y, C - 1)});
+        if (lane == C - 1) wholes[wave] = g;
+        __syncthreads();
+        double before = decayed;  // the wave's chunk
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            const double x = wholes[i];
+            if (i < wave) before += x;
+            decayed += x;
+        }
+        const double whole = wholes[wave], after = before + whole, from = floor(before), down = floor(after);
         ChunkScales<C>& to = scales[wave];
         if (lane < C) {
             to.sum[lane] = g;
-            to.from_start[lane] = exp2_of(g) * a.scale;
-            to.to_end[lane] = exp2_of(whole - g);
+            to.from_start[lane] = exp2_of(g + (before - from)) * a.scale;
+            to.to_end[lane] = exp2_of(whole - g - (after - down));
         }
-        if (lane == 0) to.whole = exp2_of(whole);
+        if (lane == 0) to.by = ldexpf(1.0f, (int)(down - from));
         decays(chunk + C * WAVES);
     };
-    double decayed = 0.0;  // sum of the segment's decays so far, times log2(e)
 
     const uint32_t out_bytes = a.out_type == IQ4XS_TYPE_F32 ? 4 : 2;
     for (int i = threadIdx.x; i < 2 * DVT; i += THREADS) odd_from[i / DVT][i % DVT] = C;
@@ -452,7 +470,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         }
         f4 O[IT][NT];
         if constexpr (!STATE_ONLY) {
-            // weighted scores of tiles on and below the diagonal: keys 16 kt + 4 j + r of query 16 it + n
+            // weighted scores of tiles on and below the diagonal: keys 16 kt + 4 j + r of query 16 it + n; weights below 2^-126
+            // are zeros
             if (wave < 3) {
                 const int it = wave > 0, kt = wave > 1;
                 f4 z{0, 0, 0, 0};
@@ -552,8 +571,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
             for (int p = 0; p < IN; ++p) V[u][p] = eight_tokens<VTile>(v_column + v_buffer + 8 * u + p * VTile::BYTES);
         const bool some_odd = odd[parity] != 0;
         float w[8];
-        const float whole = sc.whole;
-        if constexpr (STATE_ONLY) decayed += sc.sum[C - 1];
+        const float by = sc.by;
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = sc.to_end[8 * j + e];
         u4 y[IT][OUT];
@@ -580,8 +598,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int u = 0; u < NT; ++u) S[s][h][u] *= whole;
+                for (int u = 0; u < NT; ++u) S[s][h][u] *= by;
         };
+        if (!DECAY_BESIDE && by != 1.0f) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) decay(s);
+        }
         // values times what is left of them at the chunk's end, and the state's update
         u4 W[NT][3];
 #pragma unroll
@@ -603,8 +625,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
         for (int s = 0; s < KS; ++s) {
             if (s + 1 < KS) keys(s + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (s == 0) decay(0);
-            if (s + 1 < KS) decay(s + 1);
+            if (DECAY_BESIDE && s == 0) decay(0);
+            if (DECAY_BESIDE && s + 1 < KS) decay(s + 1);
 #pragma unroll
             for (int o = 2; o >= 0; --o)
 #pragma unroll
@@ -664,6 +686,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
                 : last     ? state_at(a, a.to_slots, seq, head, DK * dv)
                            : nullptr;
     if (!to) return;
+    const float rest = exp2_of(decayed - floor(decayed));
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -672,7 +695,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunk_kernel(LinearArgs 
             for (int u = 0; u < NT; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    *state_place(to, s, t, u, r) = S[s][t][u][r];
+                    *state_place(to, s, t, u, r) = S[s][t][u][r] * rest;
 }
 
 // The states that segments begin with, in the place of what each adds, from the third on.  Bound by memory: 16 bytes read and
