@@ -375,8 +375,12 @@ struct SharedPlan {
 // Once costs two more launches, each sequence by itself reads shared keys again, though from caches that hold them: 8 heads of
 // 128, one token each, fp16, 4096 shared tokens, 8, 16 and 32 sequences 29, 32, 37 us once and 21, 34, 56 each; 16384, 2, 4
 // and 64 sequences 26, 28, 74 and 22, 34, 317; 8 bits 4 heads of 256, 4 tokens each, 4096, 16 and 32 sequences 77, 81 and 66,
-// 117: from 2^26 elements of keys read again on.  Full tiles of rows are bound by their products, of which there are no
-// fewer (64 tokens of 64 heads, 16384, 8 and 16 sequences 246, 456 and 238, 444).
+// 117: from 2^26 elements of keys read again on.  Between 2^25 and 2^26 the sides differ by type (4 fp16 sequences behind 16384
+// 28 once and 34 each, but 16 of 8 bits behind 4096 42 and 32), and there is no third launch each by itself.
+// 128 rows of a sequence and head on each: the products bound such calls, of which there are no fewer, but those of a last tile
+// that is hardly used (64 tokens of 64 heads on 8, fp16, 16384 shared: 4, 8 and 16 sequences 179, 331, 630 once and 166, 311,
+// 585 each; 24 tokens, 192 rows, 95, 162, 285 and 95, 171, 297; 17 tokens, 136 rows, 80, 127, 204 and 89, 162, 287; behind
+// 4096 tokens 17 take 51, 66, 79 and 41, 63, 89).  A caller that knows such rows says so by `path`.
 inline bool shared_once(const iq4xs_paged_attention_args& g, const iq4xs_shared_prefix& x) {
     if (x.path != IQ4XS_SHARED_AUTO) return x.path == IQ4XS_SHARED_ONCE;
     const int64_t most_q = g.most_q < g.total ? g.most_q : g.total;

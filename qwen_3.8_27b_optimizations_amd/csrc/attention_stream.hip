@@ -28,8 +28,8 @@
 // two taken out of each row, exact down to 2^-14 of the row's largest element.
 //
 // First tokens beside a window are further steps before those of the window, of the first split, with masks of their own: 64
-// sequences of up to 32768 tokens, window 4096, 4 first tokens, 64 heads on 8 of 128, bf16: 155 us, 5.2 TB/s; 8 x 5 tokens
-// over a window of 2048 and 64 first tokens, 8-bit heads of 256: 37 us.
+// sequences of up to 32768 tokens, window 4096, 4 first tokens, 64 heads on 8 of 128, bf16: 157 us of a call's 168 (4.8 TB/s
+// of the call); 8 x 5 tokens over a window of 2048 and 64 first tokens, 8-bit heads of 256: 35 of 39 us.
 #include "attention_core.h"
 #include "attention_internal.h"
 #include "iq4xs_internal.h"

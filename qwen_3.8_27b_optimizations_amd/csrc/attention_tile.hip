@@ -28,8 +28,8 @@
 // 1517 and 2603); the kernel of few rows takes 2428 (2911, 4960).
 //
 // First tokens beside a window are further tiles before those of the window, in the first split: 2048 tokens at the end of
-// 16384, window 4096, 16 first tokens, fp16: 313 to 319 us, 870 TFLOP/s.  The rows of all sequences behind a shared prefix
-// are one sequence's that sees all of it: 64 tokens of 64 sequences over 16384 shared keys 50 us, 690 TFLOP/s.
+// 16384, window 4096, 16 first tokens, fp16: 317 to 320 us, 865 TFLOP/s.  The rows of all sequences behind a shared prefix
+// are one sequence's that sees all of it: the next tokens of 64 sequences over 16384 shared keys 50 us, 690 TFLOP/s.
 #include <type_traits>
 
 #include "attention_core.h"

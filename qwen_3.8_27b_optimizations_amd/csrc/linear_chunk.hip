@@ -14,21 +14,20 @@
 // - LDS holds queries once, keys and values twice: the next chunk goes in beside this one's products (where three parts
 //   have no room for that, after them).  Two waits of the workgroup for each chunk.
 // - Decays go into the accumulators as whole powers of two, which rounds nothing, with each chunk that comes to one; the rest
-//   is in the scales of what is read and added, which are 1 or less (of decays, no growth), so that what fits fp32 fits here.
-//   (Up to 2^40 in the scales saves 2 of 116 us of the 4096 tokens below, and large values overflow.  Fractions in the
+//   is in the scales of what is read and added, so that the accumulators never hold more than the state.
+//   (Up to 2^40 in the scales saves 3 of 117 us of the 4096 tokens below, and large values overflow.  Fractions in the
 //   accumulators, without a rest: 116 us, and 7.0e-7 for 4.8e-7 of error in the states of the prompts below.)  Scales are
 //   made for as many chunks as there are waves at a time, a chunk to a wave.
 // - A long sequence is cut into segments side by side: a first pass leaves what each adds to the state, a launch joins them,
 //   and the second pass begins with the states.
 // Bound by vector instructions (parts of the state and of the weighted values: about as many issue cycles as the products
 // take) and by the chain read, multiply, exchange, multiply, wait of each chunk, with two waves to a SIMD to hide it.
-// Measured: 4096 tokens, 64 heads of 128 x 128 on 16 of q and k, bf16: 116 us (40 for the states, 10 to join them, 80 with the
-// clock of a trace), of which memory takes 34; a chunk 2.1 us of a CU.  5 prompts of 987 to 4001 tokens, 32 heads of 128 x
-// 256, fp16 to fp32: 471 us, 1.85 TB/s.  One prompt of 4096 tokens beside 63 single ones, bf16: 216 us for 138 of memory.
-// Of fp16, 64 columns on four waves, two workgroups to a CU: 469 for 481 us of the prompts before, but 131 for 116 of 4 x 1024
-// tokens.
-// Slower or no faster: chunks of 64 tokens (an earlier second pass 82 us for 70: registers), one tile of columns on eight
-// waves for bf16 (77 and 79), three workgroups to a CU (87), single buffers (490 and 474 us of the prompts, earlier),
+// Measured: 4096 tokens, 64 heads of 128 x 128 on 16 of q and k, bf16: 117 us (traced 40 for the states, 10 to join them, 80),
+// of which memory takes 34; a chunk 2.1 us of a CU.  5 prompts of 987 to 4001 tokens, 32 heads of 128 x 256, fp16 to fp32:
+// 471 us, 1.85 TB/s.  One prompt of 4096 tokens beside 63 single ones, bf16: 217 us for 138 of memory.
+// Slower or no faster: 64 columns of fp16 on four waves, two workgroups to a CU (473 and 474 us of the prompts, 131 and 116 of
+// 4 x 1024 tokens), chunks of 64 tokens (an earlier second pass 82 us for 70: registers), one tile of columns on
+// eight waves for bf16 (77 and 79), three workgroups to a CU (87), single buffers (490 and 474 us of the prompts, earlier),
 // scales by one wave a chunk ahead (as fast alone, but the pass over states waits for it), fp16 inputs as they are with
 // the state in fp16's range (500 us: keeping the range costs what the parts do), sums of earlier segments in each
 // workgroup instead of a launch that joins (96 against 64 + 12 us).

@@ -65,15 +65,17 @@ inline bool linear_plan(const iq4xs_linear_attention_args& g, int64_t cus, Linea
     p.length = (int)(most < MOST - 63 ? (most + 63) / 64 * 64 : MOST);  // one segment: as long as any sequence
     if (g.seqs > MOST / g.heads / 8) return false;  // 32 columns of 256 at a time
     p.units = g.seqs * g.heads * (g.dv / 32);
-    // Token by token while that is no slower: a chunk's work hardly grows with its tokens, a step's does (64 sequences of 64
-    // heads of 128 x 128, of 4, 8 and 16 tokens: bf16 115, 153 and 239 us in steps and 111, 113 and 117 in a chunk, fp16 111,
-    // 153, 237 and 158, 161, 163, fp32 124, 169, 268 and 179, 183, 195; one sequence 10, 11, 18 and 11 to 14).
+    // Token by token while that is no slower: a chunk's work hardly grows with its tokens, a step's does (64 heads of 128 x
+    // 128, steps and chunks in turn.  64 sequences of 4, 5, 8 and 16 tokens: bf16 114, 125, 154, 238 us and 113, 113, 114, 118;
+    // fp16 111, 122, 154, 236 and 155, 155, 156, 159; fp32 124, 135, 169, 268 and 175, 176, 180, 190.  8 sequences of 4, 5 and
+    // 8: bf16 17, 18, 22 and 17, 18, 18; of 5, 8 and 12: fp16 18, 22, 27 and 23, 23, 23.  One of 5 and 8: bf16 11, 11 and 11,
+    // 11; of 8 and 12: fp16 11, 14 and 11, 11.  Between, 4 of 8 fp16 tokens lose 3 us: 14 and 11).
     if (most <= (g.in_type == IQ4XS_TYPE_BF16 ? 4 : 8)) return true;
     p.steps = false;
     // Segments: as long as makes work for the workgroups that the CUs hold at once, two each of bf16 inputs and one of others,
-    // whose parts fill LDS, and none less than 256 tokens (4096 tokens of 64 heads, bf16: 8 segments 117 us, 4 160, 11 153).
+    // whose parts fill LDS, and none less than 256 tokens (4096 tokens of 64 heads, bf16: 8 segments 117 us, 4 147, 11 135).
     // Their states cost half of the work again, so only where the longest sequence would take half as long again as that
-    // (5 prompts of 987 to 4001 tokens, fp16: 474 us whole, 660 in up to 3 segments).
+    // (5 prompts of 987 to 4001 tokens, fp16: 471 us whole, 664 in up to 2 segments).
     const int64_t units = g.heads * (g.dv / linear_chunk_columns(g.dk, g.dv));
     const int64_t slots = (g.in_type == IQ4XS_TYPE_BF16 ? 2 : 1) * cus;
     int64_t length = (g.total * units + slots - 1) / slots;
